@@ -71,6 +71,45 @@ class WsView(ctypes.Structure):
                 ("tc_slots", ctypes.c_uint32), ("max_tc", ctypes.c_uint32)]
 
 
+class KvDesc(ctypes.Structure):
+    """pulsar_kv_desc (include/pulsar_kv.h)."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("table", ctypes.c_void_p),
+                ("k_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p),
+                ("page_stride", ctypes.c_uint64), ("head_stride", ctypes.c_uint64), ("tok_stride", ctypes.c_uint64),
+                ("table_stride", ctypes.c_uint64),
+                ("n_pages", ctypes.c_uint32), ("page_size", ctypes.c_uint32), ("n_kv", ctypes.c_uint32),
+                ("head_dim", ctypes.c_uint32), ("n_rows", ctypes.c_uint32), ("max_pages", ctypes.c_uint32),
+                ("dtype", ctypes.c_uint32)]
+
+
+class KvAppendArgs(ctypes.Structure):
+    """pulsar_kv_append_args."""
+    _fields_ = [("q", ctypes.c_void_p), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("q_out", ctypes.c_void_p),
+                ("seq", ctypes.c_void_p), ("pos", ctypes.c_void_p), ("cos_sin", ctypes.c_void_p),
+                ("q_stride", ctypes.c_uint64), ("k_stride", ctypes.c_uint64), ("v_stride", ctypes.c_uint64),
+                ("q_out_stride", ctypes.c_uint64),
+                ("n_tok", ctypes.c_uint32), ("n_head", ctypes.c_uint32), ("rot_dim", ctypes.c_uint32),
+                ("n_pos", ctypes.c_uint32), ("x_type", ctypes.c_uint32), ("q_out_type", ctypes.c_uint32),
+                ("interleaved", ctypes.c_uint32)]
+
+
+class KvAttendArgs(ctypes.Structure):
+    """pulsar_kv_attend_args."""
+    _fields_ = [("q", ctypes.c_void_p), ("out", ctypes.c_void_p), ("lse", ctypes.c_void_p),
+                ("lens", ctypes.c_void_p), ("seq", ctypes.c_void_p), ("sinks", ctypes.c_void_p),
+                ("q_stride", ctypes.c_uint64), ("out_stride", ctypes.c_uint64), ("scale", ctypes.c_float),
+                ("n_rows", ctypes.c_uint32), ("n_q", ctypes.c_uint32), ("n_head", ctypes.c_uint32),
+                ("window", ctypes.c_uint32), ("q_type", ctypes.c_uint32)]
+
+
+class KvPoolDesc(ctypes.Structure):
+    """pulsar_kv_pool."""
+    _fields_ = [("table", ctypes.c_void_p), ("len", ctypes.c_void_p), ("refs", ctypes.c_void_p),
+                ("data", ctypes.c_void_p), ("slab_stride", ctypes.c_uint64), ("page_bytes", ctypes.c_uint64),
+                ("table_stride", ctypes.c_uint64), ("n_rows", ctypes.c_uint32), ("max_pages", ctypes.c_uint32),
+                ("n_pages", ctypes.c_uint32), ("page_size", ctypes.c_uint32), ("n_slab", ctypes.c_uint32)]
+
+
 # (name, argtypes) of every C entry point, in header order
 _P, _U32, _U64, _F = ctypes.c_void_p, ctypes.c_uint32, ctypes.c_uint64, ctypes.c_float
 _SIGS = {
@@ -95,6 +134,11 @@ _SIGS = {
     "pulsar_moe_layer_ws_view": [ctypes.POINTER(LayerDesc), _U32, _P, ctypes.POINTER(WsView)],
     "pulsar_quantize_rows": [_P, _P, _P, _U32, _U64, _U32, _P],
     "pulsar_repack_q2k_tiles": [_P, _P, _U32, _U32, _U32, _U64, _U64, _P],
+    "pulsar_kv_append": [ctypes.POINTER(KvDesc), ctypes.POINTER(KvAppendArgs), _P],
+    "pulsar_kv_attend": [ctypes.POINTER(KvDesc), ctypes.POINTER(KvAttendArgs), _P, ctypes.c_size_t, _P],
+    "pulsar_kv_grow": [ctypes.POINTER(KvPoolDesc), _P, _P, _U32, _P, _P, ctypes.c_size_t, _P],
+    "pulsar_kv_fork": [ctypes.POINTER(KvPoolDesc), _P, _P, _U32, _P, _P, ctypes.c_size_t, _P],
+    "pulsar_kv_compact": [ctypes.POINTER(KvPoolDesc), _P, _P, ctypes.c_size_t, _P],
 }
 
 
@@ -132,6 +176,12 @@ def lib() -> ctypes.CDLL:
         L.pulsar_row_bytes.restype = _U64
         L.pulsar_b200_abi_error.argtypes = []
         L.pulsar_b200_abi_error.restype = _U32
+        L.pulsar_kv_attend_workspace.argtypes = [ctypes.POINTER(KvDesc), ctypes.POINTER(KvAttendArgs)]
+        L.pulsar_kv_attend_workspace.restype = ctypes.c_size_t
+        L.pulsar_kv_pool_workspace.argtypes = [ctypes.POINTER(KvPoolDesc), _U32]
+        L.pulsar_kv_pool_workspace.restype = ctypes.c_size_t
+        L.pulsar_kv_error.argtypes = []
+        L.pulsar_kv_error.restype = _U32
         _LIB = L
     return _LIB
 
