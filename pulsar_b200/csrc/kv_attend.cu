@@ -1,109 +1,81 @@
-/* kv_attend.cu - attention of new tokens over a paged cache.
- *
- *   o = sum_j e^(s_j - m) v_j / (sum_j e^(s_j - m) + e^(sink - m)),  s_j = scale q.k_j
- * One warp per (token, query head); lanes hold 8 values of the head each,
- * the keys pass once with the running maximum and sum. */
-#include "pk_common.h"
+/* kv_attend.cu - attention over a paged cache: arguments, the choice of a
+ * kernel, the workspace (the kernels are in pk_attend.cuh). */
+#include "pk_attend.cuh"
 
-template <uint32_t T>
-__device__ __forceinline__ float pk_get(const void *p, uint64_t at) {
-    return pk_type<T>::get(((const typename pk_type<T>::t *)p)[at]);
-}
+/* what a call's sizes settle */
+struct pk_attend_plan {
+    int dp, mt;              /* padded head width; 8-row tiles a CTA takes together */
+    bool three;
+    uint32_t workers, least;
+    size_t counters, bytes;  /* of the workspace */
+};
 
-template <uint32_t Q, uint32_t C>
-__global__ void __launch_bounds__(32) pk_attend_kernel(const pulsar_kv_desc D, const pulsar_kv_attend_args A,
-                                                       uint32_t *err) {
-    const uint32_t lane = threadIdx.x, h = blockIdx.y, hk = h / (A.n_head / D.n_kv);
-    const uint32_t b = blockIdx.x / A.n_q, i = blockIdx.x % A.n_q;
-    const int32_t row = A.seq ? A.seq[b] : (int32_t)b;
-    int64_t len = A.lens[b];
-    if (row < 0 || len < 0) len = 0;
-    else if ((uint32_t)row >= D.n_rows) {
-        if (lane == 0) atomicOr(err, PULSAR_KV_ERR_ROW);
-        len = 0;
-    }
-    if (len > (int64_t)D.max_pages * D.page_size) {
-        if (lane == 0) atomicOr(err, PULSAR_KV_ERR_SPAN);
-        len = (int64_t)D.max_pages * D.page_size;
-    }
-    const int64_t hi = len - (int64_t)(A.n_q - 1 - i), lo = A.window && hi > A.window ? hi - A.window : 0;
-    const float ks = D.k_scale ? D.k_scale[hk] : 1.0f, vs = D.v_scale ? D.v_scale[hk] : 1.0f;
-    float q[8], o[8];
-    const uint64_t at = blockIdx.x * A.q_stride + (uint64_t)h * D.head_dim;
-    for (int x = 0; x < 8; x++) {
-        const uint32_t c = lane + 32 * x;
-        q[x] = c < D.head_dim ? pk_get<Q>(A.q, at + c) * A.scale * ks : 0.0f;
-        o[x] = 0.0f;
-    }
-    float m = -INFINITY, l = 0.0f;
-    for (int64_t j = lo; j < hi; j++) {
-        const int32_t page = D.table[(uint64_t)row * D.table_stride + j / D.page_size];
-        if ((uint32_t)page >= D.n_pages) {
-            if (lane == 0) atomicOr(err, PULSAR_KV_ERR_PAGE);
-            continue;
-        }
-        const uint64_t e = (uint64_t)page * D.page_stride + hk * D.head_stride + (j % D.page_size) * D.tok_stride;
-        float s = 0.0f;
-        for (int x = 0; x < 8; x++)
-            if (lane + 32 * x < D.head_dim) s += q[x] * pk_get<C>(D.k, e + lane + 32 * x);
-        for (int w = 16; w; w >>= 1) s += __shfl_xor_sync(~0u, s, w);
-        const float m2 = fmaxf(m, s), base = m2 == -INFINITY ? 0.0f : m2;
-        const float keep = expf(m - base), p = expf(s - base);
-        m = m2;
-        l = l * keep + p;
-        for (int x = 0; x < 8; x++)
-            o[x] = o[x] * keep +
-                   (lane + 32 * x < D.head_dim ? p * pk_get<C>(D.v, e + lane + 32 * x) : 0.0f);
-    }
-    const bool empty = hi <= lo;
-    if (A.sinks && !empty) {
-        const float m2 = fmaxf(m, A.sinks[h]), keep = expf(m - m2);
-        l = l * keep + expf(A.sinks[h] - m2);
-        for (int x = 0; x < 8; x++) o[x] *= keep;
-        m = m2;
-    }
-    typedef typename pk_type<Q>::t T;
-    T *out = (T *)A.out + blockIdx.x * A.out_stride + (uint64_t)h * D.head_dim;
-    for (int x = 0; x < 8; x++)
-        if (lane + 32 * x < D.head_dim) out[lane + 32 * x] = pk_type<Q>::put(l > 0.0f || isnan(l) ? o[x] * vs / l : 0.0f);
-    if (A.lse && lane == 0)
-        A.lse[(uint64_t)blockIdx.x * A.n_head + h] = empty ? -INFINITY : logf(l) + m;
+static int pk_attend_prepare(const pulsar_kv_desc *d, const pulsar_kv_attend_args *a, pk_attend_job *J,
+                             pk_attend_plan *p) {
+    const char *f = pk_desc_fault(d);
+    if (f) return pk_refuse(f);
+    if (!a) return pk_refuse("kv attend: null arguments");
+    if (a->q_type > PULSAR_TYPE_F16) return pk_refuse("kv attend: values are f32, bf16 or f16");
+    if (!a->n_head || a->n_head > 0xffffu || a->n_head % d->n_kv)
+        return pk_refuse("kv attend: n_head is a multiple of n_kv, at most 65535");
+    if (!a->n_rows || !a->n_q || (uint64_t)a->n_rows * a->n_q > 0x7fffffffull ||
+        (uint64_t)a->n_q * a->n_head > 0x7fffffffull)
+        return pk_refuse("kv attend: between 1 and 2^31 - 1 tokens");
+    J->D = *d;
+    J->A = *a;
+    J->group = a->n_head / d->n_kv;
+    J->rows = a->n_q * J->group;
+    p->dp = d->head_dim <= 64 ? 64 : d->head_dim <= 128 ? 128 : 256;
+    /* 16 query rows share one reading of the keys where there are that many;
+     * at 256 columns their output tiles would not fit the registers */
+    p->mt = J->rows > 8 && p->dp <= 128 ? 2 : 1;
+    /* two bf16 parts hold bf16 exactly; wider q wants three for f32 results */
+    p->three = d->dtype == PULSAR_TYPE_BF16 && a->q_type != PULSAR_TYPE_BF16;
+    J->tiles = (J->rows + 8 * p->mt - 1) / (8 * p->mt);
+    if ((uint64_t)J->tiles * d->n_kv > 0x7fffffffull) return pk_refuse("kv attend: too many heads and tokens");
+    J->segs = J->tiles * d->n_kv;
+    J->page_shift = -1;
+    for (int s = 0; s < 31; s++)
+        if (d->page_size == 1u << s) J->page_shift = s;
+    const uint32_t elt = pk_type_bytes(d->dtype), ck = (uint32_t)p->dp * elt >= 256 ? 16 : 32;
+    J->least = p->least = 128 / ck;
+    /* CTAs that are resident together: shared memory holds two, one at 256 columns */
+    p->workers = pk_sm_count() * (p->dp == 256 ? 1 : 2);
+    if (p->workers > PK_MAX_WORKERS) p->workers = PK_MAX_WORKERS;
+    /* no more CTAs than the longest rows could feed */
+    uint64_t keys = (uint64_t)d->max_pages * d->page_size;
+    if (a->window && keys > (uint64_t)a->window + a->n_q - 1) keys = (uint64_t)a->window + a->n_q - 1;
+    const uint64_t most = (uint64_t)a->n_rows * J->segs * (keys / ck + 2);
+    if (p->workers > most) p->workers = (uint32_t)most;
+    p->counters = 4ull * 2 * 2 * PK_MAX_WORKERS;
+    p->bytes = PULSAR_KV_WS_ZEROED + 4ull * p->workers * 2 * 8 * p->mt * (p->dp + 2);
+    return 1;
 }
+static_assert(4 * 2 * 2 * PK_MAX_WORKERS <= PULSAR_KV_WS_ZEROED, "the counters are in the zeroed bytes");
 
 extern "C" size_t pulsar_kv_attend_workspace(const pulsar_kv_desc *d, const pulsar_kv_attend_args *a) {
-    return pk_desc_fault(d) || !a ? 0 : PULSAR_KV_WS_ZEROED;
-}
-
-template <uint32_t Q>
-static int pk_attend_by_cache(const pulsar_kv_desc *d, const pulsar_kv_attend_args *a, cudaStream_t st) {
-    const dim3 grid(a->n_rows * a->n_q, a->n_head);
-    if (d->dtype == PULSAR_TYPE_BF16)
-        pk_attend_kernel<Q, PULSAR_TYPE_BF16><<<grid, 32, 0, st>>>(*d, *a, pk_err_word());
-    else if (d->dtype == PULSAR_TYPE_F16)
-        pk_attend_kernel<Q, PULSAR_TYPE_F16><<<grid, 32, 0, st>>>(*d, *a, pk_err_word());
-    else
-        pk_attend_kernel<Q, PULSAR_TYPE_E4M3><<<grid, 32, 0, st>>>(*d, *a, pk_err_word());
-    return pm_ok(cudaGetLastError(), "kv attend launch");
+    pk_attend_job J;
+    pk_attend_plan p;
+    return pk_attend_prepare(d, a, &J, &p) ? p.bytes : 0;
 }
 
 extern "C" int pulsar_kv_attend(const pulsar_kv_desc *d, const pulsar_kv_attend_args *a, void *ws, size_t ws_bytes,
                                 void *stream) {
-    const char *f = pk_desc_fault(d);
-    if (f) return pk_refuse(f);
-    if (!a || !a->q || !a->out || !a->lens || !ws) return pk_refuse("kv attend: null arguments");
-    if (a->q_type > PULSAR_TYPE_F16) return pk_refuse("kv attend: values are f32, bf16 or f16");
-    if (!a->n_head || a->n_head > 0xffffu || a->n_head % d->n_kv)
-        return pk_refuse("kv attend: n_head is a multiple of n_kv, at most 65535");
-    if (!a->n_rows || !a->n_q || (uint64_t)a->n_rows * a->n_q > 0x7fffffffull)
-        return pk_refuse("kv attend: between 1 and 2^31 - 1 tokens");
+    pk_attend_job J;
+    pk_attend_plan p;
+    if (!pk_attend_prepare(d, a, &J, &p)) return 0;
+    if (!a->q || !a->out || !a->lens || !ws || ((uintptr_t)ws & 15u)) return pk_refuse("kv attend: null arguments");
     if (!a->seq && a->n_rows > d->n_rows) return pk_refuse("kv attend: more rows than the table has");
     const uint64_t w = (uint64_t)a->n_head * d->head_dim;
     if ((uint64_t)a->n_rows * a->n_q > 1 && (a->q_stride < w || a->out_stride < w))
         return pk_refuse("kv attend: tokens overlap");
-    if (ws_bytes < pulsar_kv_attend_workspace(d, a)) return pk_refuse("kv attend: workspace too small");
-    if (!pk_err_word()) return pk_refuse("kv: no error word on this device");
-    const cudaStream_t st = pk_stream(stream);
-    if (a->q_type == PULSAR_TYPE_F32) return pk_attend_by_cache<PULSAR_TYPE_F32>(d, a, st);
-    if (a->q_type == PULSAR_TYPE_BF16) return pk_attend_by_cache<PULSAR_TYPE_BF16>(d, a, st);
-    return pk_attend_by_cache<PULSAR_TYPE_F16>(d, a, st);
+    if (ws_bytes < p.bytes) return pk_refuse("kv attend: workspace too small");
+    J.counters = (uint32_t *)ws;
+    J.parts = (float *)((uint8_t *)ws + PULSAR_KV_WS_ZEROED);
+    J.err = pk_err_word();
+    if (!J.err) return pk_refuse("kv: no error word on this device");
+    const pk_attend_fn f = d->dtype == PULSAR_TYPE_BF16  ? pk_attend_bf16(p.dp, p.mt, p.three)
+                           : d->dtype == PULSAR_TYPE_F16 ? pk_attend_f16(p.dp, p.mt, p.three)
+                                                         : pk_attend_e4m3(p.dp, p.mt, p.three);
+    return f(J, p.workers, pk_stream(stream));
 }

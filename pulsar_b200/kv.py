@@ -218,11 +218,12 @@ class PagedKv:
         a.scale = D ** -0.5 if scale is None else scale
         a.n_rows, a.n_q, a.n_head, a.window, a.q_type = n, n_q, n_head, window, TYPES[q.dtype]
         if ws is None:
-            if self._sized != (n, n_q, n_head, a.q_type):
+            size = (n, n_q, n_head, a.q_type, window)
+            if self._sized != size:
                 need = self.workspace_bytes()
                 if self._ws is None or self._ws.numel() < need:
                     self._ws = torch.zeros(need, dtype=torch.uint8, device=dev)
-                self._sized = (n, n_q, n_head, a.q_type)
+                self._sized = size
             ws = self._ws
         check(self._lib.pulsar_kv_attend(self._pdesc, self._pargs, ws.data_ptr(), ws.numel(), _stream(stream)),
               "kv_attend")
