@@ -4,10 +4,10 @@
 
 /* what a call's sizes settle */
 struct pk_attend_plan {
-    int dp, mt;              /* padded head width; 8-row tiles a CTA takes together */
-    bool three;
-    uint32_t workers, least;
-    size_t counters, bytes;  /* of the workspace */
+    int dp, r, mt;           /* padded head width; the kernel's R and MT */
+    bool wide;               /* q has more bits than one 16-bit part of the cache's kind holds */
+    uint32_t workers;
+    size_t bytes;            /* of the workspace */
 };
 
 static int pk_attend_prepare(const pulsar_kv_desc *d, const pulsar_kv_attend_args *a, pk_attend_job *J,
@@ -26,19 +26,24 @@ static int pk_attend_prepare(const pulsar_kv_desc *d, const pulsar_kv_attend_arg
     J->group = a->n_head / d->n_kv;
     J->rows = a->n_q * J->group;
     p->dp = d->head_dim <= 64 ? 64 : d->head_dim <= 128 ? 128 : 256;
-    /* 16 query rows share one reading of the keys where there are that many;
-     * at 256 columns their output tiles would not fit the registers */
-    p->mt = J->rows > 8 && p->dp <= 128 ? 2 : 1;
-    /* two bf16 parts hold bf16 exactly; wider q wants three for f32 results */
-    p->three = d->dtype == PULSAR_TYPE_BF16 && a->q_type != PULSAR_TYPE_BF16;
-    J->tiles = (J->rows + 8 * p->mt - 1) / (8 * p->mt);
+    /* q in one part: the cache's own 16-bit type, or bf16 (8 bits) beside f16 and e4m3 */
+    p->wide = a->q_type == PULSAR_TYPE_F32 || (d->dtype == PULSAR_TYPE_BF16 && a->q_type == PULSAR_TYPE_F16);
+    /* up to 32 query rows share one reading of the keys, where q's parts and
+     * the rows' output tiles fit registers and shared memory: 16 for wide q
+     * and at 256 columns */
+    p->r = J->rows > 8 ? 2 : 1;
+    p->mt = J->rows > 16 && !p->wide && p->dp <= 128 ? 2 : 1;
+    const uint32_t heads = 8u * p->r * p->mt;
+    J->tiles = (J->rows + heads - 1) / heads;
     if ((uint64_t)J->tiles * d->n_kv > 0x7fffffffull) return pk_refuse("kv attend: too many heads and tokens");
     J->segs = J->tiles * d->n_kv;
     J->page_shift = -1;
     for (int s = 0; s < 31; s++)
         if (d->page_size == 1u << s) J->page_shift = s;
+    const uint32_t qe = pk_type_bytes(a->q_type);
+    J->pairs = (((uintptr_t)a->q | a->q_stride * qe) % (2 * qe)) == 0;
     const uint32_t elt = pk_type_bytes(d->dtype), ck = (uint32_t)p->dp * elt >= 256 ? 16 : 32;
-    J->least = p->least = 128 / ck;
+    J->least = 128 / ck;
     /* CTAs that are resident together: shared memory holds two, one at 256 columns */
     p->workers = pk_sm_count() * (p->dp == 256 ? 1 : 2);
     if (p->workers > PK_MAX_WORKERS) p->workers = PK_MAX_WORKERS;
@@ -47,8 +52,7 @@ static int pk_attend_prepare(const pulsar_kv_desc *d, const pulsar_kv_attend_arg
     if (a->window && keys > (uint64_t)a->window + a->n_q - 1) keys = (uint64_t)a->window + a->n_q - 1;
     const uint64_t most = (uint64_t)a->n_rows * J->segs * (keys / ck + 2);
     if (p->workers > most) p->workers = (uint32_t)most;
-    p->counters = 4ull * 2 * 2 * PK_MAX_WORKERS;
-    p->bytes = PULSAR_KV_WS_ZEROED + 4ull * p->workers * 2 * 8 * p->mt * (p->dp + 2);
+    p->bytes = PULSAR_KV_WS_ZEROED + 4ull * p->workers * 2 * heads * (p->dp + 2);
     return 1;
 }
 static_assert(4 * 2 * 2 * PK_MAX_WORKERS <= PULSAR_KV_WS_ZEROED, "the counters are in the zeroed bytes");
@@ -74,8 +78,8 @@ extern "C" int pulsar_kv_attend(const pulsar_kv_desc *d, const pulsar_kv_attend_
     J.parts = (float *)((uint8_t *)ws + PULSAR_KV_WS_ZEROED);
     J.err = pk_err_word();
     if (!J.err) return pk_refuse("kv: no error word on this device");
-    const pk_attend_fn f = d->dtype == PULSAR_TYPE_BF16  ? pk_attend_bf16(p.dp, p.mt, p.three)
-                           : d->dtype == PULSAR_TYPE_F16 ? pk_attend_f16(p.dp, p.mt, p.three)
-                                                         : pk_attend_e4m3(p.dp, p.mt, p.three);
+    const pk_attend_fn f = d->dtype == PULSAR_TYPE_BF16  ? pk_attend_bf16(p.dp, p.r, p.mt, p.wide)
+                           : d->dtype == PULSAR_TYPE_F16 ? pk_attend_f16(p.dp, p.r, p.mt, p.wide)
+                                                         : pk_attend_e4m3(p.dp, p.r, p.mt, p.wide);
     return f(J, p.workers, pk_stream(stream));
 }

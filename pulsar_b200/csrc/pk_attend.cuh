@@ -7,27 +7,32 @@
  * per key are far below what the warp matrix instructions do in that time.
  *
  * Work.  The query rows of a key head are its n_q * (n_head / n_kv) (token,
- * head) pairs; a tile is 8 * MT of them.  All (sequence, key head, tile)
+ * head) pairs; a tile is HEADS of them.  All (sequence, key head, tile)
  * segments lie one behind the other on a line, counted in chunks of CK keys,
- * and the CTAs take equal slices of it: no length, batch or head count leaves
- * SMs idle, and the host needs no lengths.  A segment that a slice cuts is
- * joined through the workspace by the CTA that arrives last, in the order of
- * the slices (a fixed order: the same call gives the same bits), 32 parts at
- * a time.
+ * and the workers take equal slices of it: no length, batch or head count
+ * leaves SMs idle, and the host needs no lengths.  Long segments: a worker is
+ * a CTA, whose four warps take the chunks of its slice in turn, each with its
+ * own running maximum, sum and output tile, and meet at a segment's end; a
+ * segment that a slice cuts is joined through the workspace by the CTA that
+ * arrives last, in the order of the slices (a fixed order: the same call
+ * gives the same bits), 32 parts at a time.  Many short segments (16 chunks
+ * or fewer on average, more of them than CTAs): a worker is a warp, which
+ * takes whole segments and meets nobody.
  *
- * Inside a CTA four warps take the chunks of its slice in turn.  Each warp
- * fills a ring of its own with 16-byte asynchronous copies (no barrier in the
- * stream; keys out of the span are filled with zeros, so stale bytes never
- * meet the arithmetic) and keeps its own running maximum, sum and output
- * tile; the four meet at a segment's end.
+ * Each warp fills a ring of its own with 16-byte asynchronous copies: no
+ * barrier in the stream, and keys out of the span are filled with zeros, so
+ * that stale bytes never meet the arithmetic.
  *
- * Products.  A 16-row matrix tile holds 8 query rows twice: the leading 16
- * bits of each value in row g and the next 16 in row g + 8, of q for the
- * scores and of the probabilities for the output.  The tile is 16 rows high
- * anyway, so the second half costs nothing and the sums keep 22 bits of each
- * factor (f16 parts; q's rows are first scaled by a power of two) or 16 (bf16
- * parts); THREE adds a third bf16 part where a bf16 cache meets wider q, so
- * that f32 results are f32 results.  Sums, maxima and outputs are f32. */
+ * Products.  q and the probabilities p are taken in 16-bit parts (leading 16
+ * bits, the next, ...), keys and values as they are, sums in f32.
+ *   R = 1 (up to 8 query rows): the 16 rows of a matrix tile are 8 query rows
+ *   twice, the leading part in row g and the next in row g + 8: the tile is
+ *   16 rows high anyway, so the second part costs nothing.
+ *   R = 2: 16 query rows a tile, one product per part.
+ * Two f16 parts hold 22 bits (q's rows are first scaled by a power of two, p
+ * by 2^15: nothing of weight falls among f16's subnormals), two bf16 parts
+ * 16; QP = 3 adds a third where a bf16 cache meets wider q, so that f32
+ * results are f32 results.  QP = 1: q has the cache's type or fewer bits. */
 #pragma once
 #include "pk_common.h"
 
@@ -46,9 +51,10 @@ struct pk_attend_job {
     uint32_t tiles;      /* tiles per key head */
     uint32_t segs;       /* segments per sequence: n_kv * tiles */
     int32_t page_shift;  /* log2(page_size), or -1 */
+    uint32_t pairs;      /* q's rows are aligned for loads of two values */
     uint32_t least;      /* least chunks in a slice, where segments are long */
     uint32_t *counters;  /* [2][2 * PK_MAX_WORKERS] */
-    float *parts;        /* [workers][2] parts of 8 * MT * (DP + 2) floats */
+    float *parts;        /* [workers][2] parts of HEADS * (DP + 2) floats */
     uint32_t *err;
 };
 
@@ -134,17 +140,19 @@ __device__ __forceinline__ uint32_t pk_e4m3x2(uint32_t v) {
  * of +-inf makes the lower parts' products NaN, the leading one's +-inf */
 __device__ __forceinline__ float pk_fold(float lead, float rest) { return isfinite(rest) ? lead + rest : lead; }
 
-/* what a sequence's length, window and row say */
+/* ------------------------------------------------------------ the line */
+
+#define PK_CACHED 256u /* sequences whose length and table row are kept in shared memory */
+
+/* what a sequence's length, window and table row say */
 struct pk_row {
-    int32_t len, c0, n;       /* keys; first chunk; chunks (at least 1) */
+    int32_t len, c0, n; /* keys; first chunk; chunks (at least 1) */
     const int32_t *table;
 };
 
-template <int CK>
-__device__ __forceinline__ pk_row pk_row_of(const pk_attend_job &J, uint32_t b, bool tell) {
-    pk_row r;
-    const int32_t row = J.A.seq ? J.A.seq[b] : (int32_t)b;
-    int32_t len = J.A.lens[b];
+/* (keys, table row) of sequence b, checked */
+__device__ __forceinline__ int2 pk_len_of(const pk_attend_job &J, uint32_t b, bool tell) {
+    int32_t row = J.A.seq ? J.A.seq[b] : (int32_t)b, len = J.A.lens[b];
     const int32_t cap = (int32_t)(J.D.max_pages * J.D.page_size);
     uint32_t bad = 0;
     if (row < 0 || len < 0) len = 0;
@@ -157,12 +165,18 @@ __device__ __forceinline__ pk_row pk_row_of(const pk_attend_job &J, uint32_t b, 
         len = cap;
     }
     if (bad && tell) atomicOr(J.err, bad);
-    r.len = len;
-    const int64_t lo = J.A.window ? (int64_t)len - (J.A.n_q - 1) - J.A.window : 0;
-    r.c0 = lo > 0 ? (int32_t)(lo / CK) : 0;
-    const int32_t end = (int32_t)(((int64_t)len + CK - 1) / CK);
+    return make_int2(len, len ? row : 0);
+}
+
+template <int CK>
+__device__ __forceinline__ pk_row pk_row_of(const pk_attend_job &J, int2 lr) {
+    pk_row r;
+    r.len = lr.x;
+    const int64_t lo = J.A.window ? (int64_t)lr.x - (J.A.n_q - 1) - J.A.window : 0;
+    r.c0 = lo > 0 ? (int32_t)lo / CK : 0;
+    const int32_t end = (int32_t)(((uint32_t)lr.x + CK - 1) / CK);
     r.n = end > r.c0 ? end - r.c0 : 1;
-    r.table = J.D.table + (uint64_t)(len ? row : 0) * J.D.table_stride;
+    r.table = J.D.table + (uint64_t)lr.y * J.D.table_stride;
     return r;
 }
 
@@ -173,37 +187,113 @@ __device__ __forceinline__ void pk_span(const pk_attend_job &J, int32_t len, uin
     lo = J.A.window && (uint32_t)hi > J.A.window ? hi - (int32_t)J.A.window : 0;
 }
 
-__device__ __forceinline__ float pk_q_at(const pk_attend_job &J, uint64_t at) {
-    if (J.A.q_type == PULSAR_TYPE_BF16) return __bfloat162float(((const __nv_bfloat16 *)J.A.q)[at]);
-    if (J.A.q_type == PULSAR_TYPE_F16) return __half2float(((const __half *)J.A.q)[at]);
-    return ((const float *)J.A.q)[at];
-}
-
-/* A warp's place on the line: the chunk `pos` of segment `seg` of sequence b */
-template <int CK>
+/* a warp's place on the line: chunk pos of tile `tile` of key head hk of
+ * sequence b, and the keys that the tile's rows see between them */
+template <int CK, int HEADS>
 struct pk_cursor {
-    uint32_t b, seg;
-    int32_t pos;
+    uint32_t b, hk, tile;
+    int32_t pos, lo, hi;
     pk_row row;
-    __device__ __forceinline__ void step(const pk_attend_job &J, int32_t by) {
-        pos += by;
-        while (pos >= row.n) {
-            pos -= row.n;
-            if (++seg == J.segs) {
-                seg = 0;
-                if (++b >= J.A.n_rows) return; /* past the line's end: not used again */
-                row = pk_row_of<CK>(J, b, false);
-            }
+    __device__ __forceinline__ void enter(const pk_attend_job &J) {
+        uint32_t i0 = 0, i1 = 0;
+        if (J.A.n_q > 1) {
+            const uint32_t v0 = tile * HEADS, v1 = v0 + HEADS < J.rows ? v0 + HEADS - 1 : J.rows - 1;
+            i0 = v0 / J.group;
+            i1 = v1 / J.group;
         }
+        int32_t x;
+        pk_span(J, row.len, i0, lo, x);
+        pk_span(J, row.len, i1, x, hi);
+    }
+    __device__ __forceinline__ void step(const pk_attend_job &J, const int2 *cached, int32_t by) {
+        pos += by;
+        if (pos < row.n) return;
+        do {
+            pos -= row.n;
+            if (++tile == J.tiles) {
+                tile = 0;
+                if (++hk == J.D.n_kv) {
+                    hk = 0;
+                    if (++b >= J.A.n_rows) return; /* past the line's end: not used again */
+                    row = pk_row_of<CK>(J, J.A.n_rows <= PK_CACHED ? cached[b] : pk_len_of(J, b, false));
+                }
+            }
+        } while (pos >= row.n);
+        enter(J);
     }
 };
 
-/* columns col .. col + 3 of query row v (of key head hk, sequence b): top
- * and sum are the row's maximum (log2 units) and sum, x its output sums */
-template <int DP>
-__device__ __forceinline__ void pk_attend_out(const pk_attend_job &J, uint32_t b, int32_t len, uint32_t hk, uint32_t v,
-                                              uint32_t col, float top, float sum, float4 x) {
-    if (v >= J.rows || col >= J.D.head_dim) return;
+/* a warp finds the sequence that holds the line position `at`: upto[t] are
+ * the chunks of one segment each up to the rows of thread t (`run` rows a
+ * thread); before = those of all earlier rows */
+template <int CK>
+__device__ __forceinline__ uint32_t pk_locate(const pk_attend_job &J, const int2 *cached, const unsigned long long *upto,
+                                              uint32_t run, unsigned long long at, unsigned long long *before) {
+    const uint32_t lane = threadIdx.x & 31u;
+    uint32_t t = 0;
+#pragma unroll
+    for (uint32_t k = 0; k < PK_WARPS; k++) t += __popc(__ballot_sync(~0u, upto[k * 32 + lane] * J.segs <= at));
+    unsigned long long sum = t ? upto[t - 1] : 0;
+    for (uint32_t r0 = t * run;; r0 += 32) {
+        const uint32_t r = r0 + lane;
+        const bool in = r < (t + 1) * run && r < J.A.n_rows;
+        unsigned long long n = 0, x;
+        if (in) n = (uint32_t)pk_row_of<CK>(J, J.A.n_rows <= PK_CACHED ? cached[r] : pk_len_of(J, r, false)).n;
+        x = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const unsigned long long y = __shfl_up_sync(~0u, x, o);
+            if (lane >= o) x += y;
+        }
+        const uint32_t hit = __ballot_sync(~0u, in && (sum + x) * J.segs > at);
+        if (hit || r0 + 32 >= (t + 1) * run || r0 + 32 >= J.A.n_rows) {
+            const uint32_t k = hit ? __ffs(hit) - 1 : 0;
+            *before = sum + __shfl_sync(~0u, x - n, k);
+            return r0 + k;
+        }
+        sum += __shfl_sync(~0u, x, 31);
+    }
+}
+
+__device__ __forceinline__ unsigned long long pk_div(unsigned long long a, uint32_t b) {
+    return a >> 32 ? a / b : (uint32_t)a / b;
+}
+
+/* ------------------------------------------------------------ q, results */
+
+/* a lane's q values of one row: runs (x[ks][0..1], x[ks][2..3]) at 16 ks +
+ * d0 and d1 further on.  All loads of a row are in flight together: the type
+ * is settled outside the loop.  pairs: q is aligned for loads of two. */
+template <uint32_t QT, int KS>
+__device__ __forceinline__ void pk_q_row(const pk_attend_job &J, uint64_t at, uint32_t d0, uint32_t d1, bool have,
+                                         bool pairs, float (*x)[4]) {
+    typedef typename pk_type<QT>::t T;
+    struct __align__(2 * sizeof(T)) two {
+        T v[2];
+    };
+    const T *q = (const T *)J.A.q + at;
+#pragma unroll
+    for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+        for (int e = 0; e < 4; e += 2) {
+            const uint32_t d = ks * 16 + d0 + (e ? d1 : 0);
+            const bool in = have && ks * 16u < J.D.head_dim; /* head_dim is a multiple of 16 */
+            two r;
+            if (pairs) {
+                if (in) r = *(const two *)(q + d);
+            } else if (in) {
+                r.v[0] = q[d];
+                r.v[1] = q[d + 1];
+            }
+            x[ks][e] = in ? pk_type<QT>::get(r.v[0]) : 0.0f;
+            x[ks][e + 1] = in ? pk_type<QT>::get(r.v[1]) : 0.0f;
+        }
+}
+
+/* what query row v's output sums are multiplied with, given its maximum
+ * (log2 units) and sum; writes lse where `tell` */
+__device__ __forceinline__ float pk_finish(const pk_attend_job &J, uint32_t b, int32_t len, uint32_t hk, uint32_t v,
+                                           float top, float sum, bool tell) {
     const uint32_t i = v / J.group, h = hk * J.group + v % J.group;
     int32_t lo, hi;
     pk_span(J, len, i, lo, hi);
@@ -217,27 +307,43 @@ __device__ __forceinline__ void pk_attend_out(const pk_attend_job &J, uint32_t b
             top = t;
         }
     }
-    const uint64_t tok = (uint64_t)b * J.A.n_q + i;
-    if (J.A.lse && col == 0) J.A.lse[tok * J.A.n_head + h] = empty ? -INFINITY : logf(sum) + top * 0.6931471805599453f;
+    if (J.A.lse && tell)
+        J.A.lse[((uint64_t)b * J.A.n_q + i) * J.A.n_head + h] =
+            empty ? -INFINITY : logf(sum) + top * 0.6931471805599453f;
     by = sum == 0.0f ? 0.0f : by / sum;
-    if (J.D.v_scale) by *= __ldg(J.D.v_scale + hk);
-    if (sum == 0.0f) x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    const uint64_t at = tok * J.A.out_stride + (uint64_t)h * J.D.head_dim + col;
-    const float y[4] = {x.x * by, x.y * by, x.z * by, x.w * by};
+    return J.D.v_scale ? by * __ldg(J.D.v_scale + hk) : by;
+}
+
+/* N neighbouring columns of query row v's output */
+template <int N>
+__device__ __forceinline__ void pk_put(const pk_attend_job &J, uint32_t b, uint32_t hk, uint32_t v, uint32_t col,
+                                       const float *y) {
+    const uint64_t tok = (uint64_t)b * J.A.n_q + v / J.group;
+    const uint64_t at = tok * J.A.out_stride + (uint64_t)(hk * J.group + v % J.group) * J.D.head_dim + col;
     if (J.A.q_type == PULSAR_TYPE_F32) {
         float *d = (float *)J.A.out + at;
 #pragma unroll
-        for (int e = 0; e < 4; e++) d[e] = y[e];
+        for (int e = 0; e < N; e++) d[e] = y[e];
     } else if (J.A.q_type == PULSAR_TYPE_BF16) {
         __nv_bfloat16 *d = (__nv_bfloat16 *)J.A.out + at;
 #pragma unroll
-        for (int e = 0; e < 4; e++) d[e] = __float2bfloat16_rn(y[e]);
+        for (int e = 0; e < N; e++) d[e] = __float2bfloat16_rn(y[e]);
     } else {
         __half *d = (__half *)J.A.out + at;
 #pragma unroll
-        for (int e = 0; e < 4; e++) d[e] = __float2half_rn(y[e]);
+        for (int e = 0; e < N; e++) d[e] = __float2half_rn(y[e]);
     }
 }
+
+/* ------------------------------------------------------------ joins */
+
+/* a segment that several workers share */
+struct pk_joint {
+    uint32_t b, hk, v0, w0, w1;
+    int32_t len;
+    bool inside; /* it begins inside w0's slice: w0's part is in slot 2 w0 + 1, others' (w) in 2 w */
+    __device__ __forceinline__ uint32_t slot(uint32_t k) const { return 2 * (w0 + k) + (k == 0 && inside); }
+};
 
 /* one more part of a counter's `of` is in the workspace; true for the CTA
  * whose part completes them (which leaves the counter at zero).  Every thread
@@ -255,176 +361,214 @@ __device__ __forceinline__ bool pk_arrive(uint32_t *counter, uint32_t of, uint32
     return yes;
 }
 
-/* The join of a cut segment, which the workers w0 .. w1 share; worker w's
- * part is in slot 2 w, but in 2 w0 + 1 where the segment begins inside w0's
- * slice.  The parts meet PK_GROUP at a time (the group's sum replaces its
- * first part), then the groups; the sums run in the order of the workers. */
-template <int DP, int MT>
-__device__ void pk_attend_join(const pk_attend_job &J, uint32_t b, int32_t len, uint32_t hk, uint32_t v0, uint32_t w0,
-                               uint32_t w1, bool inside, uint32_t *last, float (*ml)[2]) {
-    constexpr uint32_t HEADS = 8 * MT;
+/* the parts meet PK_GROUP at a time, then the groups */
+__device__ __forceinline__ bool pk_joint_arrive(const pk_attend_job &J, const pk_joint &S, uint32_t *last) {
+    const uint32_t n = S.w1 - S.w0 + 1, first = (blockIdx.x - S.w0) / PK_GROUP * PK_GROUP;
+    return pk_arrive(J.counters + S.slot(first), n - first < PK_GROUP ? n - first : PK_GROUP, last);
+}
+
+/* sums of `count` parts (step apart) from `first` on, in their order; done by
+ * the CTA that completed them.  A thread has the loads of 8 parts in flight. */
+template <int DP, int HEADS>
+__device__ void pk_join(const pk_attend_job &J, const pk_joint &S, uint32_t first, uint32_t step, uint32_t count,
+                        bool final, float (*ml)[2]) {
     constexpr uint64_t FLOATS = (uint64_t)HEADS * (DP + 2);
-    const uint32_t n = w1 - w0 + 1, groups = (n + PK_GROUP - 1) / PK_GROUP;
-    const uint32_t mine = (blockIdx.x - w0) / PK_GROUP;
-    uint32_t first = mine * PK_GROUP, step = 1, count = n - first < PK_GROUP ? n - first : PK_GROUP;
-    const uint32_t name = 2 * w0 + inside; /* no other segment's first slot */
-    bool final = groups == 1;
-    if (!pk_arrive(J.counters + (final ? name : 2 * (w0 + first) + (first == 0 && inside)), count, last)) return;
-    for (;;) {
-        for (uint32_t x = threadIdx.x; x < HEADS * DP / 4; x += PK_WARPS * 32) {
-            const uint32_t head = x / (DP / 4), col = x % (DP / 4) * 4;
-            auto part = [&](uint32_t k) {
-                const uint32_t at = first + k * step;
-                return J.parts + (2ull * (w0 + at) + (at == 0 && inside)) * FLOATS;
-            };
-            float top = -INFINITY, sum = 0.0f;
-#pragma unroll 4
-            for (uint32_t k = 0; k < count; k++) top = fmaxf(top, __ldcg(part(k) + 2 * head));
-            const float zero = top == -INFINITY ? 0.0f : top;
-            float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-            for (uint32_t k = 0; k < count; k++) {
-                const float2 x2 = __ldcg((const float2 *)(part(k) + 2 * head));
-                const float4 v = __ldcg((const float4 *)(part(k) + 2 * HEADS + head * DP + col));
-                const float f = exp2f(x2.x - zero);
-                sum += x2.y * f;
-                acc.x += v.x * f;
-                acc.y += v.y * f;
-                acc.z += v.z * f;
-                acc.w += v.w * f;
-            }
-            if (final) {
-                pk_attend_out<DP>(J, b, len, hk, v0 + head, col, top, sum, acc);
-            } else {
-                __stcg((float4 *)(part(0) + 2 * HEADS + head * DP + col), acc);
-                if (col == 0) {
-                    ml[head][0] = top;
-                    ml[head][1] = sum;
+    for (uint32_t x = threadIdx.x; x < HEADS * DP / 4; x += PK_WARPS * 32) {
+        const uint32_t head = x / (DP / 4), col = x % (DP / 4) * 4;
+        float top = -INFINITY, sum = 0.0f, acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (uint32_t k0 = 0; k0 < count; k0 += 8) {
+            float2 m8[8];
+            float4 v8[8];
+#pragma unroll
+            for (uint32_t k = 0; k < 8; k++) {
+                m8[k] = make_float2(-INFINITY, 0.0f);
+                v8[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                if (k0 + k < count) {
+                    const float *p = J.parts + S.slot(first + (k0 + k) * step) * FLOATS;
+                    m8[k] = __ldcg((const float2 *)(p + 2 * head));
+                    v8[k] = __ldcg((const float4 *)(p + 2 * HEADS + head * DP + col));
                 }
             }
+            float t = top;
+#pragma unroll
+            for (uint32_t k = 0; k < 8; k++) t = fmaxf(t, m8[k].x);
+            const float zero = t == -INFINITY ? 0.0f : t, keep = exp2f(top - zero);
+            top = t;
+            sum *= keep;
+#pragma unroll
+            for (int e = 0; e < 4; e++) acc[e] *= keep;
+#pragma unroll
+            for (uint32_t k = 0; k < 8; k++) {
+                const float f = exp2f(m8[k].x - zero);
+                sum += m8[k].y * f;
+                acc[0] += v8[k].x * f;
+                acc[1] += v8[k].y * f;
+                acc[2] += v8[k].z * f;
+                acc[3] += v8[k].w * f;
+            }
         }
-        if (final) return;
-        __syncthreads(); /* part 0's maxima and sums have been read */
-        if (threadIdx.x < HEADS)
-            __stcg((float2 *)(J.parts + (2ull * (w0 + first) + (first == 0 && inside)) * FLOATS + 2 * threadIdx.x),
-                   make_float2(ml[threadIdx.x][0], ml[threadIdx.x][1]));
-        if (!pk_arrive(J.counters + 2 * PK_MAX_WORKERS + name, groups, last)) return;
-        first = 0;
-        step = PK_GROUP;
-        count = groups;
-        final = true;
+        if (final) {
+            const uint32_t v = S.v0 + head;
+            if (v < J.rows && col < J.D.head_dim) {
+                const float by = pk_finish(J, S.b, S.len, S.hk, v, top, sum, col == 0);
+#pragma unroll
+                for (int e = 0; e < 4; e++) acc[e] *= by;
+                pk_put<4>(J, S.b, S.hk, v, col, acc);
+            }
+        } else {
+            __stcg((float4 *)(J.parts + S.slot(first) * FLOATS + 2 * HEADS + head * DP + col),
+                   make_float4(acc[0], acc[1], acc[2], acc[3]));
+            if (col == 0) {
+                ml[head][0] = top;
+                ml[head][1] = sum;
+            }
+        }
     }
 }
 
-template <uint32_t CT, int DP, int MT, bool THREE>
+/* the join of a segment by the CTA that completed its group */
+template <int DP, int HEADS>
+__device__ void pk_joint_finish(const pk_attend_job &J, const pk_joint &S, uint32_t *last, float (*ml)[2]) {
+    const uint32_t n = S.w1 - S.w0 + 1, groups = (n + PK_GROUP - 1) / PK_GROUP;
+    const uint32_t first = (blockIdx.x - S.w0) / PK_GROUP * PK_GROUP;
+    __syncthreads();
+    pk_join<DP, HEADS>(J, S, first, 1, n - first < PK_GROUP ? n - first : PK_GROUP, groups == 1, ml);
+    if (groups == 1) return;
+    __syncthreads(); /* part `first`'s maxima and sums have been read, the new ones are in ml */
+    if (threadIdx.x < HEADS)
+        __stcg((float2 *)(J.parts + S.slot(first) * (uint64_t)(HEADS * (DP + 2)) + 2 * threadIdx.x),
+               make_float2(ml[threadIdx.x][0], ml[threadIdx.x][1]));
+    if (pk_arrive(J.counters + 2 * PK_MAX_WORKERS + S.slot(0), groups, last))
+        pk_join<DP, HEADS>(J, S, 0, PK_GROUP, groups, true, ml);
+}
+
+/* ------------------------------------------------------------ the kernel */
+
+template <uint32_t CT, int DP, int R, int MT, int QP>
 __global__ void __launch_bounds__(PK_WARPS * 32, 1) pk_attend_kernel(const __grid_constant__ pk_attend_job J) {
     typedef pk_shape<CT, DP> S;
     constexpr bool BF = CT == PULSAR_TYPE_BF16;
     constexpr bool F8 = CT == PULSAR_TYPE_E4M3;
     constexpr int CK = S::CK, KS = DP / 16, NT = DP / 8, KT = CK / 8;
-    constexpr int HEADS = 8 * MT;
-    constexpr bool QSM = MT * DP > 128 || THREE;          /* q's parts wait in shared memory, not registers */
+    constexpr int LR = MT * R, HEADS = 8 * LR;            /* a lane's query rows; a tile's */
+    constexpr bool QSM = MT > 1 || DP > 128;              /* q's parts wait in shared memory, not registers */
+    constexpr int QW = R == 1 ? (QP == 3 ? 6 : 4) : 4 * QP; /* words per lane and k-step */
+    constexpr int PP = QP == 3 ? 3 : 2;                   /* parts of p */
+    constexpr int PW = R == 1 ? (PP == 3 ? 6 : 4) : 4 * PP;
+    constexpr bool REST = R == 1 ? QP == 3 : QP > 1;      /* lower parts of q have sums of their own */
     constexpr float LIFT = BF ? 0.0f : 15.0f;
-    constexpr int QPARTS = THREE ? 6 : 4;                 /* words per lane and k-step */
 
     extern __shared__ __align__(128) uint8_t smem[];
     uint8_t *ring = smem + (threadIdx.x >> 5) * S::RING;
     float *join = (float *)(smem + PK_WARPS * S::RING);
-    /* QSM: [MT][KS][QPARTS][32], in the same bytes: q is done with when a segment's warps meet */
+    unsigned long long *upto = (unsigned long long *)join; /* in the beginning */
+    /* QSM: [MT][KS][QW][32], in the same bytes: q is done with when a segment's warps meet */
     uint32_t *qsm = (uint32_t *)join;
-    static_assert(!QSM || MT * KS * QPARTS * 128 <= S::JOIN, "q's parts fit beside the ring");
+    static_assert(!QSM || MT * KS * QW * 128 <= S::JOIN, "q's parts fit beside the ring");
+    static_assert(PK_WARPS * 32 * 8 <= S::JOIN, "the line's sums fit");
     __shared__ float wml[PK_WARPS][HEADS][2];             /* each warp's maximum and sum */
     __shared__ float fml[HEADS][2];
     __shared__ uint32_t vmask[PK_WARPS][PK_STAGES];       /* keys of a stage that are there */
-    __shared__ unsigned long long scan[PK_WARPS + 2];
-    __shared__ uint32_t found[2], last;
+    __shared__ int2 cached[PK_CACHED];
+    __shared__ uint32_t last;
 
     const uint32_t tid = threadIdx.x, lane = tid & 31u, w = tid >> 5;
     const uint32_t g = lane >> 2, c = lane & 3u;          /* row and column pair of a fragment */
 
-    /* ---- the line's length, this CTA's slice, and where that begins */
+    /* ---- the line's length */
     const uint32_t B = J.A.n_rows;
     const uint32_t run = (B + PK_WARPS * 32 - 1) / (PK_WARPS * 32);
-    const uint32_t r0 = tid * run < B ? tid * run : B, r1 = B - r0 < run ? B : r0 + run;
     unsigned long long mine = 0;
-    for (uint32_t r = r0; r < r1; r++) mine += (unsigned long long)pk_row_of<CK>(J, r, blockIdx.x == 0).n;
-    unsigned long long upto = mine;
+    for (uint32_t r = tid * run; r < (tid + 1) * run && r < B; r++) {
+        const int2 lr = pk_len_of(J, r, blockIdx.x == 0);
+        if (B <= PK_CACHED) cached[r] = lr;
+        mine += (uint32_t)pk_row_of<CK>(J, lr).n;
+    }
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const unsigned long long y = __shfl_up_sync(~0u, upto, o);
-        if (lane >= o) upto += y;
+        const unsigned long long y = __shfl_up_sync(~0u, mine, o);
+        if (lane >= o) mine += y;
     }
-    if (lane == 31) scan[w] = upto;
-    __syncthreads();
-    unsigned long long before = 0, all = 0;
-#pragma unroll
-    for (uint32_t k = 0; k < PK_WARPS; k++) {
-        if (k < w) before += scan[k];
-        all += scan[k];
-    }
-    upto += before;
-    const unsigned long long total = all * J.segs;
-    unsigned long long per = (total + gridDim.x - 1) / gridDim.x;
-    /* a segment of up to 16 chunks is not cut to fill idle SMs: joining it costs more than reading it */
-    const unsigned long long least = all <= 16ull * B ? (all + B - 1) / B : J.least;
-    if (per < least) per = least;
-    const unsigned long long lo = per * blockIdx.x;
-    if (lo >= total) return;
-    const unsigned long long hi = total - lo < per ? total : lo + per;
-    if ((upto - mine) * J.segs <= lo && lo < upto * J.segs) { /* one thread: lo is in its rows */
-        unsigned long long at = upto - mine;
-        for (uint32_t r = r0; r < r1; r++) {
-            const uint32_t n = (uint32_t)pk_row_of<CK>(J, r, false).n;
-            if (lo < (at + n) * J.segs) {
-                found[0] = r;
-                scan[PK_WARPS] = at * J.segs;
-                break;
-            }
-            at += n;
-        }
-    }
+    upto[tid] = mine;
     /* columns from head_dim to DP stay zero: copies never write them */
     const uint32_t units = J.D.head_dim * S::ELT / 16;
     if (units < S::UNITS)
         for (uint32_t o = tid * 16; o < PK_WARPS * S::RING; o += PK_WARPS * 32 * 16)
             *(uint4 *)(smem + o) = make_uint4(0, 0, 0, 0);
     __syncthreads();
-
-    /* ---- cursors: cons walks the CTA's segments, prod runs ahead by the warp's chunks */
-    pk_cursor<CK> cons;
-    cons.b = found[0];
-    cons.row = pk_row_of<CK>(J, cons.b, false);
-    {
-        const unsigned long long in = lo - scan[PK_WARPS];
-        cons.seg = (uint32_t)(in / (uint32_t)cons.row.n);
-        cons.pos = (int32_t)(in % (uint32_t)cons.row.n);
+    unsigned long long before = 0, all = 0;
+#pragma unroll
+    for (uint32_t k = 0; k < PK_WARPS; k++) {
+        const unsigned long long x = upto[k * 32 + 31];
+        if (k < w) before += x;
+        all += x;
     }
-    pk_cursor<CK> prod = cons;
-    prod.step(J, (int32_t)w);
-    const uint32_t slice = (uint32_t)(hi - lo);           /* chunks in this CTA's slice */
-    uint32_t ahead = w;                                   /* slice offset of prod */
+    __syncthreads();
+    upto[tid] = mine + before;
+    __syncthreads();
 
+    /* ---- the worker's slice of it */
+    const unsigned long long total = all * J.segs;
+    const bool solo = !QSM && all <= 16ull * B && (unsigned long long)B * J.segs > gridDim.x;
+    const uint32_t workers = solo ? gridDim.x * PK_WARPS : gridDim.x, me = solo ? blockIdx.x * PK_WARPS + w : blockIdx.x;
+    unsigned long long per = pk_div(total + workers - 1, workers);
+    if (!solo) {
+        /* a segment of up to 16 chunks is not cut to fill idle SMs: joining it costs more than reading it */
+        const unsigned long long least = all <= 16ull * B ? pk_div(all + B - 1, B) : J.least;
+        per = per < least ? least : (per + PK_WARPS - 1) & ~(unsigned long long)(PK_WARPS - 1);
+    }
+    unsigned long long lo = per * me, hi = lo + per;
+    if (hi > total) hi = total;
+    pk_cursor<CK, HEADS> cons;
+    cons.b = cons.hk = cons.tile = 0;
+    cons.pos = 0;
+    if (lo < total) {
+        unsigned long long at;
+        cons.b = pk_locate<CK>(J, cached, upto, run, lo, &at);
+        cons.row = pk_row_of<CK>(J, B <= PK_CACHED ? cached[cons.b] : pk_len_of(J, cons.b, false));
+        const unsigned long long in = lo - at * J.segs;
+        const uint32_t seg = (uint32_t)pk_div(in, cons.row.n);
+        cons.pos = (int32_t)(in - (unsigned long long)seg * cons.row.n);
+        cons.hk = seg / J.tiles;
+        cons.tile = seg - cons.hk * J.tiles;
+        cons.enter(J);
+        if (solo) {
+            /* whole segments: those that begin in [lo, hi) */
+            if (cons.pos) {
+                const int32_t rest = cons.row.n - cons.pos;
+                lo += rest;
+                cons.step(J, cached, rest);
+            }
+            if (hi < total) {
+                const uint32_t b2 = pk_locate<CK>(J, cached, upto, run, hi, &at);
+                const uint32_t n2 = pk_row_of<CK>(J, B <= PK_CACHED ? cached[b2] : pk_len_of(J, b2, false)).n;
+                const unsigned long long off = hi - at * J.segs;
+                hi = at * J.segs + pk_div(off + n2 - 1, n2) * n2;
+            }
+        }
+    }
+    __syncthreads(); /* `upto` has been read */
+    if (lo >= hi) return; /* a CTA's four warps alike, but for solo ones, which meet no more */
+
+    /* ---- cursors: cons walks the worker's segments, prod runs ahead by the warp's chunks */
+    const uint32_t stride = solo ? 1 : PK_WARPS, lead = solo ? 0 : w;
+    const uint32_t slice = (uint32_t)(hi - lo);           /* chunks in the slice */
+    pk_cursor<CK, HEADS> prod = cons;
+    uint32_t ahead = lead;                                /* slice offset of prod */
+    if (lead) prod.step(J, cached, (int32_t)lead);
     const uint32_t kbase = pk_saddr(ring);
-    const uint64_t elt = S::ELT;
 
     auto issue = [&](uint32_t st) {
         if (ahead < slice) {
-            const uint32_t hk = prod.seg / J.tiles, tile = prod.seg % J.tiles;
-            int32_t tlo, thi, x;
-            {
-                const uint32_t v0 = tile * HEADS, v1 = v0 + HEADS < J.rows ? v0 + HEADS - 1 : J.rows - 1;
-                pk_span(J, prod.row.len, v0 / J.group, tlo, x);
-                pk_span(J, prod.row.len, v1 / J.group, x, thi);
-            }
             const int32_t j = (prod.row.c0 + prod.pos) * CK + (int32_t)(lane % CK);
             uint64_t off = 0;
-            bool real = j >= tlo && j < thi;
+            bool real = j >= prod.lo && j < prod.hi;
             if (real) {
                 const uint32_t pi = J.page_shift >= 0 ? (uint32_t)j >> J.page_shift : (uint32_t)j / J.D.page_size;
                 const uint32_t slot = (uint32_t)j - pi * J.D.page_size;
                 const uint32_t page = (uint32_t)__ldg(prod.row.table + pi);
                 if (page < J.D.n_pages) {
-                    off = ((uint64_t)page * J.D.page_stride + hk * J.D.head_stride + slot * J.D.tok_stride) * elt;
+                    off = ((uint64_t)page * J.D.page_stride + prod.hk * J.D.head_stride + slot * J.D.tok_stride) * S::ELT;
                 } else {
                     real = false;
                     atomicOr(J.err, PULSAR_KV_ERR_PAGE);
@@ -434,7 +578,7 @@ __global__ void __launch_bounds__(PK_WARPS * 32, 1) pk_attend_kernel(const __gri
             if (lane == 0) vmask[w][st] = CK == 32 ? there : there & ((1u << (CK & 31)) - 1u);
             if (there) {
                 const uint32_t lo32 = (uint32_t)off, hi32 = (uint32_t)(off >> 32);
-                constexpr uint32_t RPI = 32 / S::UNITS ? 32 / S::UNITS : 1; /* rows per instruction */
+                constexpr uint32_t RPI = 32 / S::UNITS; /* keys per instruction */
                 const uint32_t u = lane % S::UNITS, rr = lane / S::UNITS;
                 const uint32_t dst = kbase + st * S::STAGE;
 #pragma unroll
@@ -449,100 +593,121 @@ __global__ void __launch_bounds__(PK_WARPS * 32, 1) pk_attend_kernel(const __gri
                     }
                 }
             }
-            prod.step(J, PK_WARPS);
-            ahead += PK_WARPS;
+            ahead += stride;
+            if (ahead < slice) prod.step(J, cached, (int32_t)stride);
         }
         pk_cp_commit();
     };
-#pragma unroll
+#pragma unroll 1
     for (uint32_t st = 0; st < PK_STAGES - 1; st++) issue(st);
 
     uint32_t stage = 0;
     uint32_t done = 0;                                    /* slice offset where the segment at hand begins */
-    uint32_t next = w;                                    /* slice offset of this warp's next chunk */
-    unsigned long long base = lo;                         /* line position of `done` */
+    uint32_t next = lead;                                 /* slice offset of this warp's next chunk */
+    pk_joint owed;                                        /* a join that this CTA completed, put off to the end */
+    bool owes = false;
 
     while (done < slice) {
         const int32_t from = cons.pos;                    /* chunks [from, to) of this segment are ours */
         const int32_t to = (uint32_t)(cons.row.n - from) <= slice - done ? cons.row.n : from + (int32_t)(slice - done);
-        const uint32_t hk = cons.seg / J.tiles, tile = cons.seg % J.tiles;
-        const uint32_t v0 = tile * HEADS;
+        const uint32_t v0 = cons.tile * HEADS;
 
-        /* ---- q of this tile, in 16-bit parts */
-        uint32_t qr[QSM ? 1 : MT][QSM ? 1 : KS][4];
-        float unit[MT];                                   /* score units: log2, the power of two taken from q */
-        int32_t slo[MT], shi[MT];
+        /* ---- q of this tile, in 16-bit parts; row 8 y + g of it is the lane's row y */
+        uint32_t qr[QSM ? 1 : KS][QW];
+        float unit[LR];                                   /* score units: log2, the power of two taken from q */
+        int32_t slo[LR], shi[LR];
 #pragma unroll
         for (int mt = 0; mt < MT; mt++) {
-            const uint32_t v = v0 + mt * 8 + g;
-            const bool have = v < J.rows;
-            const uint32_t i = have ? v / J.group : 0, h = hk * J.group + (have ? v % J.group : 0);
-            pk_span(J, cons.row.len, i, slo[mt], shi[mt]);
-            if (!have) shi[mt] = 0;
-            const uint64_t at = ((uint64_t)cons.b * J.A.n_q + i) * J.A.q_stride + (uint64_t)h * J.D.head_dim;
-            float x[KS][4], most = 0.0f;
+            float x[R][KS][4];
 #pragma unroll
-            for (int ks = 0; ks < KS; ks++) {
+            for (int r = 0; r < R; r++) {
+                const int y = mt * R + r;
+                const uint32_t v = v0 + y * 8 + g;
+                const bool have = v < J.rows;
+                const uint32_t i = have ? v / J.group : 0, h = cons.hk * J.group + (have ? v % J.group : 0);
+                pk_span(J, cons.row.len, i, slo[y], shi[y]);
+                if (!have) shi[y] = 0;
+                const uint64_t at = ((uint64_t)cons.b * J.A.n_q + i) * J.A.q_stride + (uint64_t)h * J.D.head_dim;
                 /* e4m3 rows come as four neighbouring values a lane, 16-bit ones as two pairs */
-                const uint32_t d0 = ks * 16 + (F8 ? 4 * c : 2 * c), d1 = d0 + (F8 ? 2 : 8);
+                const uint32_t d0 = F8 ? 4 * c : 2 * c, d1 = F8 ? 2 : 8;
+                if (J.A.q_type == PULSAR_TYPE_BF16) pk_q_row<PULSAR_TYPE_BF16, KS>(J, at, d0, d1, have, J.pairs, x[r]);
+                else if (J.A.q_type == PULSAR_TYPE_F16) pk_q_row<PULSAR_TYPE_F16, KS>(J, at, d0, d1, have, J.pairs, x[r]);
+                else pk_q_row<PULSAR_TYPE_F32, KS>(J, at, d0, d1, have, J.pairs, x[r]);
+                unit[y] = J.A.scale * PK_LOG2E * (F8 && J.D.k_scale ? __ldg(J.D.k_scale + cons.hk) : 1.0f);
+                if (!BF) {
+                    /* the row's largest value to [2^14, 2^15): small ones stay clear of f16's subnormals */
+                    float most = 0.0f;
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const uint32_t d = (e < 2 ? d0 : d1) + (e & 1);
-                    x[ks][e] = have && d < J.D.head_dim ? pk_q_at(J, at + d) : 0.0f;
-                    most = fmaxf(most, fabsf(x[ks][e]));
+                    for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) most = fmaxf(most, fabsf(x[r][ks][e]));
+                    most = fmaxf(most, __shfl_xor_sync(~0u, most, 1));
+                    most = fmaxf(most, __shfl_xor_sync(~0u, most, 2));
+                    uint32_t ex = __float_as_uint(most) >> 23;
+                    ex = ex < 15 ? 15 : ex > 253 ? 253 : ex;
+                    const float up = __uint_as_float((268u - ex) << 23);
+                    unit[y] *= __uint_as_float((ex - 14u) << 23);
+#pragma unroll
+                    for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) x[r][ks][e] *= up;
                 }
             }
-            unit[mt] = J.A.scale * PK_LOG2E * (F8 && J.D.k_scale ? __ldg(J.D.k_scale + hk) : 1.0f);
-            if (!BF) {
-                most = fmaxf(most, __shfl_xor_sync(~0u, most, 1));
-                most = fmaxf(most, __shfl_xor_sync(~0u, most, 2));
-                uint32_t ex = __float_as_uint(most) >> 23;
-                ex = ex < 15 ? 15 : ex > 253 ? 253 : ex;
-                /* the row's largest value to [2^14, 2^15): small ones stay clear of f16's subnormals */
-                const float down = __uint_as_float((268u - ex) << 23);
-                unit[mt] *= __uint_as_float((ex - 14u) << 23);
-#pragma unroll
-                for (int ks = 0; ks < KS; ks++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) x[ks][e] *= down;
-            }
 #pragma unroll
             for (int ks = 0; ks < KS; ks++) {
-                uint32_t p[QPARTS];
-                p[0] = pk_split<BF>(x[ks][0], x[ks][1]);
-                p[2] = pk_split<BF>(x[ks][2], x[ks][3]);
-                p[1] = pk_split<BF>(x[ks][0], x[ks][1]);
-                p[3] = pk_split<BF>(x[ks][2], x[ks][3]);
-                if constexpr (THREE) {
-                    p[4] = pk_split<BF>(x[ks][0], x[ks][1]);
-                    p[5] = pk_split<BF>(x[ks][2], x[ks][3]);
+                uint32_t p[QW];
+                if constexpr (R == 1) {
+                    p[0] = pk_split<BF>(x[0][ks][0], x[0][ks][1]);
+                    p[2] = pk_split<BF>(x[0][ks][2], x[0][ks][3]);
+                    p[1] = pk_split<BF>(x[0][ks][0], x[0][ks][1]);
+                    p[3] = pk_split<BF>(x[0][ks][2], x[0][ks][3]);
+                    if constexpr (QP == 3) {
+                        p[4] = pk_split<BF>(x[0][ks][0], x[0][ks][1]);
+                        p[5] = pk_split<BF>(x[0][ks][2], x[0][ks][3]);
+                    }
+                } else {
+#pragma unroll
+                    for (int q = 0; q < QP; q++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            p[4 * q + e] = pk_split<BF>(x[e & 1][ks][e & 2], x[e & 1][ks][(e & 2) + 1]);
                 }
                 if constexpr (QSM) {
                     if (ks % PK_WARPS == w)
 #pragma unroll
-                        for (int e = 0; e < QPARTS; e++) qsm[((mt * KS + ks) * QPARTS + e) * 32 + lane] = p[e];
+                        for (int e = 0; e < QW; e++) qsm[((mt * KS + ks) * QW + e) * 32 + lane] = p[e];
                 } else {
 #pragma unroll
-                    for (int e = 0; e < 4; e++) qr[mt][ks][e] = p[e];
+                    for (int e = 0; e < QW; e++) qr[ks][e] = p[e];
                 }
             }
         }
         if constexpr (QSM) __syncthreads();
-
-        float o[MT][NT][4], m[MT], l[MT];
+        auto q_words = [&](int mt, int ks, uint32_t *a) {
 #pragma unroll
-        for (int mt = 0; mt < MT; mt++) {
-            m[mt] = -INFINITY;
-            l[mt] = 0.0f;
+            for (int e = 0; e < QW; e++) {
+                if constexpr (QSM) a[e] = qsm[((mt * KS + ks) * QW + e) * 32 + lane];
+                else a[e] = qr[ks][e];
+            }
+        };
+
+        float o[MT][NT][4], m[LR], l[LR];
+#pragma unroll
+        for (int y = 0; y < LR; y++) {
+            m[y] = -INFINITY;
+            l[y] = 0.0f;
+        }
+#pragma unroll
+        for (int mt = 0; mt < MT; mt++)
 #pragma unroll
             for (int t = 0; t < NT; t++)
 #pragma unroll
                 for (int e = 0; e < 4; e++) o[mt][t][e] = 0.0f;
-        }
 
         /* ---- the warp's chunks of this segment */
         const uint32_t end = done + (uint32_t)(to - from);
-        for (; next < end; next += PK_WARPS) {
+#pragma unroll 1
+        for (; next < end; next += stride) {
             pk_cp_wait<PK_STAGES - 2>();
             __syncwarp();
             issue(stage + PK_STAGES - 1 < PK_STAGES ? stage + PK_STAGES - 1 : stage - 1);
@@ -552,278 +717,349 @@ __global__ void __launch_bounds__(PK_WARPS * 32, 1) pk_attend_kernel(const __gri
             if (!there) continue;
             const int32_t key0 = (cons.row.c0 + from + (int32_t)(next - done)) * CK;
 
+            /* scores: keys are the columns */
+            float s[MT][KT][4], rest[REST ? MT : 1][KT][4];
 #pragma unroll
-            for (int mt = 0; mt < MT; mt++) {
-                /* scores: keys are the columns */
-                float s[KT][4], s3[THREE ? KT : 1][4];
+            for (int mt = 0; mt < MT; mt++)
 #pragma unroll
                 for (int t = 0; t < KT; t++)
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        s[t][e] = 0.0f;
-                        if constexpr (THREE) s3[t][e] = 0.0f;
+                        s[mt][t][e] = 0.0f;
+                        if constexpr (REST) rest[mt][t][e] = 0.0f;
                     }
+            auto score = [&](int mt, int t, const uint32_t *a, uint32_t b0, uint32_t b1) {
+                pk_mma<BF>(s[mt][t], a[0], a[1], a[2], a[3], b0, b1);
+                if constexpr (R == 1 && QP == 3) pk_mma<BF>(rest[mt][t], a[4], 0, a[5], 0, b0, b1);
+                if constexpr (R == 2 && QP > 1) pk_mma<BF>(rest[mt][t], a[4], a[5], a[6], a[7], b0, b1);
+                if constexpr (R == 2 && QP > 2) pk_mma<BF>(rest[mt][t], a[8], a[9], a[10], a[11], b0, b1);
+            };
+            constexpr int KQ = F8 && KT == 2 ? 2 : 1; /* k-steps per load: 16-key e4m3 chunks take two */
 #pragma unroll
-                for (int ks = 0; ks < KS; ks++) {
-                    uint32_t a[QPARTS];
-                    if constexpr (QSM) {
+            for (int ks = 0; ks < KS; ks += KQ) {
+                uint32_t a[MT][KQ][QW];
 #pragma unroll
-                        for (int e = 0; e < QPARTS; e++) a[e] = qsm[((mt * KS + ks) * QPARTS + e) * 32 + lane];
-                    } else {
+                for (int mt = 0; mt < MT; mt++)
 #pragma unroll
-                        for (int e = 0; e < 4; e++) a[e] = qr[mt][ks][e];
+                    for (int q = 0; q < KQ; q++) q_words(mt, ks + q, a[mt][q]);
+                if constexpr (!F8) {
+                    /* matrices (keys 0-7, d 0-7), (0-7, 8-15), (8-15, 0-7), (8-15, 8-15) */
+#pragma unroll
+                    for (int t = 0; t < KT; t += 2) {
+                        uint32_t b[4];
+                        const uint32_t r = t * 8 + (lane >> 4) * 8 + (lane & 7u), u = ks * 2 + ((lane >> 3) & 1u);
+                        pk_ldm4(b, ka + r * S::ROW + (u ^ (r & 7u)) * 16);
+#pragma unroll
+                        for (int mt = 0; mt < MT; mt++) {
+                            score(mt, t, a[mt][0], b[0], b[1]);
+                            score(mt, t + 1, a[mt][0], b[2], b[3]);
+                        }
                     }
-                    if constexpr (!F8) {
-                        /* 16 keys x 16 values at a time: matrices (keys 0-7, d 0-7), (0-7, 8-15), (8-15, 0-7), (8-15, 8-15) */
+                } else if constexpr (KT == 4) {
+                    /* a matrix is 8 keys x 16 bytes */
+                    uint32_t b[4];
+                    const uint32_t sw = S::ROW >= 128 ? (uint32_t)ks ^ (lane & 7u) : (uint32_t)ks ^ ((lane >> 1) & 3u);
+                    pk_ldm4(b, ka + lane * S::ROW + sw * 16);
 #pragma unroll
-                        for (int t = 0; t < KT; t += 2) {
-                            uint32_t b[4];
-                            const uint32_t r = t * 8 + (lane >> 4) * 8 + (lane & 7u), u = ks * 2 + ((lane >> 3) & 1u);
-                            pk_ldm4(b, ka + r * S::ROW + (u ^ (r & 7u)) * 16);
-                            pk_mma<BF>(s[t], a[0], a[1], a[2], a[3], b[0], b[1]);
-                            pk_mma<BF>(s[t + 1], a[0], a[1], a[2], a[3], b[2], b[3]);
-                            if constexpr (THREE) {
-                                pk_mma<BF>(s3[t], a[4], 0, a[5], 0, b[0], b[1]);
-                                pk_mma<BF>(s3[t + 1], a[4], 0, a[5], 0, b[2], b[3]);
-                            }
-                        }
-                    } else {
-                        /* a matrix is 8 keys x 16 bytes; 16-key chunks take two k-steps at a time */
-                        if constexpr (KT == 4) {
-                            uint32_t b[4];
-                            const uint32_t sw = S::ROW >= 128 ? (uint32_t)ks ^ (lane & 7u) : (uint32_t)ks ^ ((lane >> 1) & 3u);
-                            pk_ldm4(b, ka + lane * S::ROW + sw * 16);
+                    for (int t = 0; t < 4; t++) {
+                        const uint32_t b0 = pk_e4m3x2(b[t]), b1 = pk_e4m3x2(b[t] >> 16);
 #pragma unroll
-                            for (int t = 0; t < 4; t++)
-                                pk_mma<BF>(s[t], a[0], a[1], a[2], a[3], pk_e4m3x2(b[t]), pk_e4m3x2(b[t] >> 16));
-                        } else if (ks % 2 == 0) {
-                            uint32_t b[4], a2[4];
-                            const uint32_t r = lane & 15u, u = ks + (lane >> 4);
-                            pk_ldm4(b, ka + r * S::ROW + (u ^ (r & 7u)) * 16);
+                        for (int mt = 0; mt < MT; mt++) score(mt, t, a[mt][0], b0, b1);
+                    }
+                } else {
+                    uint32_t b[4];
+                    const uint32_t r = lane & 15u, u = ks + (lane >> 4);
+                    pk_ldm4(b, ka + r * S::ROW + (u ^ (r & 7u)) * 16);
 #pragma unroll
-                            for (int e = 0; e < 4; e++) {
-                                if constexpr (QSM) a2[e] = qsm[((mt * KS + ks + 1) * QPARTS + e) * 32 + lane];
-                                else a2[e] = qr[mt][ks + 1 < KS ? ks + 1 : ks][e];
-                            }
+                    for (int t = 0; t < 4; t++) {
+                        const uint32_t b0 = pk_e4m3x2(b[t]), b1 = pk_e4m3x2(b[t] >> 16);
 #pragma unroll
-                            for (int t = 0; t < 2; t++) {
-                                pk_mma<BF>(s[t], a[0], a[1], a[2], a[3], pk_e4m3x2(b[t]), pk_e4m3x2(b[t] >> 16));
-                                pk_mma<BF>(s[t], a2[0], a2[1], a2[2], a2[3], pk_e4m3x2(b[2 + t]),
-                                           pk_e4m3x2(b[2 + t] >> 16));
-                            }
-                        }
+                        for (int mt = 0; mt < MT; mt++) score(mt, t & 1, a[mt][KQ - 1 < (t >> 1) ? 0 : t >> 1], b0, b1);
                     }
                 }
-                /* fold the parts, mask, running maximum and sum: a lane has columns 2c, 2c + 1 of row g */
-                const bool whole = there == (CK == 32 ? ~0u : (1u << (CK & 31)) - 1u) && key0 >= slo[mt] &&
-                                   key0 + CK <= shi[mt];
-                float p[KT][2], top = -INFINITY;
+            }
+
+            /* fold the parts, mask, running maximum and sum (a lane has columns 2c, 2c + 1 of its rows); p's
+             * parts are the left factors of the output products in the layout that they already have */
+            uint32_t pa[MT][KT / 2][PW];
 #pragma unroll
-                for (int t = 0; t < KT; t++)
+            for (int mt = 0; mt < MT; mt++) {
+                float p[R][KT][2], keep[R];
+                bool moved = false;
 #pragma unroll
-                    for (int e = 0; e < 2; e++) {
-                        float x = pk_fold(s[t][e], THREE ? s[t][e + 2] + s3[t][e] : s[t][e + 2]) * unit[mt];
-                        if (!whole) {
-                            const int32_t k = t * 8 + 2 * (int32_t)c + e;
-                            if (!(there >> k & 1u) || key0 + k < slo[mt] || key0 + k >= shi[mt]) x = -INFINITY;
+                for (int r = 0; r < R; r++) {
+                    const int y = mt * R + r;
+                    const bool whole = there == (CK == 32 ? ~0u : (1u << (CK & 31)) - 1u) && key0 >= slo[y] &&
+                                       key0 + CK <= shi[y];
+                    float top = -INFINITY;
+#pragma unroll
+                    for (int t = 0; t < KT; t++)
+#pragma unroll
+                        for (int e = 0; e < 2; e++) {
+                            float x = s[mt][t][2 * r + e];
+                            if constexpr (R == 1) x = pk_fold(x, QP == 3 ? s[mt][t][e + 2] + rest[0][t][e] : s[mt][t][e + 2]);
+                            else if constexpr (QP > 1) x = pk_fold(x, rest[mt][t][2 * r + e]);
+                            x *= unit[y];
+                            if (!whole) {
+                                const int32_t k = t * 8 + 2 * (int32_t)c + e;
+                                if (!(there >> k & 1u) || key0 + k < slo[y] || key0 + k >= shi[y]) x = -INFINITY;
+                            }
+                            p[r][t][e] = x;
+                            top = fmaxf(top, x);
                         }
-                        p[t][e] = x;
-                        top = fmaxf(top, x);
-                    }
-                top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
-                top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
-                top = fmaxf(top, m[mt]);
-                /* weights are relative to the maximum less LIFT, so that small ones stay clear of f16's
-                 * subnormals; nothing seen yet: every weight is 0 */
-                const float zero = (top == -INFINITY ? 0.0f : top) - LIFT;
-                const float keep = exp2f(m[mt] - LIFT - zero);
-                if (__any_sync(~0u, top != m[mt])) {
-                    l[mt] *= keep;
+                    top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
+                    top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
+                    top = fmaxf(top, m[y]);
+                    /* weights are relative to the maximum less LIFT; nothing seen yet: every weight is 0 */
+                    const float zero = (top == -INFINITY ? 0.0f : top) - LIFT;
+                    keep[r] = exp2f(m[y] - LIFT - zero);
+                    moved |= top != m[y];
+                    m[y] = top;
+                    l[y] *= keep[r];
+#pragma unroll
+                    for (int t = 0; t < KT; t++)
+#pragma unroll
+                        for (int e = 0; e < 2; e++) {
+                            p[r][t][e] = exp2f(p[r][t][e] - zero);
+                            l[y] += p[r][t][e];
+                        }
+                }
+                if (__any_sync(~0u, moved))
 #pragma unroll
                     for (int t = 0; t < NT; t++)
 #pragma unroll
-                        for (int e = 0; e < 4; e++) o[mt][t][e] *= keep;
-                }
-                m[mt] = top;
+                        for (int e = 0; e < 4; e++) o[mt][t][e] *= keep[R == 1 ? 0 : e >> 1];
 #pragma unroll
-                for (int t = 0; t < KT; t++)
-#pragma unroll
-                    for (int e = 0; e < 2; e++) {
-                        p[t][e] = exp2f(p[t][e] - zero);
-                        l[mt] += p[t][e];
-                    }
-                /* output: the weights are the left factor in the layout that they already have */
-#pragma unroll
-                for (int kt = 0; kt < KT; kt += 2) {
-                    uint32_t a[6];
-                    a[0] = pk_split<BF>(p[kt][0], p[kt][1]);
-                    a[2] = pk_split<BF>(p[kt + 1][0], p[kt + 1][1]);
-                    a[1] = pk_split<BF>(p[kt][0], p[kt][1]);
-                    a[3] = pk_split<BF>(p[kt + 1][0], p[kt + 1][1]);
-                    if constexpr (THREE) {
-                        a[4] = pk_split<BF>(p[kt][0], p[kt][1]);
-                        a[5] = pk_split<BF>(p[kt + 1][0], p[kt + 1][1]);
-                    }
-                    /* matrices (keys 0-7, unit u), (keys 8-15, u), (0-7, u + 1), (8-15, u + 1) */
-                    const uint32_t r = kt * 8 + (lane & 15u), up = lane >> 4;
-#pragma unroll
-                    for (int u = 0; u < S::UNITS; u += 2) {
-                        uint32_t b[4];
-                        const uint32_t sw = S::ROW >= 128 ? (u + up) ^ (r & 7u) : (u + up) ^ ((r >> 1) & 3u);
-                        pk_ldm4t(b, va + r * S::ROW + sw * 16);
-                        if constexpr (!F8) {
-                            pk_mma<BF>(o[mt][u], a[0], a[1], a[2], a[3], b[0], b[1]);
-                            pk_mma<BF>(o[mt][u + 1], a[0], a[1], a[2], a[3], b[2], b[3]);
-                            if constexpr (THREE) {
-                                pk_mma<BF>(o[mt][u], a[4], 0, a[5], 0, b[0], b[1]);
-                                pk_mma<BF>(o[mt][u + 1], a[4], 0, a[5], 0, b[2], b[3]);
-                            }
-                        } else {
-                            /* a 16-bit column is two values: the even ones to tile 2u, the odd ones to 2u + 1 */
-#pragma unroll
-                            for (int y = 0; y < 2; y++) {
-                                const uint32_t x0 = b[2 * y], x1 = b[2 * y + 1];
-                                pk_mma<BF>(o[mt][2 * (u + y)], a[0], a[1], a[2], a[3], pk_e4m3x2(__byte_perm(x0, 0, 0x0020)),
-                                           pk_e4m3x2(__byte_perm(x1, 0, 0x0020)));
-                                pk_mma<BF>(o[mt][2 * (u + y) + 1], a[0], a[1], a[2], a[3],
-                                           pk_e4m3x2(__byte_perm(x0, 0, 0x0031)), pk_e4m3x2(__byte_perm(x1, 0, 0x0031)));
-                            }
+                for (int kt = 0; kt < KT / 2; kt++) {
+                    uint32_t *a = pa[mt][kt];
+                    if constexpr (R == 1) {
+                        a[0] = pk_split<BF>(p[0][2 * kt][0], p[0][2 * kt][1]);
+                        a[2] = pk_split<BF>(p[0][2 * kt + 1][0], p[0][2 * kt + 1][1]);
+                        a[1] = pk_split<BF>(p[0][2 * kt][0], p[0][2 * kt][1]);
+                        a[3] = pk_split<BF>(p[0][2 * kt + 1][0], p[0][2 * kt + 1][1]);
+                        if constexpr (PP == 3) {
+                            a[4] = pk_split<BF>(p[0][2 * kt][0], p[0][2 * kt][1]);
+                            a[5] = pk_split<BF>(p[0][2 * kt + 1][0], p[0][2 * kt + 1][1]);
                         }
+                    } else {
+#pragma unroll
+                        for (int q = 0; q < PP; q++)
+#pragma unroll
+                            for (int e = 0; e < 4; e++)
+                                a[4 * q + e] = pk_split<BF>(p[e & 1][2 * kt + (e >> 1)][0], p[e & 1][2 * kt + (e >> 1)][1]);
                     }
                 }
             }
-        }
-
-        /* ---- the four warps meet: maxima, then each quarter of the columns goes to one warp */
-        const bool cut = from != 0 || to != cons.row.n;
-        const uint32_t slot = 2 * blockIdx.x + (done != 0);
-        const uint64_t part_floats = (uint64_t)HEADS * (DP + 2);
+            auto weigh = [&](int t, int kt, uint32_t b0, uint32_t b1) {
 #pragma unroll
-        for (int mt = 0; mt < MT; mt++) {
-            l[mt] += __shfl_xor_sync(~0u, l[mt], 1);
-            l[mt] += __shfl_xor_sync(~0u, l[mt], 2);
-            if (c == 0) {
-                wml[w][mt * 8 + g][0] = m[mt];
-                wml[w][mt * 8 + g][1] = l[mt];
-            }
-        }
-        __syncthreads();
-#pragma unroll
-        for (int mt = 0; mt < MT; mt++) {
-            if (mt) __syncthreads(); /* the previous tile's sums are out of `join` */
-            float top = -INFINITY, sum = 0.0f;
-#pragma unroll
-            for (uint32_t k = 0; k < PK_WARPS; k++) top = fmaxf(top, wml[k][mt * 8 + g][0]);
-            const float zero = top == -INFINITY ? 0.0f : top;
-#pragma unroll
-            for (uint32_t k = 0; k < PK_WARPS; k++) sum += wml[k][mt * 8 + g][1] * exp2f(wml[k][mt * 8 + g][0] - LIFT - zero);
-            const float keep = exp2f(m[mt] - LIFT - zero);
-            if (w == 0 && c == 0) {
-                fml[mt * 8 + g][0] = top;
-                fml[mt * 8 + g][1] = sum;
-            }
-#pragma unroll
-            for (int t = 0; t < NT; t++) {
-                o[mt][t][0] = pk_fold(o[mt][t][0], o[mt][t][2]) * keep;
-                o[mt][t][1] = pk_fold(o[mt][t][1], o[mt][t][3]) * keep;
-            }
-            /* column of (tile t, element e) within its quarter: a lane's run of 2 (16-bit) or 4 (e4m3) columns */
-            constexpr int QT = NT / 4, RUN = F8 ? 4 : 2;
-            auto place = [&](uint32_t owner, uint32_t source, int tq) {
-                return join + ((owner * 3 + source) * 8 + g) * S::QROW + (F8 ? tq * 8 + 4 * c : tq * 8 + 2 * c);
+                for (int mt = 0; mt < MT; mt++) {
+                    const uint32_t *a = pa[mt][kt];
+                    pk_mma<BF>(o[mt][t], a[0], a[1], a[2], a[3], b0, b1);
+                    if constexpr (R == 1 && PP == 3) pk_mma<BF>(o[mt][t], a[4], 0, a[5], 0, b0, b1);
+                    if constexpr (R == 2) pk_mma<BF>(o[mt][t], a[4], a[5], a[6], a[7], b0, b1);
+                    if constexpr (R == 2 && PP == 3) pk_mma<BF>(o[mt][t], a[8], a[9], a[10], a[11], b0, b1);
+                }
             };
 #pragma unroll
-            for (uint32_t q = 0; q < 4; q++)
-                if (q != w)
+            for (int kt = 0; kt < KT / 2; kt++) {
+                /* matrices (keys 0-7, unit u), (keys 8-15, u), (0-7, u + 1), (8-15, u + 1) */
+                const uint32_t r = kt * 16 + (lane & 15u), up = lane >> 4;
 #pragma unroll
-                    for (int t = 0; t < QT; t += RUN / 2) {
-                        float *d = place(q, w < q ? w : w - 1, t);
-                        const float *x = o[mt][q * QT + t];
-                        if constexpr (F8) {
-                            const float *y = o[mt][q * QT + t + 1];
-                            *(float4 *)d = make_float4(x[0], y[0], x[1], y[1]);
-                        } else {
-                            *(float2 *)d = make_float2(x[0], x[1]);
+                for (int u = 0; u < S::UNITS; u += 2) {
+                    uint32_t b[4];
+                    const uint32_t sw = S::ROW >= 128 ? (u + up) ^ (r & 7u) : (u + up) ^ ((r >> 1) & 3u);
+                    pk_ldm4t(b, va + r * S::ROW + sw * 16);
+                    if constexpr (!F8) {
+                        weigh(u, kt, b[0], b[1]);
+                        weigh(u + 1, kt, b[2], b[3]);
+                    } else {
+                        /* a 16-bit column is two values: the even ones to tile 2u, the odd ones to 2u + 1 */
+#pragma unroll
+                        for (int y = 0; y < 2; y++) {
+                            const uint32_t x0 = b[2 * y], x1 = b[2 * y + 1];
+                            weigh(2 * (u + y), kt, pk_e4m3x2(__byte_perm(x0, 0, 0x0020)), pk_e4m3x2(__byte_perm(x1, 0, 0x0020)));
+                            weigh(2 * (u + y) + 1, kt, pk_e4m3x2(__byte_perm(x0, 0, 0x0031)),
+                                  pk_e4m3x2(__byte_perm(x1, 0, 0x0031)));
                         }
                     }
-            __syncthreads();
-#pragma unroll
-            for (uint32_t q = 0; q < 4; q++)
-                if (q == w)
-#pragma unroll
-                    for (int t = 0; t < QT; t += RUN / 2) {
-                        const float *x = o[mt][q * QT + t];
-                        float own[RUN], sum4[RUN];
-                        own[0] = x[0];
-                        if constexpr (F8) {
-                            const float *y = o[mt][q * QT + t + 1];
-                            own[1] = y[0];
-                            own[2] = x[1];
-                            own[3] = y[1];
-                        } else {
-                            own[1] = x[1];
-                        }
-#pragma unroll
-                        for (int e = 0; e < RUN; e++) sum4[e] = 0.0f;
-#pragma unroll
-                        for (uint32_t k = 0; k < 4; k++)
-#pragma unroll
-                            for (int e = 0; e < RUN; e++) sum4[e] += k == q ? own[e] : place(q, k < q ? k : k - 1, t)[e];
-                        float *d = place(q, 0, t);
-#pragma unroll
-                        for (int e = 0; e < RUN; e++) d[e] = sum4[e];
-                    }
-            __syncthreads();
-
-            /* ---- out, or into the workspace */
-            for (uint32_t x = tid; x < 8 * DP / 4; x += PK_WARPS * 32) {
-                const uint32_t hh = x / (DP / 4), col = x % (DP / 4) * 4, q = col / (DP / 4);
-                const float4 v = *(const float4 *)(join + ((q * 3) * 8 + hh) * S::QROW + col % (DP / 4));
-                const uint32_t head = mt * 8 + hh;
-                if (cut) {
-                    float *part = J.parts + slot * part_floats;
-                    __stcg((float4 *)(part + 2 * HEADS + head * DP + col), v);
-                    if (col == 0) __stcg((float2 *)(part + 2 * head), make_float2(fml[head][0], fml[head][1]));
-                } else {
-                    pk_attend_out<DP>(J, cons.b, cons.row.len, hk, v0 + head, col, fml[head][0], fml[head][1], v);
                 }
             }
         }
-        if (cut) {
-            const unsigned long long seg0 = base - (uint32_t)from, seg1 = seg0 + (uint32_t)cons.row.n;
-            const uint32_t w0 = (uint32_t)(seg0 / per), w1 = (uint32_t)((seg1 - 1) / per);
-            pk_attend_join<DP, MT>(J, cons.b, cons.row.len, hk, v0, w0, w1, seg0 > per * w0, &last, fml);
-        }
-        __syncthreads(); /* wml, fml, join and qsm are free again */
 
+        /* ---- the segment's end */
         const uint32_t took = (uint32_t)(to - from);
+        constexpr int QT = NT / 4, RUN = F8 ? 4 : 2;      /* tiles of a quarter of the columns; a lane's run of columns */
+        /* RUN neighbouring columns of row y at tile t: folded parts, times by */
+        auto columns = [&](int y, int t, float by, float *x) {
+            const float *a = o[y / R][t], *b2 = o[y / R][F8 ? t + 1 : t];
+            if constexpr (R == 1) {
+                x[0] = pk_fold(a[0], a[2]);
+                x[RUN - 2 > 0 ? 2 : 1] = pk_fold(a[1], a[3]);
+                if constexpr (F8) {
+                    x[1] = pk_fold(b2[0], b2[2]);
+                    x[RUN - 1] = pk_fold(b2[1], b2[3]);
+                }
+            } else {
+                x[0] = a[2 * (y % R)];
+                x[RUN - 2 > 0 ? 2 : 1] = a[2 * (y % R) + 1];
+                if constexpr (F8) {
+                    x[1] = b2[2 * (y % R)];
+                    x[RUN - 1] = b2[2 * (y % R) + 1];
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < RUN; e++) x[e] *= by;
+        };
+#pragma unroll
+        for (int y = 0; y < LR; y++) {
+            l[y] += __shfl_xor_sync(~0u, l[y], 1);
+            l[y] += __shfl_xor_sync(~0u, l[y], 2);
+        }
+        const float drop = BF ? 1.0f : 1.0f / 32768.0f;   /* 2^-LIFT */
+        if (solo) {
+#pragma unroll
+            for (int y = 0; y < LR; y++) {
+                const uint32_t v = v0 + y * 8 + g;
+                if (v >= J.rows) continue;
+                const float by = drop * pk_finish(J, cons.b, cons.row.len, cons.hk, v, m[y], l[y] * drop, c == 0);
+#pragma unroll
+                for (int t = 0; t < NT; t += RUN / 2) {
+                    const uint32_t col = t * 8 + RUN * c;
+                    float x[RUN];
+                    columns(y, t, by, x);
+                    if (col < J.D.head_dim) pk_put<RUN>(J, cons.b, cons.hk, v, col, x);
+                }
+            }
+        } else {
+            /* the four warps meet: maxima, then each quarter of the columns goes to one warp */
+            const bool cut = from != 0 || to != cons.row.n;
+            float *part = J.parts + (uint64_t)(2 * blockIdx.x + (done != 0)) * (HEADS * (DP + 2));
+#pragma unroll
+            for (int y = 0; y < LR; y++)
+                if (c == 0) *(float2 *)wml[w][y * 8 + g] = make_float2(m[y], l[y] * drop);
+            __syncthreads();
+#pragma unroll
+            for (int y = 0; y < LR; y++) {
+                if (y) __syncthreads(); /* the previous rows' sums are out of `join` */
+                float top = -INFINITY, sum = 0.0f;
+#pragma unroll
+                for (uint32_t k = 0; k < PK_WARPS; k++) top = fmaxf(top, wml[k][y * 8 + g][0]);
+                const float zero = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+                for (uint32_t k = 0; k < PK_WARPS; k++) sum += wml[k][y * 8 + g][1] * exp2f(wml[k][y * 8 + g][0] - zero);
+                const float keep = drop * exp2f(m[y] - zero);
+                if (w == 0 && c == 0) *(float2 *)fml[y * 8 + g] = make_float2(top, sum);
+                auto place = [&](uint32_t owner, uint32_t source, int tq) {
+                    return join + ((owner * 3 + source) * 8 + g) * S::QROW + tq * 8 + RUN * c;
+                };
+#pragma unroll
+                for (uint32_t q = 0; q < 4; q++)
+                    if (q != w)
+#pragma unroll
+                        for (int t = 0; t < QT; t += RUN / 2) {
+                            float x[RUN], *d = place(q, w < q ? w : w - 1, t);
+                            columns(y, q * QT + t, keep, x);
+                            if constexpr (F8) *(float4 *)d = make_float4(x[0], x[1], x[RUN - 2], x[RUN - 1]);
+                            else *(float2 *)d = make_float2(x[0], x[1]);
+                        }
+                __syncthreads();
+#pragma unroll
+                for (uint32_t q = 0; q < 4; q++)
+                    if (q == w)
+#pragma unroll
+                        for (int t = 0; t < QT; t += RUN / 2) {
+                            float own[RUN], x[RUN], *d = place(q, 0, t);
+                            columns(y, q * QT + t, keep, own);
+#pragma unroll
+                            for (int e = 0; e < RUN; e++) {
+                                x[e] = 0.0f;
+#pragma unroll
+                                for (uint32_t k = 0; k < 4; k++) x[e] += k == q ? own[e] : place(q, k < q ? k : k - 1, t)[e];
+                            }
+#pragma unroll
+                            for (int e = 0; e < RUN; e++) d[e] = x[e];
+                        }
+                __syncthreads();
+
+                /* out, or into the workspace */
+                for (uint32_t i = tid; i < 8 * DP / 4; i += PK_WARPS * 32) {
+                    const uint32_t hh = i / (DP / 4), col = i % (DP / 4) * 4, q = col / (DP / 4);
+                    float4 x = *(const float4 *)(join + ((q * 3) * 8 + hh) * S::QROW + col % (DP / 4));
+                    const uint32_t head = y * 8 + hh;
+                    if (cut) {
+                        __stcg((float4 *)(part + 2 * HEADS + head * DP + col), x);
+                        if (col == 0) __stcg((float2 *)(part + 2 * head), make_float2(fml[head][0], fml[head][1]));
+                    } else if (v0 + head < J.rows && col < J.D.head_dim) {
+                        const float by = pk_finish(J, cons.b, cons.row.len, cons.hk, v0 + head, fml[head][0], fml[head][1],
+                                                   col == 0);
+                        const float z[4] = {x.x * by, x.y * by, x.z * by, x.w * by};
+                        pk_put<4>(J, cons.b, cons.hk, v0 + head, col, z);
+                    }
+                }
+            }
+            if (cut) {
+                /* a join that falls to this CTA waits for its slice's end: others may wait for the rest of it */
+                const unsigned long long seg0 = lo + done - (uint32_t)from;
+                pk_joint S2;
+                S2.b = cons.b;
+                S2.hk = cons.hk;
+                S2.v0 = v0;
+                S2.len = cons.row.len;
+                S2.w0 = (uint32_t)(seg0 / per);
+                S2.w1 = (uint32_t)((seg0 + (uint32_t)cons.row.n - 1) / per);
+                S2.inside = seg0 > per * S2.w0;
+                if (pk_joint_arrive(J, S2, &last)) {
+                    if (done + took < slice) {
+                        owed = S2;
+                        owes = true;
+                    } else {
+                        pk_joint_finish<DP, HEADS>(J, S2, &last, fml);
+                    }
+                }
+            }
+            __syncthreads(); /* wml, fml, join and qsm are free again */
+        }
         done += took;
-        base += took;
-        if (done < slice) cons.step(J, (int32_t)took);
+        if (done < slice) cons.step(J, cached, (int32_t)took);
     }
     pk_cp_wait<0>();
+    if (owes) pk_joint_finish<DP, HEADS>(J, owed, &last, fml);
 }
 
-template <uint32_t CT, int DP, int MT, bool THREE>
+template <uint32_t CT, int DP, int R, int MT, int QP>
 static int pk_attend_launch(const pk_attend_job &J, uint32_t grid, cudaStream_t st) {
     typedef pk_shape<CT, DP> S;
     static uint64_t done = 0;
     constexpr uint32_t smem = PK_WARPS * S::RING + S::JOIN;
-    auto kernel = pk_attend_kernel<CT, DP, MT, THREE>;
+    auto kernel = pk_attend_kernel<CT, DP, R, MT, QP>;
     if (!pm_smem_attr(kernel, smem, &done)) return 0;
     kernel<<<grid, PK_WARPS * 32, smem, st>>>(J);
     return pm_ok(cudaGetLastError(), "kv attend launch");
 }
 
-/* one translation unit per cache type (kv_attend_*.cu) */
+/* one translation unit per cache type (kv_attend_*.cu); r, mt and qp as the
+ * kernel's, wide: q has more bits than one part holds */
 typedef int (*pk_attend_fn)(const pk_attend_job &, uint32_t, cudaStream_t);
-pk_attend_fn pk_attend_bf16(int dp, int mt, bool three);
-pk_attend_fn pk_attend_f16(int dp, int mt, bool three);
-pk_attend_fn pk_attend_e4m3(int dp, int mt, bool three);
+pk_attend_fn pk_attend_bf16(int dp, int r, int mt, bool wide);
+pk_attend_fn pk_attend_f16(int dp, int r, int mt, bool wide);
+pk_attend_fn pk_attend_e4m3(int dp, int r, int mt, bool wide);
 
-template <uint32_t CT, bool THREE>
-static pk_attend_fn pk_attend_pick(int dp, int mt) {
-    if (dp == 64) return mt == 2 ? pk_attend_launch<CT, 64, 2, THREE> : pk_attend_launch<CT, 64, 1, THREE>;
-    if (dp == 128) return mt == 2 ? pk_attend_launch<CT, 128, 2, THREE> : pk_attend_launch<CT, 128, 1, THREE>;
-    return pk_attend_launch<CT, 256, 1, THREE>;
+template <uint32_t CT, int DP>
+static pk_attend_fn pk_attend_pick_at(int r, int mt, bool wide) {
+    constexpr int MOST = CT == PULSAR_TYPE_BF16 ? 3 : 2; /* parts of wide q */
+    if (r == 1) {
+        if (MOST == 3 && wide) return pk_attend_launch<CT, DP, 1, 1, MOST>;
+        return pk_attend_launch<CT, DP, 1, 1, 2>; /* the second part is free */
+    }
+    if (wide) return pk_attend_launch<CT, DP, 2, 1, MOST>;
+    if constexpr (DP <= 128)
+        if (mt == 2) return pk_attend_launch<CT, DP, 2, 2, 1>;
+    return pk_attend_launch<CT, DP, 2, 1, 1>;
+}
+
+template <uint32_t CT>
+static pk_attend_fn pk_attend_pick(int dp, int r, int mt, bool wide) {
+    if (dp == 64) return pk_attend_pick_at<CT, 64>(r, mt, wide);
+    if (dp == 128) return pk_attend_pick_at<CT, 128>(r, mt, wide);
+    return pk_attend_pick_at<CT, 256>(r, mt, wide);
 }
