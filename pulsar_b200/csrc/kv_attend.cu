@@ -44,8 +44,8 @@ static int pk_attend_prepare(const pulsar_kv_desc *d, const pulsar_kv_attend_arg
     J->pairs = (((uintptr_t)a->q | a->q_stride * qe) % (2 * qe)) == 0;
     const uint32_t elt = pk_type_bytes(d->dtype), ck = (uint32_t)p->dp * elt >= 256 ? 16 : 32;
     J->least = 128 / ck;
-    /* CTAs that are resident together: shared memory holds two, one at 256 columns */
-    p->workers = pk_sm_count() * (p->dp == 256 ? 1 : 2);
+    /* CTAs that are resident together (pk_shape's OCC) */
+    p->workers = pk_sm_count() * (p->dp == 256 ? 1 : PK_OCC);
     if (p->workers > PK_MAX_WORKERS) p->workers = PK_MAX_WORKERS;
     /* no more CTAs than the longest rows could feed */
     uint64_t keys = (uint64_t)d->max_pages * d->page_size;

@@ -37,7 +37,9 @@
 #include "pk_common.h"
 
 #define PK_WARPS 4u
-#define PK_STAGES 3u
+#ifndef PK_OCC
+#define PK_OCC 2
+#endif
 #define PK_GROUP 32u          /* parts joined at a time */
 #define PK_MAX_WORKERS 1024u  /* 2 x 2 counters of each fill PULSAR_KV_WS_ZEROED / 2 */
 #define PK_LOG2E 1.4426950408889634f
@@ -58,16 +60,23 @@ struct pk_attend_job {
     uint32_t *err;
 };
 
-template <uint32_t CT, int DP>
+/* OCC: CTAs that an SM holds.  Three (168 registers, rings of two stages)
+ * where one 16-row output tile of up to 128 columns and q's parts fit in that;
+ * else two; one at 256 columns, whose rings fill the shared memory. */
+template <uint32_t CT, int DP, int R, int MT, int QP>
 struct pk_shape {
     static constexpr int ELT = CT == PULSAR_TYPE_E4M3 ? 1 : 2;
     static constexpr int ROW = DP * ELT;                  /* bytes of a key in shared memory */
     static constexpr int UNITS = ROW / 16;
     static constexpr int CK = ROW >= 256 ? 16 : 32;       /* keys per chunk: about 8 KB of keys and values */
+    static constexpr int OCC = DP > 128 ? 1 : PK_OCC;
+    static constexpr int STAGES = OCC == 3 ? 2 : 3;
     static constexpr int STAGE = 2 * CK * ROW;
-    static constexpr int RING = PK_STAGES * STAGE;        /* per warp */
-    static constexpr int QROW = DP / 4 + 4;               /* floats; padded against bank conflicts */
-    static constexpr int JOIN = 4 * 3 * 8 * QROW * 4;     /* bytes: each quarter of the columns, from three warps */
+    static constexpr int RING = STAGES * STAGE;           /* per warp */
+    static constexpr int PASSES = OCC == 3 && DP == 128 ? 2 : 1;       /* of the exchange at a segment's end */
+    static constexpr int QCOLS = DP / 4 / PASSES;         /* columns of a quarter in a pass */
+    static constexpr int QROW = QCOLS + 4;                /* floats; padded against bank conflicts */
+    static constexpr int JOIN = 4 * 3 * 8 * QROW * 4;     /* bytes: each quarter, from three warps */
 };
 
 __device__ __forceinline__ uint32_t pk_saddr(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -110,22 +119,25 @@ __device__ __forceinline__ void pk_mma(float *c, uint32_t a0, uint32_t a1, uint3
                      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-/* x, y rounded to 16 bits and packed, x low; x, y become what is left (0
- * where the value is not finite) */
-template <bool BF>
+/* x, y rounded to 16 bits and packed, x low; x, y become what is left (SAFE:
+ * 0 where the value is not finite) */
+template <bool BF, bool SAFE>
 __device__ __forceinline__ uint32_t pk_split(float &x, float &y) {
     uint32_t r;
+    float a, b;
     if constexpr (BF) {
         const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
         r = *(const uint32_t *)&h;
-        x = isfinite(x) ? x - __low2float(h) : 0.0f;
-        y = isfinite(y) ? y - __high2float(h) : 0.0f;
+        a = x - __low2float(h);
+        b = y - __high2float(h);
     } else {
         const __half2 h = __floats2half2_rn(x, y);
         r = *(const uint32_t *)&h;
-        x = isfinite(x) ? x - __low2float(h) : 0.0f;
-        y = isfinite(y) ? y - __high2float(h) : 0.0f;
+        a = x - __low2float(h);
+        b = y - __high2float(h);
     }
+    x = !SAFE || isfinite(x) ? a : 0.0f;
+    y = !SAFE || isfinite(y) ? b : 0.0f;
     return r;
 }
 
@@ -133,6 +145,13 @@ __device__ __forceinline__ uint32_t pk_split(float &x, float &y) {
 __device__ __forceinline__ uint32_t pk_e4m3x2(uint32_t v) {
     uint32_t r;
     asm("{\n\t.reg .b16 t;\n\tcvt.u16.u32 t, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, t;\n\t}" : "=r"(r) : "r"(v));
+    return r;
+}
+
+/* 2^x: the hardware's, within 2 ulp; below 2^-126 it is 0 */
+__device__ __forceinline__ float pk_exp2(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
 
@@ -261,33 +280,37 @@ __device__ __forceinline__ unsigned long long pk_div(unsigned long long a, uint3
 
 /* ------------------------------------------------------------ q, results */
 
-/* a lane's q values of one row: runs (x[ks][0..1], x[ks][2..3]) at 16 ks +
- * d0 and d1 further on.  All loads of a row are in flight together: the type
- * is settled outside the loop.  pairs: q is aligned for loads of two. */
-template <uint32_t QT, int KS>
-__device__ __forceinline__ void pk_q_row(const pk_attend_job &J, uint64_t at, uint32_t d0, uint32_t d1, bool have,
-                                         bool pairs, float (*x)[4]) {
+/* N k-steps of a lane's q values of one row: runs x[n][0..1], x[n][2..3] at
+ * 16 (k0 + n) + d0 and d1 further on.  No load waits for another: the type is
+ * settled outside the loop, and a row or column that is not there reads one
+ * that is.  pairs: q is aligned for loads of two. */
+template <uint32_t QT, int N>
+__device__ __forceinline__ void pk_q_load(const pk_attend_job &J, uint64_t at, uint32_t k0, uint32_t d0, uint32_t d1,
+                                          float (*x)[4]) {
     typedef typename pk_type<QT>::t T;
     struct __align__(2 * sizeof(T)) two {
         T v[2];
     };
-    const T *q = (const T *)J.A.q + at;
+    const T *q = (const T *)J.A.q + at + d0;
+    if (J.pairs) {
 #pragma unroll
-    for (int ks = 0; ks < KS; ks++)
+        for (int n = 0; n < N; n++)
 #pragma unroll
-        for (int e = 0; e < 4; e += 2) {
-            const uint32_t d = ks * 16 + d0 + (e ? d1 : 0);
-            const bool in = have && ks * 16u < J.D.head_dim; /* head_dim is a multiple of 16 */
-            two r;
-            if (pairs) {
-                if (in) r = *(const two *)(q + d);
-            } else if (in) {
-                r.v[0] = q[d];
-                r.v[1] = q[d + 1];
+            for (int e = 0; e < 4; e += 2) {
+                const uint32_t d = (k0 + n) * 16u < J.D.head_dim ? (k0 + n) * 16u : 0u;
+                const two r = *(const two *)(q + d + (e ? d1 : 0));
+                x[n][e] = pk_type<QT>::get(r.v[0]);
+                x[n][e + 1] = pk_type<QT>::get(r.v[1]);
             }
-            x[ks][e] = in ? pk_type<QT>::get(r.v[0]) : 0.0f;
-            x[ks][e + 1] = in ? pk_type<QT>::get(r.v[1]) : 0.0f;
-        }
+    } else {
+#pragma unroll
+        for (int n = 0; n < N; n++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const uint32_t d = (k0 + n) * 16u < J.D.head_dim ? (k0 + n) * 16u : 0u;
+                x[n][e] = pk_type<QT>::get(q[d + (e & 2 ? d1 : 0) + (e & 1)]);
+            }
+    }
 }
 
 /* what query row v's output sums are multiplied with, given its maximum
@@ -302,8 +325,8 @@ __device__ __forceinline__ float pk_finish(const pk_attend_job &J, uint32_t b, i
     if (J.A.sinks && !empty) {
         const float sink = __ldg(J.A.sinks + h) * PK_LOG2E, t = fmaxf(top, sink);
         if (t != -INFINITY) {
-            by = exp2f(top - t);
-            sum = sum * by + exp2f(sink - t);
+            by = pk_exp2(top - t);
+            sum = sum * by + pk_exp2(sink - t);
             top = t;
         }
     }
@@ -392,14 +415,14 @@ __device__ void pk_join(const pk_attend_job &J, const pk_joint &S, uint32_t firs
             float t = top;
 #pragma unroll
             for (uint32_t k = 0; k < 8; k++) t = fmaxf(t, m8[k].x);
-            const float zero = t == -INFINITY ? 0.0f : t, keep = exp2f(top - zero);
+            const float zero = t == -INFINITY ? 0.0f : t, keep = pk_exp2(top - zero);
             top = t;
             sum *= keep;
 #pragma unroll
             for (int e = 0; e < 4; e++) acc[e] *= keep;
 #pragma unroll
             for (uint32_t k = 0; k < 8; k++) {
-                const float f = exp2f(m8[k].x - zero);
+                const float f = pk_exp2(m8[k].x - zero);
                 sum += m8[k].y * f;
                 acc[0] += v8[k].x * f;
                 acc[1] += v8[k].y * f;
@@ -445,14 +468,14 @@ __device__ void pk_joint_finish(const pk_attend_job &J, const pk_joint &S, uint3
 /* ------------------------------------------------------------ the kernel */
 
 template <uint32_t CT, int DP, int R, int MT, int QP>
-__global__ void __launch_bounds__(PK_WARPS * 32, 1) pk_attend_kernel(const __grid_constant__ pk_attend_job J) {
-    typedef pk_shape<CT, DP> S;
+__global__ void __launch_bounds__(PK_WARPS * 32, pk_shape<CT, DP, R, MT, QP>::OCC) pk_attend_kernel(const __grid_constant__ pk_attend_job J) {
+    typedef pk_shape<CT, DP, R, MT, QP> S;
     constexpr bool BF = CT == PULSAR_TYPE_BF16;
     constexpr bool F8 = CT == PULSAR_TYPE_E4M3;
     constexpr int CK = S::CK, KS = DP / 16, NT = DP / 8, KT = CK / 8;
     constexpr int LR = MT * R, HEADS = 8 * LR;            /* a lane's query rows; a tile's */
     constexpr bool QSM = MT > 1 || DP > 128;              /* q's parts wait in shared memory, not registers */
-    constexpr int QW = R == 1 ? (QP == 3 ? 6 : 4) : 4 * QP; /* words per lane and k-step */
+    constexpr int QW = R == 1 ? 2 * QP : 4 * QP;            /* words per lane and k-step */
     constexpr int PP = QP == 3 ? 3 : 2;                   /* parts of p */
     constexpr int PW = R == 1 ? (PP == 3 ? 6 : 4) : 4 * PP;
     constexpr bool REST = R == 1 ? QP == 3 : QP > 1;      /* lower parts of q have sums of their own */
@@ -462,13 +485,13 @@ __global__ void __launch_bounds__(PK_WARPS * 32, 1) pk_attend_kernel(const __gri
     uint8_t *ring = smem + (threadIdx.x >> 5) * S::RING;
     float *join = (float *)(smem + PK_WARPS * S::RING);
     unsigned long long *upto = (unsigned long long *)join; /* in the beginning */
-    /* QSM: [MT][KS][QW][32], in the same bytes: q is done with when a segment's warps meet */
+    /* QSM: [MT][KS][QW / 2][32][2], in the same bytes: q is done with when a segment's warps meet */
     uint32_t *qsm = (uint32_t *)join;
     static_assert(!QSM || MT * KS * QW * 128 <= S::JOIN, "q's parts fit beside the ring");
     static_assert(PK_WARPS * 32 * 8 <= S::JOIN, "the line's sums fit");
     __shared__ float wml[PK_WARPS][HEADS][2];             /* each warp's maximum and sum */
     __shared__ float fml[HEADS][2];
-    __shared__ uint32_t vmask[PK_WARPS][PK_STAGES];       /* keys of a stage that are there */
+    __shared__ uint32_t vmask[PK_WARPS][S::STAGES];       /* keys of a stage that are there */
     __shared__ int2 cached[PK_CACHED];
     __shared__ uint32_t last;
 
@@ -558,48 +581,72 @@ __global__ void __launch_bounds__(PK_WARPS * 32, 1) pk_attend_kernel(const __gri
     if (lead) prod.step(J, cached, (int32_t)lead);
     const uint32_t kbase = pk_saddr(ring);
 
+    /* the page of each lane's key of prod's chunk is loaded a chunk ahead */
+    uint32_t page = 0, slot = 0;
+    bool real = false;
+    auto fetch = [&]() {
+        const int32_t j = (prod.row.c0 + prod.pos) * CK + (int32_t)(lane % CK);
+        real = j >= prod.lo && j < prod.hi;
+        if (real) {
+            const uint32_t pi = J.page_shift >= 0 ? (uint32_t)j >> J.page_shift : (uint32_t)j / J.D.page_size;
+            slot = (uint32_t)j - pi * J.D.page_size;
+            page = (uint32_t)__ldg(prod.row.table + pi);
+        }
+    };
+    constexpr uint32_t RPI = 32 / S::UNITS;               /* keys per copy instruction of a warp */
+    const uint32_t cu = lane % S::UNITS, cr = lane / S::UNITS; /* a lane's 16 bytes and first key in it */
+    const bool in_page = J.D.page_size % CK == 0;         /* a chunk is part of one page */
+    const uint64_t key_step = (uint64_t)RPI * J.D.tok_stride * S::ELT;
+    const uint64_t k_to_v = (uint64_t)((const uint8_t *)J.D.v - (const uint8_t *)J.D.k);
+    if (ahead < slice) fetch();
+
     auto issue = [&](uint32_t st) {
         if (ahead < slice) {
-            const int32_t j = (prod.row.c0 + prod.pos) * CK + (int32_t)(lane % CK);
-            uint64_t off = 0;
-            bool real = j >= prod.lo && j < prod.hi;
-            if (real) {
-                const uint32_t pi = J.page_shift >= 0 ? (uint32_t)j >> J.page_shift : (uint32_t)j / J.D.page_size;
-                const uint32_t slot = (uint32_t)j - pi * J.D.page_size;
-                const uint32_t page = (uint32_t)__ldg(prod.row.table + pi);
-                if (page < J.D.n_pages) {
-                    off = ((uint64_t)page * J.D.page_stride + prod.hk * J.D.head_stride + slot * J.D.tok_stride) * S::ELT;
-                } else {
-                    real = false;
-                    atomicOr(J.err, PULSAR_KV_ERR_PAGE);
-                }
+            if (real && page >= J.D.n_pages) {
+                real = false;
+                atomicOr(J.err, PULSAR_KV_ERR_PAGE);
             }
             const uint32_t there = __ballot_sync(~0u, real);
             if (lane == 0) vmask[w][st] = CK == 32 ? there : there & ((1u << (CK & 31)) - 1u);
-            if (there) {
-                const uint32_t lo32 = (uint32_t)off, hi32 = (uint32_t)(off >> 32);
-                constexpr uint32_t RPI = 32 / S::UNITS; /* keys per instruction */
-                const uint32_t u = lane % S::UNITS, rr = lane / S::UNITS;
-                const uint32_t dst = kbase + st * S::STAGE;
+            const uint64_t off = (uint64_t)page * J.D.page_stride + prod.hk * J.D.head_stride;
+            const uint32_t dst = kbase + st * S::STAGE + cr * S::ROW;
+            if (there == ~0u && in_page) {
+                /* one page, every key: addresses go up by a constant */
+                if (cu < units) {
+                    const uint8_t *k = (const uint8_t *)J.D.k +
+                                       (off + (slot - lane % CK + cr) * J.D.tok_stride) * S::ELT + cu * 16;
 #pragma unroll
+                    for (uint32_t i = 0; i < CK / RPI; i++) {
+                        const uint32_t r = i * RPI + cr;
+                        const uint32_t d = dst + i * RPI * S::ROW + (S::ROW >= 128 ? cu ^ (r & 7u) : cu ^ ((r >> 1) & 3u)) * 16;
+                        pk_cp16(d, k, true);
+                        pk_cp16(d + CK * S::ROW, k + k_to_v, true);
+                        k += key_step;
+                    }
+                }
+            } else if (there) {
+                const uint64_t at = real ? (off + slot * J.D.tok_stride) * S::ELT : 0;
+                const uint32_t lo32 = (uint32_t)at, hi32 = (uint32_t)(at >> 32);
+#pragma unroll 1
                 for (uint32_t i = 0; i < CK / RPI; i++) {
-                    const uint32_t r = i * RPI + rr;
+                    const uint32_t r = i * RPI + cr;
                     const uint64_t o = (uint64_t)__shfl_sync(~0u, hi32, r) << 32 | __shfl_sync(~0u, lo32, r);
-                    const uint32_t sw = S::ROW >= 128 ? u ^ (r & 7u) : u ^ ((r >> 1) & 3u);
+                    const uint32_t d = dst + i * RPI * S::ROW + (S::ROW >= 128 ? cu ^ (r & 7u) : cu ^ ((r >> 1) & 3u)) * 16;
                     const bool ok = there >> r & 1u;
-                    if (u < units) {
-                        pk_cp16(dst + r * S::ROW + sw * 16, (const uint8_t *)J.D.k + o + u * 16, ok);
-                        pk_cp16(dst + CK * S::ROW + r * S::ROW + sw * 16, (const uint8_t *)J.D.v + o + u * 16, ok);
+                    if (cu < units) {
+                        pk_cp16(d, (const uint8_t *)J.D.k + o + cu * 16, ok);
+                        pk_cp16(d + CK * S::ROW, (const uint8_t *)J.D.v + o + cu * 16, ok);
                     }
                 }
             }
             ahead += stride;
-            if (ahead < slice) prod.step(J, cached, (int32_t)stride);
+            if (ahead < slice) {
+                prod.step(J, cached, (int32_t)stride);
+                fetch();
+            }
         }
         pk_cp_commit();
     };
-#pragma unroll 1
-    for (uint32_t st = 0; st < PK_STAGES - 1; st++) issue(st);
 
     uint32_t stage = 0;
     uint32_t done = 0;                                    /* slice offset where the segment at hand begins */
@@ -612,16 +659,17 @@ __global__ void __launch_bounds__(PK_WARPS * 32, 1) pk_attend_kernel(const __gri
         const int32_t to = (uint32_t)(cons.row.n - from) <= slice - done ? cons.row.n : from + (int32_t)(slice - done);
         const uint32_t v0 = cons.tile * HEADS;
 
-        /* ---- q of this tile, in 16-bit parts; row 8 y + g of it is the lane's row y */
+        /* ---- q of this tile, in 16-bit parts; row 8 y + g of it is the lane's row y.  In shared memory the
+         * warps' shares (KN k-steps each) meet; in registers each warp has all. */
+        constexpr int KN = QSM ? KS / PK_WARPS : KS;
+        const uint32_t k0 = QSM ? w * KN : 0;
         uint32_t qr[QSM ? 1 : KS][QW];
         float unit[LR];                                   /* score units: log2, the power of two taken from q */
         int32_t slo[LR], shi[LR];
+        {
+            float x[LR][KN][4];
 #pragma unroll
-        for (int mt = 0; mt < MT; mt++) {
-            float x[R][KS][4];
-#pragma unroll
-            for (int r = 0; r < R; r++) {
-                const int y = mt * R + r;
+            for (int y = 0; y < LR; y++) {
                 const uint32_t v = v0 + y * 8 + g;
                 const bool have = v < J.rows;
                 const uint32_t i = have ? v / J.group : 0, h = cons.hk * J.group + (have ? v % J.group : 0);
@@ -630,64 +678,85 @@ __global__ void __launch_bounds__(PK_WARPS * 32, 1) pk_attend_kernel(const __gri
                 const uint64_t at = ((uint64_t)cons.b * J.A.n_q + i) * J.A.q_stride + (uint64_t)h * J.D.head_dim;
                 /* e4m3 rows come as four neighbouring values a lane, 16-bit ones as two pairs */
                 const uint32_t d0 = F8 ? 4 * c : 2 * c, d1 = F8 ? 2 : 8;
-                if (J.A.q_type == PULSAR_TYPE_BF16) pk_q_row<PULSAR_TYPE_BF16, KS>(J, at, d0, d1, have, J.pairs, x[r]);
-                else if (J.A.q_type == PULSAR_TYPE_F16) pk_q_row<PULSAR_TYPE_F16, KS>(J, at, d0, d1, have, J.pairs, x[r]);
-                else pk_q_row<PULSAR_TYPE_F32, KS>(J, at, d0, d1, have, J.pairs, x[r]);
+                if (J.A.q_type == PULSAR_TYPE_BF16) pk_q_load<PULSAR_TYPE_BF16, KN>(J, at, k0, d0, d1, x[y]);
+                else if (J.A.q_type == PULSAR_TYPE_F16) pk_q_load<PULSAR_TYPE_F16, KN>(J, at, k0, d0, d1, x[y]);
+                else pk_q_load<PULSAR_TYPE_F32, KN>(J, at, k0, d0, d1, x[y]);
                 unit[y] = J.A.scale * PK_LOG2E * (F8 && J.D.k_scale ? __ldg(J.D.k_scale + cons.hk) : 1.0f);
+            }
+            if (done == 0) /* behind q's loads in the queue, not before them */
+#pragma unroll 1
+                for (uint32_t st = 0; st < S::STAGES - 1; st++) issue(st);
+            float most[LR];
+#pragma unroll
+            for (int y = 0; y < LR; y++) {
+                most[y] = 0.0f;
+#pragma unroll
+                for (int n = 0; n < KN; n++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        if (v0 + y * 8 + g >= J.rows || (k0 + n) * 16u >= J.D.head_dim) x[y][n][e] = 0.0f;
+                        most[y] = fmaxf(most[y], fabsf(x[y][n][e]));
+                    }
                 if (!BF) {
+                    most[y] = fmaxf(most[y], __shfl_xor_sync(~0u, most[y], 1));
+                    most[y] = fmaxf(most[y], __shfl_xor_sync(~0u, most[y], 2));
+                    if (QSM && c == 0) wml[w][y * 8 + g][0] = most[y];
+                }
+            }
+            if (!BF) {
+                if (QSM) __syncthreads();
+#pragma unroll
+                for (int y = 0; y < LR; y++) {
+                    if (QSM)
+#pragma unroll
+                        for (uint32_t k = 0; k < PK_WARPS; k++) most[y] = fmaxf(most[y], wml[k][y * 8 + g][0]);
                     /* the row's largest value to [2^14, 2^15): small ones stay clear of f16's subnormals */
-                    float most = 0.0f;
-#pragma unroll
-                    for (int ks = 0; ks < KS; ks++)
-#pragma unroll
-                        for (int e = 0; e < 4; e++) most = fmaxf(most, fabsf(x[r][ks][e]));
-                    most = fmaxf(most, __shfl_xor_sync(~0u, most, 1));
-                    most = fmaxf(most, __shfl_xor_sync(~0u, most, 2));
-                    uint32_t ex = __float_as_uint(most) >> 23;
+                    uint32_t ex = __float_as_uint(most[y]) >> 23;
                     ex = ex < 15 ? 15 : ex > 253 ? 253 : ex;
                     const float up = __uint_as_float((268u - ex) << 23);
                     unit[y] *= __uint_as_float((ex - 14u) << 23);
 #pragma unroll
-                    for (int ks = 0; ks < KS; ks++)
+                    for (int n = 0; n < KN; n++)
 #pragma unroll
-                        for (int e = 0; e < 4; e++) x[r][ks][e] *= up;
+                        for (int e = 0; e < 4; e++) x[y][n][e] *= up;
                 }
             }
 #pragma unroll
-            for (int ks = 0; ks < KS; ks++) {
-                uint32_t p[QW];
-                if constexpr (R == 1) {
-                    p[0] = pk_split<BF>(x[0][ks][0], x[0][ks][1]);
-                    p[2] = pk_split<BF>(x[0][ks][2], x[0][ks][3]);
-                    p[1] = pk_split<BF>(x[0][ks][0], x[0][ks][1]);
-                    p[3] = pk_split<BF>(x[0][ks][2], x[0][ks][3]);
-                    if constexpr (QP == 3) {
-                        p[4] = pk_split<BF>(x[0][ks][0], x[0][ks][1]);
-                        p[5] = pk_split<BF>(x[0][ks][2], x[0][ks][3]);
+            for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+                for (int n = 0; n < KN; n++) {
+                    uint32_t p[QW];
+                    if constexpr (R == 1) {
+#pragma unroll
+                        for (int e = 0; e < QW; e++) p[e] = pk_split<BF, true>(x[0][n][2 * (e & 1)], x[0][n][2 * (e & 1) + 1]);
+                    } else {
+#pragma unroll
+                        for (int q = 0; q < QP; q++)
+#pragma unroll
+                            for (int e = 0; e < 4; e++) {
+                                float *z = x[mt * R + (e & 1) * (R - 1)][n] + (e & 2);
+                                p[4 * q + e] = pk_split<BF, true>(z[0], z[1]);
+                            }
                     }
-                } else {
 #pragma unroll
-                    for (int q = 0; q < QP; q++)
-#pragma unroll
-                        for (int e = 0; e < 4; e++)
-                            p[4 * q + e] = pk_split<BF>(x[e & 1][ks][e & 2], x[e & 1][ks][(e & 2) + 1]);
+                    for (int e = 0; e < QW; e++) {
+                        if constexpr (QSM) qsm[(((mt * KS + k0 + n) * (QW / 2) + e / 2) * 32 + lane) * 2 + (e & 1)] = p[e];
+                        else qr[n][e] = p[e];
+                    }
                 }
-                if constexpr (QSM) {
-                    if (ks % PK_WARPS == w)
-#pragma unroll
-                        for (int e = 0; e < QW; e++) qsm[((mt * KS + ks) * QW + e) * 32 + lane] = p[e];
-                } else {
-#pragma unroll
-                    for (int e = 0; e < QW; e++) qr[ks][e] = p[e];
-                }
-            }
         }
         if constexpr (QSM) __syncthreads();
         auto q_words = [&](int mt, int ks, uint32_t *a) {
 #pragma unroll
-            for (int e = 0; e < QW; e++) {
-                if constexpr (QSM) a[e] = qsm[((mt * KS + ks) * QW + e) * 32 + lane];
-                else a[e] = qr[ks][e];
+            for (int e = 0; e < QW; e += 2) {
+                if constexpr (QSM) {
+                    const uint2 z = ((const uint2 *)qsm)[((mt * KS + ks) * (QW / 2) + e / 2) * 32 + lane];
+                    a[e] = z.x;
+                    a[e + 1] = z.y;
+                } else {
+                    a[e] = qr[ks][e];
+                    a[e + 1] = qr[ks][e + 1];
+                }
             }
         };
 
@@ -708,13 +777,21 @@ __global__ void __launch_bounds__(PK_WARPS * 32, 1) pk_attend_kernel(const __gri
         const uint32_t end = done + (uint32_t)(to - from);
 #pragma unroll 1
         for (; next < end; next += stride) {
-            pk_cp_wait<PK_STAGES - 2>();
+            pk_cp_wait<S::STAGES - 2>();
             __syncwarp();
-            issue(stage + PK_STAGES - 1 < PK_STAGES ? stage + PK_STAGES - 1 : stage - 1);
+            issue(stage == 0 ? S::STAGES - 1 : stage - 1);
             const uint32_t there = vmask[w][stage];
-            const uint32_t ka = kbase + stage * S::STAGE, va = ka + CK * S::ROW;
-            stage = stage + 1 == PK_STAGES ? 0 : stage + 1;
+            const uint32_t ka = kbase + stage * S::STAGE;
+            stage = stage + 1 == S::STAGES ? 0 : stage + 1;
             if (!there) continue;
+            /* the lane's ldmatrix rows; 16-byte unit u of row r sits at unit u ^ swizzle(r), the swizzle within
+             * 128 aligned bytes, so that unit u + v (no carry) is an exclusive or away */
+            auto unit_at = [](uint32_t x, int u) { return (x ^ ((u & 7) * 16)) + (u >> 3) * 128; };
+            const uint32_t kr = F8 ? (KT == 4 ? lane : lane & 15u) : (lane >> 4) * 8 + (lane & 7u);
+            const uint32_t ku = F8 ? (KT == 4 ? 0u : lane >> 4) : (lane >> 3) & 1u;
+            const uint32_t kx = ka + kr * S::ROW + (S::ROW >= 128 ? ku ^ (kr & 7u) : ku ^ ((kr >> 1) & 3u)) * 16;
+            const uint32_t vr = lane & 15u, vu = lane >> 4;
+            const uint32_t vx = ka + CK * S::ROW + vr * S::ROW + (S::ROW >= 128 ? vu ^ (vr & 7u) : vu ^ ((vr >> 1) & 3u)) * 16;
             const int32_t key0 = (cons.row.c0 + from + (int32_t)(next - done)) * CK;
 
             /* scores: keys are the columns */
@@ -729,7 +806,8 @@ __global__ void __launch_bounds__(PK_WARPS * 32, 1) pk_attend_kernel(const __gri
                         if constexpr (REST) rest[mt][t][e] = 0.0f;
                     }
             auto score = [&](int mt, int t, const uint32_t *a, uint32_t b0, uint32_t b1) {
-                pk_mma<BF>(s[mt][t], a[0], a[1], a[2], a[3], b0, b1);
+                if constexpr (R == 1) pk_mma<BF>(s[mt][t], a[0], QP > 1 ? a[QW > 2 ? 2 : 0] : 0, a[1], QP > 1 ? a[QW > 2 ? 3 : 1] : 0, b0, b1);
+                else pk_mma<BF>(s[mt][t], a[0], a[1], a[2], a[3], b0, b1);
                 if constexpr (R == 1 && QP == 3) pk_mma<BF>(rest[mt][t], a[4], 0, a[5], 0, b0, b1);
                 if constexpr (R == 2 && QP > 1) pk_mma<BF>(rest[mt][t], a[4], a[5], a[6], a[7], b0, b1);
                 if constexpr (R == 2 && QP > 2) pk_mma<BF>(rest[mt][t], a[8], a[9], a[10], a[11], b0, b1);
@@ -747,8 +825,7 @@ __global__ void __launch_bounds__(PK_WARPS * 32, 1) pk_attend_kernel(const __gri
 #pragma unroll
                     for (int t = 0; t < KT; t += 2) {
                         uint32_t b[4];
-                        const uint32_t r = t * 8 + (lane >> 4) * 8 + (lane & 7u), u = ks * 2 + ((lane >> 3) & 1u);
-                        pk_ldm4(b, ka + r * S::ROW + (u ^ (r & 7u)) * 16);
+                        pk_ldm4(b, unit_at(kx, 2 * ks) + t * 8 * S::ROW);
 #pragma unroll
                         for (int mt = 0; mt < MT; mt++) {
                             score(mt, t, a[mt][0], b[0], b[1]);
@@ -758,8 +835,7 @@ __global__ void __launch_bounds__(PK_WARPS * 32, 1) pk_attend_kernel(const __gri
                 } else if constexpr (KT == 4) {
                     /* a matrix is 8 keys x 16 bytes */
                     uint32_t b[4];
-                    const uint32_t sw = S::ROW >= 128 ? (uint32_t)ks ^ (lane & 7u) : (uint32_t)ks ^ ((lane >> 1) & 3u);
-                    pk_ldm4(b, ka + lane * S::ROW + sw * 16);
+                    pk_ldm4(b, unit_at(kx, ks));
 #pragma unroll
                     for (int t = 0; t < 4; t++) {
                         const uint32_t b0 = pk_e4m3x2(b[t]), b1 = pk_e4m3x2(b[t] >> 16);
@@ -768,8 +844,7 @@ __global__ void __launch_bounds__(PK_WARPS * 32, 1) pk_attend_kernel(const __gri
                     }
                 } else {
                     uint32_t b[4];
-                    const uint32_t r = lane & 15u, u = ks + (lane >> 4);
-                    pk_ldm4(b, ka + r * S::ROW + (u ^ (r & 7u)) * 16);
+                    pk_ldm4(b, unit_at(kx, ks));
 #pragma unroll
                     for (int t = 0; t < 4; t++) {
                         const uint32_t b0 = pk_e4m3x2(b[t]), b1 = pk_e4m3x2(b[t] >> 16);
@@ -797,8 +872,9 @@ __global__ void __launch_bounds__(PK_WARPS * 32, 1) pk_attend_kernel(const __gri
 #pragma unroll
                         for (int e = 0; e < 2; e++) {
                             float x = s[mt][t][2 * r + e];
-                            if constexpr (R == 1) x = pk_fold(x, QP == 3 ? s[mt][t][e + 2] + rest[0][t][e] : s[mt][t][e + 2]);
-                            else if constexpr (QP > 1) x = pk_fold(x, rest[mt][t][2 * r + e]);
+                            if constexpr (R == 1 && QP > 1)
+                                x = pk_fold(x, QP == 3 ? s[mt][t][e + 2] + rest[0][t][e] : s[mt][t][e + 2]);
+                            if constexpr (R == 2 && QP > 1) x = pk_fold(x, rest[mt][t][2 * r + e]);
                             x *= unit[y];
                             if (!whole) {
                                 const int32_t k = t * 8 + 2 * (int32_t)c + e;
@@ -812,7 +888,7 @@ __global__ void __launch_bounds__(PK_WARPS * 32, 1) pk_attend_kernel(const __gri
                     top = fmaxf(top, m[y]);
                     /* weights are relative to the maximum less LIFT; nothing seen yet: every weight is 0 */
                     const float zero = (top == -INFINITY ? 0.0f : top) - LIFT;
-                    keep[r] = exp2f(m[y] - LIFT - zero);
+                    keep[r] = pk_exp2(m[y] - LIFT - zero);
                     moved |= top != m[y];
                     m[y] = top;
                     l[y] *= keep[r];
@@ -820,7 +896,7 @@ __global__ void __launch_bounds__(PK_WARPS * 32, 1) pk_attend_kernel(const __gri
                     for (int t = 0; t < KT; t++)
 #pragma unroll
                         for (int e = 0; e < 2; e++) {
-                            p[r][t][e] = exp2f(p[r][t][e] - zero);
+                            p[r][t][e] = pk_exp2(p[r][t][e] - zero);
                             l[y] += p[r][t][e];
                         }
                 }
@@ -833,20 +909,20 @@ __global__ void __launch_bounds__(PK_WARPS * 32, 1) pk_attend_kernel(const __gri
                 for (int kt = 0; kt < KT / 2; kt++) {
                     uint32_t *a = pa[mt][kt];
                     if constexpr (R == 1) {
-                        a[0] = pk_split<BF>(p[0][2 * kt][0], p[0][2 * kt][1]);
-                        a[2] = pk_split<BF>(p[0][2 * kt + 1][0], p[0][2 * kt + 1][1]);
-                        a[1] = pk_split<BF>(p[0][2 * kt][0], p[0][2 * kt][1]);
-                        a[3] = pk_split<BF>(p[0][2 * kt + 1][0], p[0][2 * kt + 1][1]);
+                        a[0] = pk_split<BF, false>(p[0][2 * kt][0], p[0][2 * kt][1]);
+                        a[2] = pk_split<BF, false>(p[0][2 * kt + 1][0], p[0][2 * kt + 1][1]);
+                        a[1] = pk_split<BF, false>(p[0][2 * kt][0], p[0][2 * kt][1]);
+                        a[3] = pk_split<BF, false>(p[0][2 * kt + 1][0], p[0][2 * kt + 1][1]);
                         if constexpr (PP == 3) {
-                            a[4] = pk_split<BF>(p[0][2 * kt][0], p[0][2 * kt][1]);
-                            a[5] = pk_split<BF>(p[0][2 * kt + 1][0], p[0][2 * kt + 1][1]);
+                            a[4] = pk_split<BF, false>(p[0][2 * kt][0], p[0][2 * kt][1]);
+                            a[5] = pk_split<BF, false>(p[0][2 * kt + 1][0], p[0][2 * kt + 1][1]);
                         }
                     } else {
 #pragma unroll
                         for (int q = 0; q < PP; q++)
 #pragma unroll
                             for (int e = 0; e < 4; e++)
-                                a[4 * q + e] = pk_split<BF>(p[e & 1][2 * kt + (e >> 1)][0], p[e & 1][2 * kt + (e >> 1)][1]);
+                                a[4 * q + e] = pk_split<BF, false>(p[e & 1][2 * kt + (e >> 1)][0], p[e & 1][2 * kt + (e >> 1)][1]);
                     }
                 }
             }
@@ -863,12 +939,10 @@ __global__ void __launch_bounds__(PK_WARPS * 32, 1) pk_attend_kernel(const __gri
 #pragma unroll
             for (int kt = 0; kt < KT / 2; kt++) {
                 /* matrices (keys 0-7, unit u), (keys 8-15, u), (0-7, u + 1), (8-15, u + 1) */
-                const uint32_t r = kt * 16 + (lane & 15u), up = lane >> 4;
 #pragma unroll
                 for (int u = 0; u < S::UNITS; u += 2) {
                     uint32_t b[4];
-                    const uint32_t sw = S::ROW >= 128 ? (u + up) ^ (r & 7u) : (u + up) ^ ((r >> 1) & 3u);
-                    pk_ldm4t(b, va + r * S::ROW + sw * 16);
+                    pk_ldm4t(b, unit_at(vx, u) + kt * 16 * S::ROW);
                     if constexpr (!F8) {
                         weigh(u, kt, b[0], b[1]);
                         weigh(u + 1, kt, b[2], b[3]);
@@ -946,54 +1020,60 @@ __global__ void __launch_bounds__(PK_WARPS * 32, 1) pk_attend_kernel(const __gri
                 for (uint32_t k = 0; k < PK_WARPS; k++) top = fmaxf(top, wml[k][y * 8 + g][0]);
                 const float zero = top == -INFINITY ? 0.0f : top;
 #pragma unroll
-                for (uint32_t k = 0; k < PK_WARPS; k++) sum += wml[k][y * 8 + g][1] * exp2f(wml[k][y * 8 + g][0] - zero);
-                const float keep = drop * exp2f(m[y] - zero);
+                for (uint32_t k = 0; k < PK_WARPS; k++) sum += wml[k][y * 8 + g][1] * pk_exp2(wml[k][y * 8 + g][0] - zero);
+                const float keep = drop * pk_exp2(m[y] - zero);
                 if (w == 0 && c == 0) *(float2 *)fml[y * 8 + g] = make_float2(top, sum);
                 auto place = [&](uint32_t owner, uint32_t source, int tq) {
                     return join + ((owner * 3 + source) * 8 + g) * S::QROW + tq * 8 + RUN * c;
                 };
 #pragma unroll
-                for (uint32_t q = 0; q < 4; q++)
-                    if (q != w)
+                for (int pass = 0; pass < S::PASSES; pass++) {
+                    constexpr int PT = QT / S::PASSES;    /* tiles of a quarter in a pass */
+                    if (pass) __syncthreads();
 #pragma unroll
-                        for (int t = 0; t < QT; t += RUN / 2) {
-                            float x[RUN], *d = place(q, w < q ? w : w - 1, t);
-                            columns(y, q * QT + t, keep, x);
-                            if constexpr (F8) *(float4 *)d = make_float4(x[0], x[1], x[RUN - 2], x[RUN - 1]);
-                            else *(float2 *)d = make_float2(x[0], x[1]);
-                        }
-                __syncthreads();
+                    for (uint32_t q = 0; q < 4; q++)
+                        if (q != w)
 #pragma unroll
-                for (uint32_t q = 0; q < 4; q++)
-                    if (q == w)
-#pragma unroll
-                        for (int t = 0; t < QT; t += RUN / 2) {
-                            float own[RUN], x[RUN], *d = place(q, 0, t);
-                            columns(y, q * QT + t, keep, own);
-#pragma unroll
-                            for (int e = 0; e < RUN; e++) {
-                                x[e] = 0.0f;
-#pragma unroll
-                                for (uint32_t k = 0; k < 4; k++) x[e] += k == q ? own[e] : place(q, k < q ? k : k - 1, t)[e];
+                            for (int t = 0; t < PT; t += RUN / 2) {
+                                float x[RUN], *d = place(q, w < q ? w : w - 1, t);
+                                columns(y, q * QT + pass * PT + t, keep, x);
+                                if constexpr (F8) *(float4 *)d = make_float4(x[0], x[1], x[RUN - 2], x[RUN - 1]);
+                                else *(float2 *)d = make_float2(x[0], x[1]);
                             }
+                    __syncthreads();
 #pragma unroll
-                            for (int e = 0; e < RUN; e++) d[e] = x[e];
-                        }
-                __syncthreads();
+                    for (uint32_t q = 0; q < 4; q++)
+                        if (q == w)
+#pragma unroll
+                            for (int t = 0; t < PT; t += RUN / 2) {
+                                float own[RUN], x[RUN], *d = place(q, 0, t);
+                                columns(y, q * QT + pass * PT + t, keep, own);
+#pragma unroll
+                                for (int e = 0; e < RUN; e++) {
+                                    x[e] = 0.0f;
+#pragma unroll
+                                    for (uint32_t k = 0; k < 4; k++) x[e] += k == q ? own[e] : place(q, k < q ? k : k - 1, t)[e];
+                                }
+#pragma unroll
+                                for (int e = 0; e < RUN; e++) d[e] = x[e];
+                            }
+                    __syncthreads();
 
-                /* out, or into the workspace */
-                for (uint32_t i = tid; i < 8 * DP / 4; i += PK_WARPS * 32) {
-                    const uint32_t hh = i / (DP / 4), col = i % (DP / 4) * 4, q = col / (DP / 4);
-                    float4 x = *(const float4 *)(join + ((q * 3) * 8 + hh) * S::QROW + col % (DP / 4));
-                    const uint32_t head = y * 8 + hh;
-                    if (cut) {
-                        __stcg((float4 *)(part + 2 * HEADS + head * DP + col), x);
-                        if (col == 0) __stcg((float2 *)(part + 2 * head), make_float2(fml[head][0], fml[head][1]));
-                    } else if (v0 + head < J.rows && col < J.D.head_dim) {
-                        const float by = pk_finish(J, cons.b, cons.row.len, cons.hk, v0 + head, fml[head][0], fml[head][1],
-                                                   col == 0);
-                        const float z[4] = {x.x * by, x.y * by, x.z * by, x.w * by};
-                        pk_put<4>(J, cons.b, cons.hk, v0 + head, col, z);
+                    /* out, or into the workspace */
+                    constexpr uint32_t C4 = S::QCOLS;     /* runs of 4 columns of a row in a pass, all quarters */
+                    for (uint32_t i = tid; i < 8 * C4; i += PK_WARPS * 32) {
+                        const uint32_t hh = i / C4, q = i % C4 / (C4 / 4), in = i % (C4 / 4) * 4;
+                        const uint32_t col = q * (DP / 4) + pass * S::QCOLS + in, head = y * 8 + hh;
+                        const float4 x = *(const float4 *)(join + ((q * 3) * 8 + hh) * S::QROW + in);
+                        if (cut) {
+                            __stcg((float4 *)(part + 2 * HEADS + head * DP + col), x);
+                            if (col == 0) __stcg((float2 *)(part + 2 * head), make_float2(fml[head][0], fml[head][1]));
+                        } else if (v0 + head < J.rows && col < J.D.head_dim) {
+                            const float by = pk_finish(J, cons.b, cons.row.len, cons.hk, v0 + head, fml[head][0],
+                                                       fml[head][1], col == 0);
+                            const float z[4] = {x.x * by, x.y * by, x.z * by, x.w * by};
+                            pk_put<4>(J, cons.b, cons.hk, v0 + head, col, z);
+                        }
                     }
                 }
             }
@@ -1028,7 +1108,7 @@ __global__ void __launch_bounds__(PK_WARPS * 32, 1) pk_attend_kernel(const __gri
 
 template <uint32_t CT, int DP, int R, int MT, int QP>
 static int pk_attend_launch(const pk_attend_job &J, uint32_t grid, cudaStream_t st) {
-    typedef pk_shape<CT, DP> S;
+    typedef pk_shape<CT, DP, R, MT, QP> S;
     static uint64_t done = 0;
     constexpr uint32_t smem = PK_WARPS * S::RING + S::JOIN;
     auto kernel = pk_attend_kernel<CT, DP, R, MT, QP>;
@@ -1047,10 +1127,7 @@ pk_attend_fn pk_attend_e4m3(int dp, int r, int mt, bool wide);
 template <uint32_t CT, int DP>
 static pk_attend_fn pk_attend_pick_at(int r, int mt, bool wide) {
     constexpr int MOST = CT == PULSAR_TYPE_BF16 ? 3 : 2; /* parts of wide q */
-    if (r == 1) {
-        if (MOST == 3 && wide) return pk_attend_launch<CT, DP, 1, 1, MOST>;
-        return pk_attend_launch<CT, DP, 1, 1, 2>; /* the second part is free */
-    }
+    if (r == 1) return wide ? pk_attend_launch<CT, DP, 1, 1, MOST> : pk_attend_launch<CT, DP, 1, 1, 1>;
     if (wide) return pk_attend_launch<CT, DP, 2, 1, MOST>;
     if constexpr (DP <= 128)
         if (mt == 2) return pk_attend_launch<CT, DP, 2, 2, 1>;
