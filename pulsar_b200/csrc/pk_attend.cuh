@@ -108,12 +108,12 @@ template <bool BF>
 __device__ __forceinline__ void pk_mma(float *c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                        uint32_t b1) {
     if constexpr (BF)
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
                      "{%0,%1,%2,%3};"
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
     else
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
                      "{%0,%1,%2,%3};"
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
@@ -391,78 +391,95 @@ __device__ __forceinline__ bool pk_joint_arrive(const pk_attend_job &J, const pk
 }
 
 /* sums of `count` parts (step apart) from `first` on, in their order; done by
- * the CTA that completed them.  A thread has the loads of 8 parts in flight. */
-template <int DP, int HEADS>
+ * the CTA that completed them.  The parts come through `room` (PARTS of them
+ * at a time) by asynchronous copies, so that one latency serves many. */
+template <int DP, int HEADS, int PARTS>
 __device__ void pk_join(const pk_attend_job &J, const pk_joint &S, uint32_t first, uint32_t step, uint32_t count,
-                        bool final, float (*ml)[2]) {
-    constexpr uint64_t FLOATS = (uint64_t)HEADS * (DP + 2);
-    for (uint32_t x = threadIdx.x; x < HEADS * DP / 4; x += PK_WARPS * 32) {
-        const uint32_t head = x / (DP / 4), col = x % (DP / 4) * 4;
-        float top = -INFINITY, sum = 0.0f, acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (uint32_t k0 = 0; k0 < count; k0 += 8) {
-            float2 m8[8];
-            float4 v8[8];
+                        bool final, float (*ml)[2], float *room) {
+    constexpr uint32_t FLOATS = HEADS * (DP + 2), THREADS = PK_WARPS * 32;
+    constexpr int NX = HEADS * DP / 4 / THREADS; /* runs of four columns a thread sums */
+    static_assert(NX * 4 * THREADS == HEADS * DP && PARTS > 0, "tiles are whole numbers of threads");
+    float4 acc[NX];
 #pragma unroll
-            for (uint32_t k = 0; k < 8; k++) {
-                m8[k] = make_float2(-INFINITY, 0.0f);
-                v8[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                if (k0 + k < count) {
-                    const float *p = J.parts + S.slot(first + (k0 + k) * step) * FLOATS;
-                    m8[k] = __ldcg((const float2 *)(p + 2 * head));
-                    v8[k] = __ldcg((const float4 *)(p + 2 * HEADS + head * DP + col));
-                }
-            }
-            float t = top;
-#pragma unroll
-            for (uint32_t k = 0; k < 8; k++) t = fmaxf(t, m8[k].x);
-            const float zero = t == -INFINITY ? 0.0f : t, keep = pk_exp2(top - zero);
-            top = t;
-            sum *= keep;
-#pragma unroll
-            for (int e = 0; e < 4; e++) acc[e] *= keep;
-#pragma unroll
-            for (uint32_t k = 0; k < 8; k++) {
-                const float f = pk_exp2(m8[k].x - zero);
-                sum += m8[k].y * f;
-                acc[0] += v8[k].x * f;
-                acc[1] += v8[k].y * f;
-                acc[2] += v8[k].z * f;
-                acc[3] += v8[k].w * f;
-            }
+    for (int n = 0; n < NX; n++) acc[n] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (threadIdx.x < HEADS) {
+        ml[threadIdx.x][0] = -INFINITY;
+        ml[threadIdx.x][1] = 0.0f;
+    }
+    for (uint32_t k0 = 0; k0 < count; k0 += PARTS) {
+        const uint32_t m = count - k0 < PARTS ? count - k0 : PARTS;
+        for (uint32_t k = 0; k < m; k++) {
+            const float *p = J.parts + S.slot(first + (k0 + k) * step) * (uint64_t)FLOATS;
+            for (uint32_t x = threadIdx.x; x < FLOATS / 4; x += THREADS)
+                pk_cp16(pk_saddr(room + k * FLOATS + 4 * x), p + 4 * x, true);
         }
-        if (final) {
-            const uint32_t v = S.v0 + head;
-            if (v < J.rows && col < J.D.head_dim) {
-                const float by = pk_finish(J, S.b, S.len, S.hk, v, top, sum, col == 0);
+        pk_cp_commit();
+        pk_cp_wait<0>();
+        __syncthreads();
+        /* each part's maximum becomes its factor, part 0's sum what is kept of the sums so far */
+        if (threadIdx.x < HEADS) {
+            float *f = room + 2 * threadIdx.x, old = ml[threadIdx.x][0], top = old, sum;
+            for (uint32_t k = 0; k < m; k++) top = fmaxf(top, f[k * FLOATS]);
+            const float zero = top == -INFINITY ? 0.0f : top;
+            sum = ml[threadIdx.x][1] * pk_exp2(old - zero);
+            for (uint32_t k = 0; k < m; k++) {
+                const float by = pk_exp2(f[k * FLOATS] - zero);
+                sum += by * f[k * FLOATS + 1];
+                f[k * FLOATS] = by;
+            }
+            f[1] = pk_exp2(old - zero);
+            ml[threadIdx.x][0] = top;
+            ml[threadIdx.x][1] = sum;
+        }
+        __syncthreads();
 #pragma unroll
-                for (int e = 0; e < 4; e++) acc[e] *= by;
-                pk_put<4>(J, S.b, S.hk, v, col, acc);
+        for (int n = 0; n < NX; n++) {
+            const float keep = room[2 * ((n * THREADS + threadIdx.x) / (DP / 4)) + 1];
+            acc[n].x *= keep;
+            acc[n].y *= keep;
+            acc[n].z *= keep;
+            acc[n].w *= keep;
+        }
+#pragma unroll 2
+        for (uint32_t k = 0; k < m; k++)
+#pragma unroll
+            for (int n = 0; n < NX; n++) {
+                const uint32_t x = n * THREADS + threadIdx.x;
+                const float by = room[k * FLOATS + 2 * (x / (DP / 4))];
+                const float4 v = *(const float4 *)(room + k * FLOATS + 2 * HEADS + 4 * x);
+                acc[n].x += v.x * by;
+                acc[n].y += v.y * by;
+                acc[n].z += v.z * by;
+                acc[n].w += v.w * by;
             }
-        } else {
-            __stcg((float4 *)(J.parts + S.slot(first) * FLOATS + 2 * HEADS + head * DP + col),
-                   make_float4(acc[0], acc[1], acc[2], acc[3]));
-            if (col == 0) {
-                ml[head][0] = top;
-                ml[head][1] = sum;
-            }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int n = 0; n < NX; n++) {
+        const uint32_t x = n * THREADS + threadIdx.x, head = x / (DP / 4), col = x % (DP / 4) * 4, v = S.v0 + head;
+        if (!final) {
+            __stcg((float4 *)(J.parts + S.slot(first) * (uint64_t)FLOATS + 2 * HEADS + 4 * x), acc[n]);
+        } else if (v < J.rows && col < J.D.head_dim) {
+            const float by = pk_finish(J, S.b, S.len, S.hk, v, ml[head][0], ml[head][1], col == 0);
+            const float y[4] = {acc[n].x * by, acc[n].y * by, acc[n].z * by, acc[n].w * by};
+            pk_put<4>(J, S.b, S.hk, v, col, y);
         }
     }
 }
 
 /* the join of a segment by the CTA that completed its group */
-template <int DP, int HEADS>
-__device__ void pk_joint_finish(const pk_attend_job &J, const pk_joint &S, uint32_t *last, float (*ml)[2]) {
+template <int DP, int HEADS, int PARTS>
+__device__ void pk_joint_finish(const pk_attend_job &J, const pk_joint &S, uint32_t *last, float (*ml)[2], float *room) {
     const uint32_t n = S.w1 - S.w0 + 1, groups = (n + PK_GROUP - 1) / PK_GROUP;
     const uint32_t first = (blockIdx.x - S.w0) / PK_GROUP * PK_GROUP;
     __syncthreads();
-    pk_join<DP, HEADS>(J, S, first, 1, n - first < PK_GROUP ? n - first : PK_GROUP, groups == 1, ml);
+    pk_join<DP, HEADS, PARTS>(J, S, first, 1, n - first < PK_GROUP ? n - first : PK_GROUP, groups == 1, ml, room);
     if (groups == 1) return;
-    __syncthreads(); /* part `first`'s maxima and sums have been read, the new ones are in ml */
     if (threadIdx.x < HEADS)
         __stcg((float2 *)(J.parts + S.slot(first) * (uint64_t)(HEADS * (DP + 2)) + 2 * threadIdx.x),
                make_float2(ml[threadIdx.x][0], ml[threadIdx.x][1]));
     if (pk_arrive(J.counters + 2 * PK_MAX_WORKERS + S.slot(0), groups, last))
-        pk_join<DP, HEADS>(J, S, 0, PK_GROUP, groups, true, ml);
+        pk_join<DP, HEADS, PARTS>(J, S, 0, PK_GROUP, groups, true, ml, room);
 }
 
 /* ------------------------------------------------------------ the kernel */
@@ -479,7 +496,7 @@ __global__ void __launch_bounds__(PK_WARPS * 32, pk_shape<CT, DP, R, MT, QP>::OC
     constexpr int PP = QP == 3 ? 3 : 2;                   /* parts of p */
     constexpr int PW = R == 1 ? (PP == 3 ? 6 : 4) : 4 * PP;
     constexpr bool REST = R == 1 ? QP == 3 : QP > 1;      /* lower parts of q have sums of their own */
-    constexpr float LIFT = BF ? 0.0f : 15.0f;
+    constexpr float LIFT = BF ? 0.0f : 7.0f, SLACK = 8.0f; /* see the running maximum below */
 
     extern __shared__ __align__(128) uint8_t smem[];
     uint8_t *ring = smem + (threadIdx.x >> 5) * S::RING;
@@ -651,8 +668,9 @@ __global__ void __launch_bounds__(PK_WARPS * 32, pk_shape<CT, DP, R, MT, QP>::OC
     uint32_t stage = 0;
     uint32_t done = 0;                                    /* slice offset where the segment at hand begins */
     uint32_t next = lead;                                 /* slice offset of this warp's next chunk */
-    pk_joint owed;                                        /* a join that this CTA completed, put off to the end */
-    bool owes = false;
+    pk_joint owed, joint;                                 /* joins that this CTA completed (a slice cuts two
+                                                           * segments at most), put off to the slice's end */
+    bool owes = false, also = false;
 
     while (done < slice) {
         const int32_t from = cons.pos;                    /* chunks [from, to) of this segment are ours */
@@ -795,7 +813,8 @@ __global__ void __launch_bounds__(PK_WARPS * 32, pk_shape<CT, DP, R, MT, QP>::OC
             const int32_t key0 = (cons.row.c0 + from + (int32_t)(next - done)) * CK;
 
             /* scores: keys are the columns */
-            float s[MT][KT][4], rest[REST ? MT : 1][KT][4];
+            constexpr int CHAINS = MT == 1 && KT == 2 ? 2 : 1; /* two columns of sums alone would wait on themselves */
+            float s[MT][KT][4], rest[REST ? MT : 1][KT][4], odd[CHAINS == 2 ? KT : 1][4];
 #pragma unroll
             for (int mt = 0; mt < MT; mt++)
 #pragma unroll
@@ -803,11 +822,13 @@ __global__ void __launch_bounds__(PK_WARPS * 32, pk_shape<CT, DP, R, MT, QP>::OC
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
                         s[mt][t][e] = 0.0f;
+                        if constexpr (CHAINS == 2) odd[t][e] = 0.0f;
                         if constexpr (REST) rest[mt][t][e] = 0.0f;
                     }
-            auto score = [&](int mt, int t, const uint32_t *a, uint32_t b0, uint32_t b1) {
-                if constexpr (R == 1) pk_mma<BF>(s[mt][t], a[0], QP > 1 ? a[QW > 2 ? 2 : 0] : 0, a[1], QP > 1 ? a[QW > 2 ? 3 : 1] : 0, b0, b1);
-                else pk_mma<BF>(s[mt][t], a[0], a[1], a[2], a[3], b0, b1);
+            auto score = [&](int mt, int t, int ks, const uint32_t *a, uint32_t b0, uint32_t b1) {
+                float *sum = CHAINS == 2 && (ks & 1) ? odd[CHAINS == 2 ? t : 0] : s[mt][t];
+                if constexpr (R == 1) pk_mma<BF>(sum, a[0], QP > 1 ? a[QW > 2 ? 2 : 0] : 0, a[1], QP > 1 ? a[QW > 2 ? 3 : 1] : 0, b0, b1);
+                else pk_mma<BF>(sum, a[0], a[1], a[2], a[3], b0, b1);
                 if constexpr (R == 1 && QP == 3) pk_mma<BF>(rest[mt][t], a[4], 0, a[5], 0, b0, b1);
                 if constexpr (R == 2 && QP > 1) pk_mma<BF>(rest[mt][t], a[4], a[5], a[6], a[7], b0, b1);
                 if constexpr (R == 2 && QP > 2) pk_mma<BF>(rest[mt][t], a[8], a[9], a[10], a[11], b0, b1);
@@ -828,8 +849,8 @@ __global__ void __launch_bounds__(PK_WARPS * 32, pk_shape<CT, DP, R, MT, QP>::OC
                         pk_ldm4(b, unit_at(kx, 2 * ks) + t * 8 * S::ROW);
 #pragma unroll
                         for (int mt = 0; mt < MT; mt++) {
-                            score(mt, t, a[mt][0], b[0], b[1]);
-                            score(mt, t + 1, a[mt][0], b[2], b[3]);
+                            score(mt, t, ks, a[mt][0], b[0], b[1]);
+                            score(mt, t + 1, ks, a[mt][0], b[2], b[3]);
                         }
                     }
                 } else if constexpr (KT == 4) {
@@ -840,7 +861,7 @@ __global__ void __launch_bounds__(PK_WARPS * 32, pk_shape<CT, DP, R, MT, QP>::OC
                     for (int t = 0; t < 4; t++) {
                         const uint32_t b0 = pk_e4m3x2(b[t]), b1 = pk_e4m3x2(b[t] >> 16);
 #pragma unroll
-                        for (int mt = 0; mt < MT; mt++) score(mt, t, a[mt][0], b0, b1);
+                        for (int mt = 0; mt < MT; mt++) score(mt, t, ks, a[mt][0], b0, b1);
                     }
                 } else {
                     uint32_t b[4];
@@ -849,92 +870,120 @@ __global__ void __launch_bounds__(PK_WARPS * 32, pk_shape<CT, DP, R, MT, QP>::OC
                     for (int t = 0; t < 4; t++) {
                         const uint32_t b0 = pk_e4m3x2(b[t]), b1 = pk_e4m3x2(b[t] >> 16);
 #pragma unroll
-                        for (int mt = 0; mt < MT; mt++) score(mt, t & 1, a[mt][KQ - 1 < (t >> 1) ? 0 : t >> 1], b0, b1);
+                        for (int mt = 0; mt < MT; mt++) score(mt, t & 1, t >> 1, a[mt][KQ - 1 < (t >> 1) ? 0 : t >> 1], b0, b1);
                     }
                 }
             }
 
-            /* fold the parts, mask, running maximum and sum (a lane has columns 2c, 2c + 1 of its rows); p's
-             * parts are the left factors of the output products in the layout that they already have */
+            /* Fold the parts and mask (a lane has columns 2c, 2c + 1 of its rows).  m is the running maximum but
+             * for SLACK: it moves, and the sums with it, only where the maximum has outgrown it by 2^SLACK.
+             * Weights are relative to m less LIFT: at most 2^15, so that f16 holds them, and small ones stay
+             * clear of its subnormals.  p's parts are the left factors of the output products in the layout that
+             * they already have. */
+            float top[LR];
+            bool moved = false;
+#pragma unroll
+            for (int y = 0; y < LR; y++) {
+                constexpr uint32_t ALL = CK == 32 ? ~0u : (1u << (CK & 31)) - 1u;
+                const int mt = y / R, r = y % R;
+                const bool whole = there == ALL && key0 >= slo[y] && key0 + CK <= shi[y];
+                top[y] = -INFINITY;
+#pragma unroll
+                for (int t = 0; t < KT; t++)
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        float &x = s[mt][t][2 * r + e];
+                        if constexpr (CHAINS == 2) x += odd[t][2 * r + e];
+                        if constexpr (R == 1 && QP > 1) {
+                            float low = s[mt][t][e + 2];
+                            if constexpr (CHAINS == 2) low += odd[t][e + 2];
+                            x = pk_fold(x, QP == 3 ? low + rest[0][t][e] : low);
+                        }
+                        if constexpr (R == 2 && QP > 1) x = pk_fold(x, rest[mt][t][2 * r + e]);
+                        x *= unit[y];
+                        if (!whole) {
+                            const int32_t k = t * 8 + 2 * (int32_t)c + e;
+                            if (!(there >> k & 1u) || key0 + k < slo[y] || key0 + k >= shi[y]) x = -INFINITY;
+                        }
+                        top[y] = fmaxf(top[y], x);
+                    }
+            }
+#pragma unroll
+            for (int o2 = 1; o2 < 4; o2 <<= 1)
+#pragma unroll
+                for (int y = 0; y < LR; y++) top[y] = fmaxf(top[y], __shfl_xor_sync(~0u, top[y], o2));
+#pragma unroll
+            for (int y = 0; y < LR; y++) moved |= top[y] > m[y] + SLACK;
+            if (__any_sync(~0u, moved)) {
+#pragma unroll
+                for (int y = 0; y < LR; y++) {
+                    const float to = top[y] > m[y] + SLACK ? top[y] : m[y];
+                    const float keep = to == m[y] ? 1.0f : pk_exp2(m[y] - to);
+                    m[y] = to;
+                    l[y] *= keep;
+#pragma unroll
+                    for (int t = 0; t < NT; t++) {
+                        if constexpr (R == 1) {
+#pragma unroll
+                            for (int e = 0; e < 4; e++) o[y][t][e] *= keep;
+                        } else {
+                            o[y / R][t][2 * (y % R)] *= keep;
+                            o[y / R][t][2 * (y % R) + 1] *= keep;
+                        }
+                    }
+                }
+            }
             uint32_t pa[MT][KT / 2][PW];
 #pragma unroll
-            for (int mt = 0; mt < MT; mt++) {
-                float p[R][KT][2], keep[R];
-                bool moved = false;
+            for (int y = 0; y < LR; y++) {
+                const float zero = (m[y] == -INFINITY ? 0.0f : m[y]) - LIFT; /* nothing seen yet: every weight is 0 */
 #pragma unroll
-                for (int r = 0; r < R; r++) {
-                    const int y = mt * R + r;
-                    const bool whole = there == (CK == 32 ? ~0u : (1u << (CK & 31)) - 1u) && key0 >= slo[y] &&
-                                       key0 + CK <= shi[y];
-                    float top = -INFINITY;
+                for (int t = 0; t < KT; t++)
 #pragma unroll
-                    for (int t = 0; t < KT; t++)
+                    for (int e = 0; e < 2; e++) {
+                        float &x = s[y / R][t][2 * (y % R) + e];
+                        x = pk_exp2(x - zero);
+                        l[y] += x;
+                    }
+            }
 #pragma unroll
-                        for (int e = 0; e < 2; e++) {
-                            float x = s[mt][t][2 * r + e];
-                            if constexpr (R == 1 && QP > 1)
-                                x = pk_fold(x, QP == 3 ? s[mt][t][e + 2] + rest[0][t][e] : s[mt][t][e + 2]);
-                            if constexpr (R == 2 && QP > 1) x = pk_fold(x, rest[mt][t][2 * r + e]);
-                            x *= unit[y];
-                            if (!whole) {
-                                const int32_t k = t * 8 + 2 * (int32_t)c + e;
-                                if (!(there >> k & 1u) || key0 + k < slo[y] || key0 + k >= shi[y]) x = -INFINITY;
-                            }
-                            p[r][t][e] = x;
-                            top = fmaxf(top, x);
-                        }
-                    top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
-                    top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
-                    top = fmaxf(top, m[y]);
-                    /* weights are relative to the maximum less LIFT; nothing seen yet: every weight is 0 */
-                    const float zero = (top == -INFINITY ? 0.0f : top) - LIFT;
-                    keep[r] = pk_exp2(m[y] - LIFT - zero);
-                    moved |= top != m[y];
-                    m[y] = top;
-                    l[y] *= keep[r];
-#pragma unroll
-                    for (int t = 0; t < KT; t++)
-#pragma unroll
-                        for (int e = 0; e < 2; e++) {
-                            p[r][t][e] = pk_exp2(p[r][t][e] - zero);
-                            l[y] += p[r][t][e];
-                        }
-                }
-                if (__any_sync(~0u, moved))
-#pragma unroll
-                    for (int t = 0; t < NT; t++)
-#pragma unroll
-                        for (int e = 0; e < 4; e++) o[mt][t][e] *= keep[R == 1 ? 0 : e >> 1];
+            for (int mt = 0; mt < MT; mt++)
 #pragma unroll
                 for (int kt = 0; kt < KT / 2; kt++) {
                     uint32_t *a = pa[mt][kt];
                     if constexpr (R == 1) {
-                        a[0] = pk_split<BF, false>(p[0][2 * kt][0], p[0][2 * kt][1]);
-                        a[2] = pk_split<BF, false>(p[0][2 * kt + 1][0], p[0][2 * kt + 1][1]);
-                        a[1] = pk_split<BF, false>(p[0][2 * kt][0], p[0][2 * kt][1]);
-                        a[3] = pk_split<BF, false>(p[0][2 * kt + 1][0], p[0][2 * kt + 1][1]);
+                        float *p0 = s[mt][2 * kt], *p1 = s[mt][2 * kt + 1];
+                        a[0] = pk_split<BF, false>(p0[0], p0[1]);
+                        a[2] = pk_split<BF, false>(p1[0], p1[1]);
+                        a[1] = pk_split<BF, false>(p0[0], p0[1]);
+                        a[3] = pk_split<BF, false>(p1[0], p1[1]);
                         if constexpr (PP == 3) {
-                            a[4] = pk_split<BF, false>(p[0][2 * kt][0], p[0][2 * kt][1]);
-                            a[5] = pk_split<BF, false>(p[0][2 * kt + 1][0], p[0][2 * kt + 1][1]);
+                            a[4] = pk_split<BF, false>(p0[0], p0[1]);
+                            a[5] = pk_split<BF, false>(p1[0], p1[1]);
                         }
                     } else {
 #pragma unroll
                         for (int q = 0; q < PP; q++)
 #pragma unroll
-                            for (int e = 0; e < 4; e++)
-                                a[4 * q + e] = pk_split<BF, false>(p[e & 1][2 * kt + (e >> 1)][0], p[e & 1][2 * kt + (e >> 1)][1]);
+                            for (int e = 0; e < 4; e++) {
+                                float *z = s[mt][2 * kt + (e >> 1)] + 2 * (e & 1);
+                                a[4 * q + e] = pk_split<BF, false>(z[0], z[1]);
+                            }
                     }
                 }
-            }
-            auto weigh = [&](int t, int kt, uint32_t b0, uint32_t b1) {
+            /* output tiles t and t + 1; a part's products for all tiles before the next part's, which add to the same sums */
+            auto weigh = [&](int t, int kt, const uint32_t *b) {
+                constexpr int TIMES = R == 1 ? PP - 1 : PP;
 #pragma unroll
-                for (int mt = 0; mt < MT; mt++) {
-                    const uint32_t *a = pa[mt][kt];
-                    pk_mma<BF>(o[mt][t], a[0], a[1], a[2], a[3], b0, b1);
-                    if constexpr (R == 1 && PP == 3) pk_mma<BF>(o[mt][t], a[4], 0, a[5], 0, b0, b1);
-                    if constexpr (R == 2) pk_mma<BF>(o[mt][t], a[4], a[5], a[6], a[7], b0, b1);
-                    if constexpr (R == 2 && PP == 3) pk_mma<BF>(o[mt][t], a[8], a[9], a[10], a[11], b0, b1);
-                }
+                for (int q = 0; q < TIMES; q++)
+#pragma unroll
+                    for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+                        for (int x = 0; x < 2; x++) {
+                            const uint32_t *a = pa[mt][kt] + 4 * q;
+                            if (R == 1 && q == 1) pk_mma<BF>(o[mt][t + x], a[0], 0, a[PW > 5 ? 1 : 0], 0, b[2 * x], b[2 * x + 1]);
+                            else pk_mma<BF>(o[mt][t + x], a[0], a[1], a[2], a[3], b[2 * x], b[2 * x + 1]);
+                        }
             };
 #pragma unroll
             for (int kt = 0; kt < KT / 2; kt++) {
@@ -944,16 +993,15 @@ __global__ void __launch_bounds__(PK_WARPS * 32, pk_shape<CT, DP, R, MT, QP>::OC
                     uint32_t b[4];
                     pk_ldm4t(b, unit_at(vx, u) + kt * 16 * S::ROW);
                     if constexpr (!F8) {
-                        weigh(u, kt, b[0], b[1]);
-                        weigh(u + 1, kt, b[2], b[3]);
+                        weigh(u, kt, b);
                     } else {
                         /* a 16-bit column is two values: the even ones to tile 2u, the odd ones to 2u + 1 */
 #pragma unroll
                         for (int y = 0; y < 2; y++) {
                             const uint32_t x0 = b[2 * y], x1 = b[2 * y + 1];
-                            weigh(2 * (u + y), kt, pk_e4m3x2(__byte_perm(x0, 0, 0x0020)), pk_e4m3x2(__byte_perm(x1, 0, 0x0020)));
-                            weigh(2 * (u + y) + 1, kt, pk_e4m3x2(__byte_perm(x0, 0, 0x0031)),
-                                  pk_e4m3x2(__byte_perm(x1, 0, 0x0031)));
+                            const uint32_t z[4] = {pk_e4m3x2(__byte_perm(x0, 0, 0x0020)), pk_e4m3x2(__byte_perm(x1, 0, 0x0020)),
+                                                   pk_e4m3x2(__byte_perm(x0, 0, 0x0031)), pk_e4m3x2(__byte_perm(x1, 0, 0x0031))};
+                            weigh(2 * (u + y), kt, z);
                         }
                     }
                 }
@@ -989,7 +1037,7 @@ __global__ void __launch_bounds__(PK_WARPS * 32, pk_shape<CT, DP, R, MT, QP>::OC
             l[y] += __shfl_xor_sync(~0u, l[y], 1);
             l[y] += __shfl_xor_sync(~0u, l[y], 2);
         }
-        const float drop = BF ? 1.0f : 1.0f / 32768.0f;   /* 2^-LIFT */
+        const float drop = BF ? 1.0f : 1.0f / 128.0f;     /* 2^-LIFT */
         if (solo) {
 #pragma unroll
             for (int y = 0; y < LR; y++) {
@@ -1078,7 +1126,7 @@ __global__ void __launch_bounds__(PK_WARPS * 32, pk_shape<CT, DP, R, MT, QP>::OC
                 }
             }
             if (cut) {
-                /* a join that falls to this CTA waits for its slice's end: others may wait for the rest of it */
+                /* a join that falls to this CTA waits for its slice's end: other joins may wait for the rest of it */
                 const unsigned long long seg0 = lo + done - (uint32_t)from;
                 pk_joint S2;
                 S2.b = cons.b;
@@ -1089,11 +1137,12 @@ __global__ void __launch_bounds__(PK_WARPS * 32, pk_shape<CT, DP, R, MT, QP>::OC
                 S2.w1 = (uint32_t)((seg0 + (uint32_t)cons.row.n - 1) / per);
                 S2.inside = seg0 > per * S2.w0;
                 if (pk_joint_arrive(J, S2, &last)) {
-                    if (done + took < slice) {
-                        owed = S2;
-                        owes = true;
+                    if (owes) {
+                        also = true;
+                        joint = S2;
                     } else {
-                        pk_joint_finish<DP, HEADS>(J, S2, &last, fml);
+                        owes = true;
+                        owed = S2;
                     }
                 }
             }
@@ -1103,7 +1152,10 @@ __global__ void __launch_bounds__(PK_WARPS * 32, pk_shape<CT, DP, R, MT, QP>::OC
         if (done < slice) cons.step(J, cached, (int32_t)took);
     }
     pk_cp_wait<0>();
-    if (owes) pk_joint_finish<DP, HEADS>(J, owed, &last, fml);
+    /* the ring is free now */
+    constexpr int PARTS = PK_WARPS * S::RING / (HEADS * (DP + 2) * 4);
+    if (owes) pk_joint_finish<DP, HEADS, PARTS>(J, owed, &last, fml, (float *)smem);
+    if (also) pk_joint_finish<DP, HEADS, PARTS>(J, joint, &last, fml, (float *)smem);
 }
 
 template <uint32_t CT, int DP, int R, int MT, int QP>
