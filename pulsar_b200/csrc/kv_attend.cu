@@ -6,7 +6,7 @@
 struct pk_attend_plan {
     int dp, r, mt;           /* padded head width; the kernel's R and MT */
     bool wide;               /* q has more bits than one 16-bit part of the cache's kind holds */
-    uint32_t workers;
+    uint32_t workers, rows;  /* CTAs and sequences of a launch */
     size_t bytes;            /* of the workspace */
 };
 
@@ -47,11 +47,14 @@ static int pk_attend_prepare(const pulsar_kv_desc *d, const pulsar_kv_attend_arg
     /* CTAs that are resident together (pk_shape's OCC) */
     p->workers = pk_sm_count() * (p->dp == 256 ? 1 : PK_OCC);
     if (p->workers > PK_MAX_WORKERS) p->workers = PK_MAX_WORKERS;
-    /* no more CTAs than the longest rows could feed */
+    /* no more CTAs than the longest rows could feed; no more rows in a launch
+     * than a line of less than 2^32 chunks holds */
     uint64_t keys = (uint64_t)d->max_pages * d->page_size;
     if (a->window && keys > (uint64_t)a->window + a->n_q - 1) keys = (uint64_t)a->window + a->n_q - 1;
-    const uint64_t most = (uint64_t)a->n_rows * J->segs * (keys / ck + 2);
-    if (p->workers > most) p->workers = (uint32_t)most;
+    const uint64_t row = (uint64_t)J->segs * (keys / ck + 2);
+    if (row > 0x7fffffffull) return pk_refuse("kv attend: a row too long for its heads");
+    p->rows = 0xffffffffull / row < a->n_rows ? (uint32_t)(0xffffffffull / row) : a->n_rows;
+    if (p->workers > row * p->rows) p->workers = (uint32_t)(row * p->rows);
     p->bytes = PULSAR_KV_WS_ZEROED + 4ull * p->workers * 2 * heads * (p->dp + 2);
     return 1;
 }
@@ -81,5 +84,20 @@ extern "C" int pulsar_kv_attend(const pulsar_kv_desc *d, const pulsar_kv_attend_
     const pk_attend_fn f = d->dtype == PULSAR_TYPE_BF16  ? pk_attend_bf16(p.dp, p.r, p.mt, p.wide)
                            : d->dtype == PULSAR_TYPE_F16 ? pk_attend_f16(p.dp, p.r, p.mt, p.wide)
                                                          : pk_attend_e4m3(p.dp, p.r, p.mt, p.wide);
-    return f(J, p.workers, pk_stream(stream));
+    for (uint32_t r = 0; r < a->n_rows; r += p.rows) {
+        J.A.n_rows = a->n_rows - r < p.rows ? a->n_rows - r : p.rows;
+        if (!f(J, p.workers, pk_stream(stream))) return 0;
+        const uint64_t tok = (uint64_t)p.rows * a->n_q;
+        J.A.q = (const uint8_t *)J.A.q + tok * a->q_stride * pk_type_bytes(a->q_type);
+        J.A.out = (uint8_t *)J.A.out + tok * a->out_stride * pk_type_bytes(a->q_type);
+        if (J.A.lse) J.A.lse += tok * a->n_head;
+        J.A.lens += p.rows;
+        if (J.A.seq) {
+            J.A.seq += p.rows;
+        } else {
+            J.D.table += p.rows * J.D.table_stride;
+            J.D.n_rows -= p.rows;
+        }
+    }
+    return 1;
 }

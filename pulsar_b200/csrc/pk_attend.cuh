@@ -10,7 +10,8 @@
  * head) pairs; a tile is HEADS of them.  All (sequence, key head, tile)
  * segments lie one behind the other on a line, counted in chunks of CK keys,
  * and the workers take equal slices of it: no length, batch or head count
- * leaves SMs idle, and the host needs no lengths.  Long segments: a worker is
+ * leaves SMs idle, and the host needs no lengths (it only sees to it that the
+ * line stays below 2^32 chunks).  Long segments: a worker is
  * a CTA, whose four warps take the chunks of its slice in turn, each with its
  * own running maximum, sum and output tile, and meet at a segment's end; a
  * segment that a slice cuts is joined through the workspace by the CTA that
@@ -242,26 +243,58 @@ struct pk_cursor {
     }
 };
 
-/* a warp finds the sequence that holds the line position `at`: upto[t] are
- * the chunks of one segment each up to the rows of thread t (`run` rows a
+/* chunks of sequence r in one segment, in units of `per` */
+template <int CK>
+__device__ __forceinline__ uint32_t pk_units(const pk_attend_job &J, const int2 *cached, uint32_t r, uint32_t per) {
+    const uint32_t n = (uint32_t)pk_row_of<CK>(J, J.A.n_rows <= PK_CACHED ? cached[r] : pk_len_of(J, r, false)).n;
+    return per == 1 ? n : (n + per - 1) / per;
+}
+
+/* inclusive prefix over the CTA's threads -> upto[]; returns their sum */
+__device__ __forceinline__ uint32_t pk_prefix(uint32_t mine, uint32_t *upto) {
+    const uint32_t lane = threadIdx.x & 31u, w = threadIdx.x >> 5;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t y = __shfl_up_sync(~0u, mine, o);
+        if (lane >= o) mine += y;
+    }
+    if (lane == 31) upto[PK_WARPS * 32 + w] = mine;
+    __syncthreads();
+    uint32_t all = 0;
+#pragma unroll
+    for (uint32_t k = 0; k < PK_WARPS; k++) {
+        const uint32_t x = upto[PK_WARPS * 32 + k];
+        if (k < w) mine += x;
+        all += x;
+    }
+    upto[threadIdx.x] = mine;
+    __syncthreads();
+    return all;
+}
+
+/* a warp finds the sequence that holds unit `at` of the line: upto[t] are the
+ * units of one segment each up to the rows of thread t (`run` rows a
  * thread); before = those of all earlier rows */
 template <int CK>
-__device__ __forceinline__ uint32_t pk_locate(const pk_attend_job &J, const int2 *cached, const unsigned long long *upto,
-                                              uint32_t run, unsigned long long at, unsigned long long *before) {
+__device__ __forceinline__ uint32_t pk_locate(const pk_attend_job &J, const int2 *cached, const uint32_t *upto,
+                                              uint32_t run, uint32_t per, uint32_t at, uint32_t *before) {
     const uint32_t lane = threadIdx.x & 31u;
     uint32_t t = 0;
 #pragma unroll
     for (uint32_t k = 0; k < PK_WARPS; k++) t += __popc(__ballot_sync(~0u, upto[k * 32 + lane] * J.segs <= at));
-    unsigned long long sum = t ? upto[t - 1] : 0;
+    uint32_t sum = t ? upto[t - 1] : 0;
+    if (run == 1) {
+        *before = sum;
+        return t;
+    }
     for (uint32_t r0 = t * run;; r0 += 32) {
         const uint32_t r = r0 + lane;
         const bool in = r < (t + 1) * run && r < J.A.n_rows;
-        unsigned long long n = 0, x;
-        if (in) n = (uint32_t)pk_row_of<CK>(J, J.A.n_rows <= PK_CACHED ? cached[r] : pk_len_of(J, r, false)).n;
-        x = n;
+        const uint32_t n = in ? pk_units<CK>(J, cached, r, per) : 0;
+        uint32_t x = n;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const unsigned long long y = __shfl_up_sync(~0u, x, o);
+            const uint32_t y = __shfl_up_sync(~0u, x, o);
             if (lane >= o) x += y;
         }
         const uint32_t hit = __ballot_sync(~0u, in && (sum + x) * J.segs > at);
@@ -272,10 +305,6 @@ __device__ __forceinline__ uint32_t pk_locate(const pk_attend_job &J, const int2
         }
         sum += __shfl_sync(~0u, x, 31);
     }
-}
-
-__device__ __forceinline__ unsigned long long pk_div(unsigned long long a, uint32_t b) {
-    return a >> 32 ? a / b : (uint32_t)a / b;
 }
 
 /* ------------------------------------------------------------ q, results */
@@ -314,9 +343,9 @@ __device__ __forceinline__ void pk_q_load(const pk_attend_job &J, uint64_t at, u
 }
 
 /* what query row v's output sums are multiplied with, given its maximum
- * (log2 units) and sum; writes lse where `tell` */
+ * (log2 units) and sum; writes its lse */
 __device__ __forceinline__ float pk_finish(const pk_attend_job &J, uint32_t b, int32_t len, uint32_t hk, uint32_t v,
-                                           float top, float sum, bool tell) {
+                                           float top, float sum, bool tell = true) {
     const uint32_t i = v / J.group, h = hk * J.group + v % J.group;
     int32_t lo, hi;
     pk_span(J, len, i, lo, hi);
@@ -454,14 +483,19 @@ __device__ void pk_join(const pk_attend_job &J, const pk_joint &S, uint32_t firs
             }
         __syncthreads();
     }
+    if (final) {
+        const uint32_t v = S.v0 + threadIdx.x;
+        if (threadIdx.x < HEADS && v < J.rows)
+            ml[threadIdx.x][0] = pk_finish(J, S.b, S.len, S.hk, v, ml[threadIdx.x][0], ml[threadIdx.x][1]);
+        __syncthreads();
+    }
 #pragma unroll
     for (int n = 0; n < NX; n++) {
         const uint32_t x = n * THREADS + threadIdx.x, head = x / (DP / 4), col = x % (DP / 4) * 4, v = S.v0 + head;
         if (!final) {
             __stcg((float4 *)(J.parts + S.slot(first) * (uint64_t)FLOATS + 2 * HEADS + 4 * x), acc[n]);
         } else if (v < J.rows && col < J.D.head_dim) {
-            const float by = pk_finish(J, S.b, S.len, S.hk, v, ml[head][0], ml[head][1], col == 0);
-            const float y[4] = {acc[n].x * by, acc[n].y * by, acc[n].z * by, acc[n].w * by};
+            const float by = ml[head][0], y[4] = {acc[n].x * by, acc[n].y * by, acc[n].z * by, acc[n].w * by};
             pk_put<4>(J, S.b, S.hk, v, col, y);
         }
     }
@@ -501,11 +535,11 @@ __global__ void __launch_bounds__(PK_WARPS * 32, pk_shape<CT, DP, R, MT, QP>::OC
     extern __shared__ __align__(128) uint8_t smem[];
     uint8_t *ring = smem + (threadIdx.x >> 5) * S::RING;
     float *join = (float *)(smem + PK_WARPS * S::RING);
-    unsigned long long *upto = (unsigned long long *)join; /* in the beginning */
+    uint32_t *upto = (uint32_t *)join;                    /* in the beginning */
     /* QSM: [MT][KS][QW / 2][32][2], in the same bytes: q is done with when a segment's warps meet */
     uint32_t *qsm = (uint32_t *)join;
     static_assert(!QSM || MT * KS * QW * 128 <= S::JOIN, "q's parts fit beside the ring");
-    static_assert(PK_WARPS * 32 * 8 <= S::JOIN, "the line's sums fit");
+    static_assert((PK_WARPS * 32 + PK_WARPS) * 4 <= S::JOIN, "the line's sums fit");
     __shared__ float wml[PK_WARPS][HEADS][2];             /* each warp's maximum and sum */
     __shared__ float fml[HEADS][2];
     __shared__ uint32_t vmask[PK_WARPS][S::STAGES];       /* keys of a stage that are there */
@@ -518,59 +552,63 @@ __global__ void __launch_bounds__(PK_WARPS * 32, pk_shape<CT, DP, R, MT, QP>::OC
     /* ---- the line's length */
     const uint32_t B = J.A.n_rows;
     const uint32_t run = (B + PK_WARPS * 32 - 1) / (PK_WARPS * 32);
-    unsigned long long mine = 0;
+    uint32_t mine = 0;
     for (uint32_t r = tid * run; r < (tid + 1) * run && r < B; r++) {
         const int2 lr = pk_len_of(J, r, blockIdx.x == 0);
         if (B <= PK_CACHED) cached[r] = lr;
         mine += (uint32_t)pk_row_of<CK>(J, lr).n;
     }
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const unsigned long long y = __shfl_up_sync(~0u, mine, o);
-        if (lane >= o) mine += y;
-    }
-    upto[tid] = mine;
     /* columns from head_dim to DP stay zero: copies never write them */
     const uint32_t units = J.D.head_dim * S::ELT / 16;
     if (units < S::UNITS)
         for (uint32_t o = tid * 16; o < PK_WARPS * S::RING; o += PK_WARPS * 32 * 16)
             *(uint4 *)(smem + o) = make_uint4(0, 0, 0, 0);
-    __syncthreads();
-    unsigned long long before = 0, all = 0;
-#pragma unroll
-    for (uint32_t k = 0; k < PK_WARPS; k++) {
-        const unsigned long long x = upto[k * 32 + 31];
-        if (k < w) before += x;
-        all += x;
-    }
-    __syncthreads();
-    upto[tid] = mine + before;
-    __syncthreads();
+    const uint32_t all = pk_prefix(mine, upto);
 
     /* ---- the worker's slice of it */
-    const unsigned long long total = all * J.segs;
-    const bool solo = !QSM && all <= 16ull * B && (unsigned long long)B * J.segs > gridDim.x;
+    const uint32_t total = all * J.segs, segs = B * J.segs;
+    const bool brief = all <= 16u * B;                    /* 16 chunks a segment or fewer, on average */
+    const bool solo = !QSM && brief && segs > gridDim.x;
     const uint32_t workers = solo ? gridDim.x * PK_WARPS : gridDim.x, me = solo ? blockIdx.x * PK_WARPS + w : blockIdx.x;
-    unsigned long long per = pk_div(total + workers - 1, workers);
-    if (!solo) {
-        /* a segment of up to 16 chunks is not cut to fill idle SMs: joining it costs more than reading it */
-        const unsigned long long least = all <= 16ull * B ? pk_div(all + B - 1, B) : J.least;
-        per = per < least ? least : (per + PK_WARPS - 1) & ~(unsigned long long)(PK_WARPS - 1);
-    }
-    unsigned long long lo = per * me, hi = lo + per;
-    if (hi > total) hi = total;
+    uint32_t per = (total + workers - 1) / workers;
+    /* Few segments: each is cut evenly among CTAs of its own, so that no CTA takes parts of two.  That makes
+     * slices longer by segs / (CTAs - segs); a second segment in a slice costs its CTA about 27 chunks' time
+     * (q, the warps' meeting, the join: 5 us). */
+    const bool own = !solo && segs < workers && (uint64_t)per * segs < 27ull * (workers - segs);
+    /* a segment of up to 16 chunks is not cut to fill idle SMs: joining it costs more than reading it */
+    const uint32_t least = !brief ? J.least : B == 1 ? all : (all + B - 1) / B;
+    if (own) per = (total + workers - segs - 1) / (workers - segs);
+    if (!solo) per = per < least ? least : (per + PK_WARPS - 1) & ~(PK_WARPS - 1);
+    uint32_t lo, hi, in, at, piece = 0, pieces = 1;         /* slice [lo, hi); piece of `pieces` of an own segment */
     pk_cursor<CK, HEADS> cons;
-    cons.b = cons.hk = cons.tile = 0;
-    cons.pos = 0;
-    if (lo < total) {
-        unsigned long long at;
-        cons.b = pk_locate<CK>(J, cached, upto, run, lo, &at);
+    if (own) {
+        __syncthreads();
+        mine = 0;
+        for (uint32_t r = tid * run; r < (tid + 1) * run && r < B; r++) mine += pk_units<CK>(J, cached, r, per);
+        if (me >= pk_prefix(mine, upto) * J.segs) return; /* more CTAs than pieces */
+        cons.b = pk_locate<CK>(J, cached, upto, run, per, me, &at);
         cons.row = pk_row_of<CK>(J, B <= PK_CACHED ? cached[cons.b] : pk_len_of(J, cons.b, false));
-        const unsigned long long in = lo - at * J.segs;
-        const uint32_t seg = (uint32_t)pk_div(in, cons.row.n);
-        cons.pos = (int32_t)(in - (unsigned long long)seg * cons.row.n);
-        cons.hk = seg / J.tiles;
-        cons.tile = seg - cons.hk * J.tiles;
+        pieces = ((uint32_t)cons.row.n + per - 1) / per;
+        in = (me - at * J.segs) / pieces;
+        piece = me - at * J.segs - in * pieces;
+        const uint32_t each = (uint32_t)cons.row.n / pieces, more = (uint32_t)cons.row.n - each * pieces;
+        lo = each * piece + (piece < more ? piece : more);
+        hi = lo + each + (piece < more);
+        cons.pos = (int32_t)lo;
+    } else {
+        lo = per * me;
+        if (per && lo / per != me) lo = total;            /* past 2^32: past the end */
+        hi = total - lo < per || lo >= total ? total : lo + per;
+        if (lo < total) {
+            cons.b = pk_locate<CK>(J, cached, upto, run, 1, lo, &at);
+            cons.row = pk_row_of<CK>(J, B <= PK_CACHED ? cached[cons.b] : pk_len_of(J, cons.b, false));
+            in = (lo - at * J.segs) / (uint32_t)cons.row.n;
+            cons.pos = (int32_t)(lo - at * J.segs - in * (uint32_t)cons.row.n);
+        }
+    }
+    if (lo < hi) {
+        cons.hk = J.tiles == 1 ? in : in / J.tiles;
+        cons.tile = in - cons.hk * J.tiles;
         cons.enter(J);
         if (solo) {
             /* whole segments: those that begin in [lo, hi) */
@@ -580,10 +618,9 @@ __global__ void __launch_bounds__(PK_WARPS * 32, pk_shape<CT, DP, R, MT, QP>::OC
                 cons.step(J, cached, rest);
             }
             if (hi < total) {
-                const uint32_t b2 = pk_locate<CK>(J, cached, upto, run, hi, &at);
-                const uint32_t n2 = pk_row_of<CK>(J, B <= PK_CACHED ? cached[b2] : pk_len_of(J, b2, false)).n;
-                const unsigned long long off = hi - at * J.segs;
-                hi = at * J.segs + pk_div(off + n2 - 1, n2) * n2;
+                const uint32_t b2 = pk_locate<CK>(J, cached, upto, run, 1, hi, &at);
+                const uint32_t n2 = pk_units<CK>(J, cached, b2, 1);
+                hi = at * J.segs + (hi - at * J.segs + n2 - 1) / n2 * n2;
             }
         }
     }
@@ -592,7 +629,7 @@ __global__ void __launch_bounds__(PK_WARPS * 32, pk_shape<CT, DP, R, MT, QP>::OC
 
     /* ---- cursors: cons walks the worker's segments, prod runs ahead by the warp's chunks */
     const uint32_t stride = solo ? 1 : PK_WARPS, lead = solo ? 0 : w;
-    const uint32_t slice = (uint32_t)(hi - lo);           /* chunks in the slice */
+    const uint32_t slice = hi - lo;                       /* chunks in the slice */
     pk_cursor<CK, HEADS> prod = cons;
     uint32_t ahead = lead;                                /* slice offset of prod */
     if (lead) prod.step(J, cached, (int32_t)lead);
@@ -1070,7 +1107,11 @@ __global__ void __launch_bounds__(PK_WARPS * 32, pk_shape<CT, DP, R, MT, QP>::OC
 #pragma unroll
                 for (uint32_t k = 0; k < PK_WARPS; k++) sum += wml[k][y * 8 + g][1] * pk_exp2(wml[k][y * 8 + g][0] - zero);
                 const float keep = drop * pk_exp2(m[y] - zero);
-                if (w == 0 && c == 0) *(float2 *)fml[y * 8 + g] = make_float2(top, sum);
+                if (w == 0 && c == 0) {
+                    const uint32_t v = v0 + y * 8 + g;
+                    if (!cut && v < J.rows) top = pk_finish(J, cons.b, cons.row.len, cons.hk, v, top, sum);
+                    *(float2 *)fml[y * 8 + g] = make_float2(top, sum); /* uncut: [0] is the output's factor */
+                }
                 auto place = [&](uint32_t owner, uint32_t source, int tq) {
                     return join + ((owner * 3 + source) * 8 + g) * S::QROW + tq * 8 + RUN * c;
                 };
@@ -1117,8 +1158,7 @@ __global__ void __launch_bounds__(PK_WARPS * 32, pk_shape<CT, DP, R, MT, QP>::OC
                             __stcg((float4 *)(part + 2 * HEADS + head * DP + col), x);
                             if (col == 0) __stcg((float2 *)(part + 2 * head), make_float2(fml[head][0], fml[head][1]));
                         } else if (v0 + head < J.rows && col < J.D.head_dim) {
-                            const float by = pk_finish(J, cons.b, cons.row.len, cons.hk, v0 + head, fml[head][0],
-                                                       fml[head][1], col == 0);
+                            const float by = fml[head][0];
                             const float z[4] = {x.x * by, x.y * by, x.z * by, x.w * by};
                             pk_put<4>(J, cons.b, cons.hk, v0 + head, col, z);
                         }
@@ -1127,15 +1167,21 @@ __global__ void __launch_bounds__(PK_WARPS * 32, pk_shape<CT, DP, R, MT, QP>::OC
             }
             if (cut) {
                 /* a join that falls to this CTA waits for its slice's end: other joins may wait for the rest of it */
-                const unsigned long long seg0 = lo + done - (uint32_t)from;
                 pk_joint S2;
                 S2.b = cons.b;
                 S2.hk = cons.hk;
                 S2.v0 = v0;
                 S2.len = cons.row.len;
-                S2.w0 = (uint32_t)(seg0 / per);
-                S2.w1 = (uint32_t)((seg0 + (uint32_t)cons.row.n - 1) / per);
-                S2.inside = seg0 > per * S2.w0;
+                if (own) {
+                    S2.w0 = me - piece;
+                    S2.w1 = S2.w0 + pieces - 1;
+                    S2.inside = false;
+                } else {
+                    const uint32_t seg0 = lo + done - (uint32_t)from;
+                    S2.w0 = seg0 / per;
+                    S2.w1 = (seg0 + (uint32_t)cons.row.n - 1) / per;
+                    S2.inside = seg0 > per * S2.w0;
+                }
                 if (pk_joint_arrive(J, S2, &last)) {
                     if (owes) {
                         also = true;

@@ -37,24 +37,39 @@ def _need(ok: bool, what: str) -> None:
         raise ValueError(what)
 
 
-def _stream(stream):
-    return torch.cuda.current_stream().cuda_stream if stream is None else stream.cuda_stream
+def _stream(stream, dev):
+    """the cudaStream_t to launch on: dev is the buffers' device index"""
+    if stream is None:
+        return torch._C._cuda_getCurrentRawStream(dev)  # current_stream() builds an object: 3 us a call
+    return stream.cuda_stream
 
 
 def _i32(t, n, dev, what):
-    if t.dtype != torch.int32 or t.device != dev or t.numel() != n or not t.is_contiguous():
+    if t.dtype is not torch.int32 or t.device != dev or t.numel() != n or not t.is_contiguous():
         raise ValueError(f"{what}: {n} contiguous int32 values on {dev}")
     return t.data_ptr()
 
 
 def _heads(t, n_tok, n_head, d, dtype, dev, what):
     """(pointer, token stride) of [n_tok][n_head][d] values, heads d apart"""
-    if t.shape != (n_tok, n_head, d) or t.dtype != dtype or t.device != dev:
+    if t.shape != (n_tok, n_head, d) or t.dtype is not dtype or t.device != dev:
         raise ValueError(f"{what}: {n_tok} x {n_head} x {d} values of {dtype} on {dev}")
     s0, s1, s2 = t.stride()
     if (s2 != 1 and d > 1) or (s1 != d and n_head > 1):
         raise ValueError(f"{what}: a token's heads are {d} values apart and contiguous")
     return t.data_ptr(), s0
+
+
+def _tokens(t, n, n_q, n_head, d):
+    """the one stride between the n * n_q tokens of attend's q or out"""
+    st = t.stride()
+    if st[-1] != 1 or (n_head > 1 and st[-2] != d):
+        raise ValueError(f"attend: a token's heads are {d} values apart and contiguous")
+    if n_q == 1:
+        return st[0] if n > 1 else n_head * d
+    if n > 1 and st[0] != n_q * st[1]:
+        raise ValueError("attend: one stride between all tokens")
+    return st[1]
 
 
 # ------------------------------------------------------------------ positions
@@ -129,7 +144,7 @@ class PagedKv:
             _need(s is None or (s.dtype == torch.float32 and s.device == k.device and s.is_contiguous()
                                 and s.numel() == k.shape[1]), "PagedKv: scales are f32 [n_kv] beside the cache")
         self.k, self.v, self.table, self.k_scale, self.v_scale = k, v, table, k_scale, v_scale
-        self.device, self.n_kv, self.head_dim = k.device, k.shape[1], k.shape[3]
+        self.device, self.n_kv, self.head_dim, self._index = k.device, k.shape[1], k.shape[3], k.device.index
         d = KvDesc()
         d.k, d.v, d.table = k.data_ptr(), v.data_ptr(), table.data_ptr()
         d.k_scale = None if k_scale is None else k_scale.data_ptr()
@@ -172,7 +187,7 @@ class PagedKv:
                 raise ValueError("append: cos_sin is f32 [n_pos][2][rot_dim / 2]")
             a.cos_sin, a.n_pos, a.rot_dim = cos_sin.data_ptr(), cos_sin.shape[0], 2 * cos_sin.shape[2]
         a.n_tok, a.x_type, a.interleaved = n_tok, TYPES[k.dtype], int(interleaved)
-        check(self._lib.pulsar_kv_append(self._pdesc, self._pappend, _stream(stream)), "kv_append")
+        check(self._lib.pulsar_kv_append(self._pdesc, self._pappend, _stream(stream, self._index)), "kv_append")
         return q_out
 
     def attend(self, q, lens, out, scale: float | None = None, window: int = 0, sinks=None, lse=None, seq=None,
@@ -185,49 +200,45 @@ class PagedKv:
         unless given.  ws: a zeroed workspace (workspace()); without one the
         object keeps its own, which serves one stream at a time."""
         a, dev, D = self._args, self.device, self.head_dim
-        if q.dim() == 3:
-            q, out = q.unsqueeze(1), out.unsqueeze(1)
-            done = out.squeeze(1)
+        shape, dtype = q.shape, q.dtype
+        kind = TYPES.get(dtype, 3)
+        if len(shape) == 4:
+            n, n_q, n_head, d = shape
         else:
-            done = out
-        n, n_q, n_head, d = q.shape
+            (n, n_head, d), n_q = shape, 1
         if n == 0 or n_q == 0:
-            return done
-        if q.dtype not in TYPES or q.dtype == torch.float8_e4m3fn or q.dtype != out.dtype or out.shape != q.shape or d != D:
-            raise ValueError("attend: q and out alike, f32, bf16 or f16 [B][n_q][n_head][head_dim]")
-        for t, x in (("q", q), ("out", out)):
-            s0, s1, s2, s3 = x.stride()
-            if x.device != dev or s3 != 1 or (n_head > 1 and s2 != D) or (n > 1 and n_q > 1 and s0 != n_q * s1):
-                raise ValueError(f"attend: {t} has one stride between tokens, heads {D} apart, beside the cache")
+            return out
+        if kind == 3 or dtype is not out.dtype or out.shape != shape or d != D or q.device != dev or out.device != dev:
+            raise ValueError("attend: q and out alike, f32, bf16 or f16 [B][n_q][n_head][head_dim], beside the cache")
         a.q, a.out = q.data_ptr(), out.data_ptr()
-        a.q_stride = q.stride(1) if n_q > 1 else q.stride(0) if n > 1 else n_head * D
-        a.out_stride = out.stride(1) if n_q > 1 else out.stride(0) if n > 1 else n_head * D
+        a.q_stride, a.out_stride = _tokens(q, n, n_q, n_head, D), _tokens(out, n, n_q, n_head, D)
         a.lens = _i32(lens, n, dev, "attend: lens")
         a.seq = None if seq is None else _i32(seq, n, dev, "attend: seq")
         a.sinks = a.lse = None
         if sinks is not None:
-            if sinks.dtype != torch.float32 or sinks.numel() != n_head or sinks.device != dev or not sinks.is_contiguous():
+            if sinks.dtype is not torch.float32 or sinks.numel() != n_head or sinks.device != dev or not sinks.is_contiguous():
                 raise ValueError("attend: sinks is f32 [n_head]")
             a.sinks = sinks.data_ptr()
         if lse is not None:
-            if lse.dtype != torch.float32 or lse.numel() != n * n_q * n_head or lse.device != dev or not lse.is_contiguous():
+            if lse.dtype is not torch.float32 or lse.numel() != n * n_q * n_head or lse.device != dev or not lse.is_contiguous():
                 raise ValueError("attend: lse is f32 [B][n_q][n_head]")
             a.lse = lse.data_ptr()
-        if window < 0 or window > 0x7fffffff:
+        if not 0 <= window <= 0x7fffffff:
             raise ValueError("attend: window is 0 (none) or a number of keys")
         a.scale = D ** -0.5 if scale is None else scale
-        a.n_rows, a.n_q, a.n_head, a.window, a.q_type = n, n_q, n_head, window, TYPES[q.dtype]
+        a.n_rows, a.n_q, a.n_head, a.window, a.q_type = n, n_q, n_head, window, kind
         if ws is None:
-            size = (n, n_q, n_head, a.q_type, window)
+            size = (n, n_q, n_head, kind, window)
             if self._sized != size:
                 need = self.workspace_bytes()
                 if self._ws is None or self._ws.numel() < need:
                     self._ws = torch.zeros(need, dtype=torch.uint8, device=dev)
-                self._sized = size
-            ws = self._ws
-        check(self._lib.pulsar_kv_attend(self._pdesc, self._pargs, ws.data_ptr(), ws.numel(), _stream(stream)),
-              "kv_attend")
-        return done
+                self._sized, self._where = size, (self._ws.data_ptr(), self._ws.numel())
+            where = self._where
+        else:
+            where = ws.data_ptr(), ws.numel()
+        check(self._lib.pulsar_kv_attend(self._pdesc, self._pargs, *where, _stream(stream, self._index)), "kv_attend")
+        return out
 
     def workspace_bytes(self) -> int:
         """bytes that the last attend() call's arguments need"""
@@ -250,7 +261,7 @@ class KvPool:
             _i32(t, n, data.device, "KvPool: " + what)
         _need(table.dim() == 2, "KvPool: table is [n_rows][max_pages]")
         self.data, self.table, self.lens, self.refs = data, table, lens, refs
-        self.device, self.n_rows, self.page_size = data.device, n_rows, data.shape[4]
+        self.device, self.n_rows, self.page_size, self._index = data.device, n_rows, data.shape[4], data.device.index
         p = KvPoolDesc()
         p.table, p.len, p.refs, p.data = table.data_ptr(), lens.data_ptr(), refs.data_ptr(), data.data_ptr()
         p.slab_stride = data.stride(1) * data.element_size()
@@ -263,6 +274,7 @@ class KvPool:
         need = int(self._lib.pulsar_kv_pool_workspace(self._p, n_rows))
         _need(need > 0, "KvPool: shape refused")
         self._ws = torch.empty(need, dtype=torch.uint8, device=self.device)
+        self._where = self._ws.data_ptr(), need
         #: what the last grow, fork and compact did (pulsar_kv.h's status words)
         self.status = torch.zeros((3, 4), dtype=torch.int32, device=self.device)
         self._status = [self.status[i].data_ptr() for i in range(3)]
@@ -284,7 +296,7 @@ class KvPool:
             return
         r = None if rows is None else _i32(rows, n, self.device, "grow: rows")
         check(self._lib.pulsar_kv_grow(self._p, r, _i32(n_new, n, self.device, "grow: n_new"), n, self._status[0],
-                                       self._ws.data_ptr(), self._ws.numel(), _stream(stream)), "kv_grow")
+                                       *self._where, _stream(stream, self._index)), "kv_grow")
 
     def fork(self, src: torch.Tensor, dst: torch.Tensor, stream=None) -> None:
         """row dst[i] becomes what row src[i] was (src -1: empty), all i at once"""
@@ -292,8 +304,8 @@ class KvPool:
         if n == 0:
             return
         check(self._lib.pulsar_kv_fork(self._p, _i32(dst, n, self.device, "fork: dst"),
-                                       _i32(src, n, self.device, "fork: src"), n, self._status[1], self._ws.data_ptr(),
-                                       self._ws.numel(), _stream(stream)), "kv_fork")
+                                       _i32(src, n, self.device, "fork: src"), n, self._status[1], *self._where,
+                                       _stream(stream, self._index)), "kv_fork")
 
     def free(self, rows: torch.Tensor, stream=None) -> None:
         """rows become empty"""
@@ -301,8 +313,8 @@ class KvPool:
 
     def compact(self, stream=None) -> None:
         """live pages move to the low ids"""
-        check(self._lib.pulsar_kv_compact(self._p, self._status[2], self._ws.data_ptr(), self._ws.numel(),
-                                          _stream(stream)), "kv_compact")
+        check(self._lib.pulsar_kv_compact(self._p, self._status[2], *self._where, _stream(stream, self._index)),
+              "kv_compact")
 
     def check(self) -> None:
         """raise if the last grow, fork or compact was refused on the device (synchronous)"""
