@@ -124,7 +124,7 @@ typedef struct pulsar_kv_pool {
     uint32_t n_rows, max_pages, n_pages, page_size, n_slab;
 } pulsar_kv_pool;
 
-/* status words (int32[4], device) of the three calls: [0] what happened,
+/* status words (int32[4], device, 16-byte aligned like ws) of the three calls: [0] what happened,
  * [1] pages taken or moved, [2] pages that were free before (grow, fork) or
  * are live (compact).  Unless [0] is PULSAR_KV_OK nothing was changed. */
 #define PULSAR_KV_OK 0

@@ -71,25 +71,33 @@ __global__ void __launch_bounds__(256)
     const float *scale = is_v ? D.v_scale : D.k_scale;
     const float sc = !is_q && scale ? scale[h] : 1.0f;
 
-    for (uint32_t t = blockIdx.y * blockDim.y + threadIdx.y; t < A.n_tok; t += gridDim.y * blockDim.y) {
-        const int32_t pos = A.pos[t], seq = A.seq[t];
-        if (pos < 0 || seq < 0) continue;
-        const uint64_t from = t * in_stride + (uint64_t)h * D.head_dim;
+    /* one latency a token: x's loads wait for nothing, and the token's
+     * position and row were loaded a token ahead */
+    const uint32_t step = gridDim.y * blockDim.y;
+    uint32_t t = blockIdx.y * blockDim.y + threadIdx.y;
+    int32_t pos = -1, seq = -1;
+    if (t < A.n_tok) {
+        pos = __ldg(A.pos + t);
+        seq = __ldg(A.seq + t);
+    }
+    for (int32_t pos2 = -1, seq2 = -1; t < A.n_tok; t += step, pos = pos2, seq = seq2) {
         float x[2 * V];
+        const uint64_t from = t * in_stride + (uint64_t)h * D.head_dim;
         pk_load<X, V>(in, from + o0, x);
+        if (turn) pk_load<X, V>(in, from + o1, x + V);
+        if (A.n_tok - t > step) {
+            pos2 = __ldg(A.pos + t + step);
+            seq2 = __ldg(A.seq + t + step);
+        }
+        if (pos < 0 || seq < 0) continue;
         if (turn) {
-            pk_load<X, V>(in, from + o1, x + V);
             if ((uint32_t)pos >= A.n_pos) {
                 atomicOr(err, PULSAR_KV_ERR_SPAN);
                 continue;
             }
             const float *cs = A.cos_sin + (uint64_t)pos * A.rot_dim + (uint64_t)j * V;
-            float c[V], s[V];
-#pragma unroll
-            for (int i = 0; i < V; i++) {
-                c[i] = __ldg(cs + i);
-                s[i] = __ldg(cs + half + i);
-            }
+            const pk_vec<float, V> c4 = *(const pk_vec<float, V> *)cs, s4 = *(const pk_vec<float, V> *)(cs + half);
+            const float *c = c4.v, *s = s4.v;
             if (A.interleaved) {
 #pragma unroll
                 for (int i = 0; i < V; i++) {
@@ -162,7 +170,9 @@ static int pk_append_by_width(const pulsar_kv_desc *d, const pulsar_kv_append_ar
     const uint32_t xe = pk_type_bytes(a->x_type), qe = pk_type_bytes(a->q_out_type);
     for (uint32_t v = 8; v > 1; v /= 2) {
         const uint32_t xb = xe * v > 16 ? 16 : xe * v, qb = qe * v > 16 ? 16 : qe * v;
-        uint64_t odd = ((uintptr_t)a->k | (uintptr_t)a->v | a->k_stride * xe | a->v_stride * xe) % xb;
+        const uint32_t cb = v < 4 ? 4 * v : 16; /* the angles' loads */
+        uint64_t odd = (uintptr_t)a->cos_sin % cb;
+        odd |= ((uintptr_t)a->k | (uintptr_t)a->v | a->k_stride * xe | a->v_stride * xe) % xb;
         if (a->n_head)
             odd |= ((uintptr_t)a->q | a->q_stride * xe) % xb | ((uintptr_t)a->q_out | a->q_out_stride * qe) % qb;
         if (odd || a->rot_dim / 2 % v) continue;

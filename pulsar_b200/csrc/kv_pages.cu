@@ -31,6 +31,28 @@ extern "C" uint32_t pulsar_kv_error(void) {
     return v;
 }
 
+/* An apply kernel is launched while its plan still runs: its CTAs take their
+ * places and wait there (in the hardware, for the plan's end and its writes),
+ * which saves the launch's latency. */
+__device__ __forceinline__ void pk_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void pk_await() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+template <class... A>
+static cudaError_t pk_launch_after(void (*kernel)(A...), uint32_t grid, uint32_t block, uint32_t smem, cudaStream_t st,
+                                   A... args) {
+    cudaLaunchAttribute early;
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t c = {};
+    c.gridDim = grid;
+    c.blockDim = block;
+    c.dynamicSmemBytes = smem;
+    c.stream = st;
+    c.attrs = &early;
+    c.numAttrs = 1;
+    return cudaLaunchKernelEx(&c, kernel, args...);
+}
+
 #define PK_PLAN 1024u /* threads of a plan CTA */
 #define PK_FORK_COLS 8u
 
@@ -69,35 +91,39 @@ __device__ __forceinline__ uint32_t pk_block_scan(uint32_t v, pk_scan &s, uint32
     return s.warp[w] + x - v;
 }
 
-/* Each warp walks its own run of [lo, hi) in page order, 32 pages a step;
+/* Each warp walks its own run of [lo, hi) in page order, 32 pages a step; the
  * pages for which refs[p] > 0 equals `live` get the ranks 0, 1, ... in page
- * order, and emit(p, rank) is called for ranks below `want`.  Returns how
- * many there are (counted over all of [lo, hi)).  The counts are read twice;
- * an SM takes them from the caches at some 64 bytes a cycle. */
-template <class F>
-__device__ uint32_t pk_choose(const int32_t *refs, uint32_t lo, uint32_t hi, bool live, uint32_t want, pk_scan &s,
-                              F emit) {
+ * order.  want(total) is asked once their number is known (by every thread
+ * alike), and emit(p, rank) is called for the ranks below it.  Returns the
+ * total.  The counts are read twice; an SM takes them from the caches at some
+ * 64 bytes a cycle. */
+template <class W, class F>
+__device__ uint32_t pk_choose(const int32_t *refs, uint32_t lo, uint32_t hi, bool live, pk_scan &s, W want, F emit) {
     const uint32_t lane = threadIdx.x & 31u, w = threadIdx.x >> 5, nw = blockDim.x >> 5;
     const uint32_t n = hi - lo;
     const uint32_t run = ((n + nw - 1) / nw + 31u) & ~31u;
     const uint64_t b64 = (uint64_t)lo + (uint64_t)w * run;
     const uint32_t b = b64 < hi ? (uint32_t)b64 : hi, e = hi - b < run ? hi : b + run;
     uint32_t count = 0;
-#pragma unroll 4
+#pragma unroll 8
     for (uint32_t p = b + lane; p < e; p += 32) count += (refs[p] > 0) == live;
     uint32_t total;
     uint32_t at = pk_block_scan(count, s, &total);
     at = __shfl_sync(~0u, at, 0); /* the warp's first rank */
-    for (uint32_t p0 = b; p0 < e && at < want; p0 += 32) {
+    const uint32_t most = want(total);
+    for (uint32_t p0 = b; p0 < e && at < most; p0 += 32) {
         const uint32_t p = p0 + lane;
         const bool hit = p < e && (refs[p] > 0) == live;
         const uint32_t m = __ballot_sync(~0u, hit);
         const uint32_t rank = at + __popc(m & ((1u << lane) - 1u));
-        if (hit && rank < want) emit(p, rank);
+        if (hit && rank < most) emit(p, rank);
         at += __popc(m);
     }
     return total;
 }
+
+/* words of row marks that a plan keeps in shared memory; longer tables use the workspace */
+#define PK_MARKS 8192u
 
 __device__ __forceinline__ uint32_t pk_ceil(uint32_t a, uint32_t b) { return (a + b - 1u) / b; }
 
@@ -108,9 +134,9 @@ __device__ __forceinline__ uint32_t pk_ceil(uint32_t a, uint32_t b) { return (a 
 __global__ void __launch_bounds__(PK_PLAN) pk_grow_kernel(pulsar_kv_pool P, const int32_t *rows, const int32_t *n_new,
                                                           uint32_t n, int32_t *status, uint32_t *ws) {
     __shared__ pk_scan scan;
-    __shared__ uint32_t bad;
+    __shared__ uint32_t bad, marks[PK_MARKS];
     __shared__ unsigned long long wanted; /* need_all could wrap: nothing is taken from it unless this fits */
-    uint32_t *mark = ws, *off = ws + P.n_rows;
+    uint32_t *mark = P.n_rows <= PK_MARKS ? marks : ws, *off = ws + P.n_rows;
     const uint32_t tid = threadIdx.x;
     const uint32_t cap = P.max_pages * P.page_size;
     if (tid == 0) {
@@ -143,23 +169,17 @@ __global__ void __launch_bounds__(PK_PLAN) pk_grow_kernel(pulsar_kv_pool P, cons
     }
     __syncthreads();
     if (bad) {
-        if (tid == 0) {
-            status[0] = bad & 1u ? PULSAR_KV_INVALID : PULSAR_KV_WIDE;
-            status[1] = status[2] = status[3] = 0;
-        }
+        if (tid == 0) *(int4 *)status = make_int4(bad & 1u ? PULSAR_KV_INVALID : PULSAR_KV_WIDE, 0, 0, 0);
         return;
     }
-    const uint32_t free_pages = pk_choose(P.refs, 0, P.n_pages, false, 0, scan, [](uint32_t, uint32_t) {});
-    const bool ok = wanted <= free_pages;
-    if (tid == 0) {
-        status[0] = ok ? PULSAR_KV_OK : PULSAR_KV_SHORT;
-        status[1] = ok ? (int32_t)need_all : 0;
-        status[2] = (int32_t)free_pages;
-        status[3] = 0;
-    }
-    if (!ok) return;
-    if (need_all)
-        pk_choose(P.refs, 0, P.n_pages, false, need_all, scan, [&](uint32_t page, uint32_t rank) {
+    bool ok = false;
+    const uint32_t free_pages = pk_choose(
+        P.refs, 0, P.n_pages, false, scan,
+        [&](uint32_t total) {
+            ok = wanted <= total;
+            return ok ? need_all : 0u;
+        },
+        [&](uint32_t page, uint32_t rank) {
             uint32_t a = 0, b = n; /* the last i with off[i] <= rank */
             while (b - a > 1) {
                 const uint32_t m = (a + b) >> 1;
@@ -170,6 +190,9 @@ __global__ void __launch_bounds__(PK_PLAN) pk_grow_kernel(pulsar_kv_pool P, cons
             P.table[r * P.table_stride + pk_ceil(P.len[r], P.page_size) + (rank - off[a])] = (int32_t)page;
             P.refs[page] = 1;
         });
+    if (tid == 0)
+        *(int4 *)status = make_int4(ok ? PULSAR_KV_OK : PULSAR_KV_SHORT, ok ? (int32_t)need_all : 0, (int32_t)free_pages, 0);
+    if (!ok) return;
     __syncthreads(); /* the lengths above are read before they change */
     for (uint32_t i = tid; i < n; i += PK_PLAN) P.len[rows ? rows[i] : (int32_t)i] += n_new[i];
 }
@@ -207,10 +230,15 @@ __global__ void __launch_bounds__(PK_PLAN) pk_fork_plan_kernel(pulsar_kv_pool P,
                                                                const int32_t *src, uint32_t n, int32_t *status,
                                                                void *wsp) {
     __shared__ pk_scan scan;
-    __shared__ uint32_t bad, wide;
-    const pk_fork_ws w = pk_fork_layout(wsp, P.n_rows, n);
+    __shared__ uint32_t bad, wide, marks[PK_MARKS];
+    pk_fork_ws w = pk_fork_layout(wsp, P.n_rows, n);
     const uint32_t tid = threadIdx.x;
     const uint32_t cap = P.max_pages * P.page_size;
+    pk_dependents();
+    if (2 * P.n_rows <= PK_MARKS) {
+        w.mark = marks;
+        w.first = marks + P.n_rows;
+    }
     if (tid == 0) bad = wide = 0;
     for (uint32_t r = tid; r < P.n_rows; r += PK_PLAN) {
         w.mark[r] = 0;
@@ -238,8 +266,7 @@ __global__ void __launch_bounds__(PK_PLAN) pk_fork_plan_kernel(pulsar_kv_pool P,
     if (bad) {
         if (tid == 0) {
             w.head[0] = 0;
-            status[0] = PULSAR_KV_INVALID;
-            status[1] = status[2] = status[3] = 0;
+            *(int4 *)status = make_int4(PULSAR_KV_INVALID, 0, 0, 0);
         }
         return;
     }
@@ -258,44 +285,54 @@ __global__ void __launch_bounds__(PK_PLAN) pk_fork_plan_kernel(pulsar_kv_pool P,
         uint32_t total;
         const uint32_t at = pk_block_scan(need, scan, &total);
         if (i < n) {
-            w.fresh[i] = need ? 0 : -1;
+            w.fresh[i] = -1;
             if (need) w.rank[copies + at] = i;
         }
         copies += total;
     }
-    const uint32_t free_pages = pk_choose(P.refs, 0, P.n_pages, false, 0, scan, [](uint32_t, uint32_t) {});
-    const bool ok = copies <= free_pages;
+    __syncthreads(); /* rank[] is whole */
+    bool ok = false;
+    const uint32_t free_pages = pk_choose(
+        P.refs, 0, P.n_pages, false, scan,
+        [&](uint32_t total) {
+            ok = copies <= total;
+            return ok ? copies : 0u;
+        },
+        [&](uint32_t page, uint32_t rank) {
+            const uint32_t i = w.rank[rank];
+            w.fresh[i] = (int32_t)page;
+            w.pair[2 * rank] = P.table[src[i] * P.table_stride + w.now[i] / P.page_size];
+            w.pair[2 * rank + 1] = (int32_t)page;
+        });
     if (tid == 0) {
         w.head[0] = ok;
         w.head[1] = copies;
         w.head[2] = wide;
-        status[0] = ok ? PULSAR_KV_OK : PULSAR_KV_SHORT;
-        status[1] = ok ? (int32_t)copies : 0;
-        status[2] = (int32_t)free_pages;
-        status[3] = 0;
+        *(int4 *)status = make_int4(ok ? PULSAR_KV_OK : PULSAR_KV_SHORT, ok ? (int32_t)copies : 0, (int32_t)free_pages, 0);
     }
-    if (!ok || !copies) return;
-    __syncthreads();
-    pk_choose(P.refs, 0, P.n_pages, false, copies, scan, [&](uint32_t page, uint32_t rank) {
-        const uint32_t i = w.rank[rank];
-        w.fresh[i] = (int32_t)page;
-        w.pair[2 * rank] = P.table[src[i] * P.table_stride + w.now[i] / P.page_size];
-        w.pair[2 * rank + 1] = (int32_t)page;
-    });
 }
 
-/* Pages from -> to of every slab.  A warp moves 2 KB at a time (16 bytes a
- * lane, four loads in flight); pages of other sizes or alignment go by bytes. */
+/* Pages from -> to of every slab.  A warp moves 4 KB at a time (16 bytes a
+ * lane, eight loads in flight); pages of other sizes or alignment go by bytes. */
+#define PK_COPY 4096u
 __device__ void pk_copy_pages(const pulsar_kv_pool &P, const int32_t *from, const int32_t *to, uint32_t step,
                               uint32_t n, uint32_t block, uint32_t blocks, uint32_t *err) {
     const uint32_t lane = threadIdx.x & 31u;
     const uint32_t warps = blocks * (blockDim.x >> 5);
-    const uint64_t per = (P.page_bytes + 2047u) >> 11;
+    const uint64_t per = (P.page_bytes + PK_COPY - 1) / PK_COPY;
     const uint64_t all = per * P.n_slab * n;
     const bool wide = (((uintptr_t)P.data | P.slab_stride | P.page_bytes) & 15u) == 0;
     for (uint64_t u = block * (blockDim.x >> 5) + (threadIdx.x >> 5); u < all; u += warps) {
-        const uint64_t part = u % per, ps = u / per;
-        const uint32_t slab = (uint32_t)(ps % P.n_slab), pr = (uint32_t)(ps / P.n_slab);
+        uint64_t part, ps;
+        if (all >> 32) {
+            part = u % per;
+            ps = u / per;
+        } else {
+            part = (uint32_t)u % (uint32_t)per;
+            ps = (uint32_t)u / (uint32_t)per;
+        }
+        const uint32_t slab = (uint32_t)(ps >> 32 ? ps % P.n_slab : (uint32_t)ps % P.n_slab);
+        const uint32_t pr = (uint32_t)(ps >> 32 ? ps / P.n_slab : (uint32_t)ps / P.n_slab);
         const uint32_t a = (uint32_t)from[pr * step], b = (uint32_t)to[pr * step];
         if (a >= P.n_pages || b >= P.n_pages) {
             if (lane == 0) atomicOr(err, PULSAR_KV_ERR_PAGE);
@@ -303,17 +340,17 @@ __device__ void pk_copy_pages(const pulsar_kv_pool &P, const int32_t *from, cons
         }
         const uint8_t *x = (const uint8_t *)P.data + slab * P.slab_stride + a * P.page_bytes;
         uint8_t *y = (uint8_t *)P.data + slab * P.slab_stride + b * P.page_bytes;
-        const uint64_t o0 = part << 11, left = P.page_bytes - o0;
-        const uint32_t m = left < 2048u ? (uint32_t)left : 2048u;
+        const uint64_t o0 = part * PK_COPY, left = P.page_bytes - o0;
+        const uint32_t m = left < PK_COPY ? (uint32_t)left : PK_COPY;
         if (wide) {
-            uint4 v[4];
+            uint4 v[PK_COPY / 512];
 #pragma unroll
-            for (uint32_t k = 0; k < 4; k++) {
+            for (uint32_t k = 0; k < PK_COPY / 512; k++) {
                 const uint32_t o = (k * 32 + lane) * 16;
-                if (o < m) v[k] = __ldg((const uint4 *)(x + o0 + o));
+                if (o < m) v[k] = __ldcs((const uint4 *)(x + o0 + o));
             }
 #pragma unroll
-            for (uint32_t k = 0; k < 4; k++) {
+            for (uint32_t k = 0; k < PK_COPY / 512; k++) {
                 const uint32_t o = (k * 32 + lane) * 16;
                 if (o < m) *(uint4 *)(y + o0 + o) = v[k];
             }
@@ -333,6 +370,7 @@ __global__ void __launch_bounds__(256) pk_fork_apply_kernel(pulsar_kv_pool P, co
                                                             uint32_t *err) {
     extern __shared__ int32_t stage[]; /* [n][PK_FORK_COLS] */
     const pk_fork_ws w = pk_fork_layout((void *)wsp, P.n_rows, n);
+    pk_await();
     if (!w.head[0]) return;
     if (blockIdx.x >= table_blocks) {
         pk_copy_pages(P, w.pair, w.pair + 1, 2, w.head[1], blockIdx.x - table_blocks, gridDim.x - table_blocks, err);
@@ -377,26 +415,27 @@ __global__ void __launch_bounds__(PK_PLAN) pk_compact_plan_kernel(pulsar_kv_pool
     const uint32_t half = P.n_pages / 2 + 1;
     uint32_t *head = ws;
     int32_t *from = (int32_t *)ws + 4, *to = from + half, *map = to + half;
-    const uint32_t live = pk_choose(P.refs, 0, P.n_pages, true, 0, scan, [](uint32_t, uint32_t) {});
-    const uint32_t moves = pk_choose(P.refs, 0, live, false, ~0u, scan,
+    const auto none = [](uint32_t) { return 0u; };
+    const auto every = [](uint32_t total) { return total; };
+    pk_dependents();
+    const uint32_t live = pk_choose(P.refs, 0, P.n_pages, true, scan, none, [](uint32_t, uint32_t) {});
+    const uint32_t moves = pk_choose(P.refs, 0, live, false, scan, every,
                                      [&](uint32_t page, uint32_t rank) { to[rank] = (int32_t)page; });
     __syncthreads();
-    pk_choose(P.refs, live, P.n_pages, true, ~0u, scan, [&](uint32_t page, uint32_t rank) {
+    pk_choose(P.refs, live, P.n_pages, true, scan, every, [&](uint32_t page, uint32_t rank) {
         from[rank] = (int32_t)page;
         map[page] = to[rank];
     });
     if (threadIdx.x == 0) {
         head[0] = moves;
         head[1] = live;
-        status[0] = PULSAR_KV_OK;
-        status[1] = (int32_t)moves;
-        status[2] = (int32_t)live;
-        status[3] = 0;
+        *(int4 *)status = make_int4(PULSAR_KV_OK, (int32_t)moves, (int32_t)live, 0);
     }
 }
 
 __global__ void __launch_bounds__(256) pk_compact_apply_kernel(pulsar_kv_pool P, uint32_t table_blocks,
                                                                const uint32_t *ws, uint32_t *err) {
+    pk_await();
     const uint32_t half = P.n_pages / 2 + 1, moves = ws[0], live = ws[1];
     const int32_t *from = (const int32_t *)ws + 4, *to = from + half, *map = to + half;
     if (blockIdx.x >= table_blocks) {
@@ -453,7 +492,8 @@ extern "C" size_t pulsar_kv_pool_workspace(const pulsar_kv_pool *p, uint32_t n) 
 static int pk_pool_check(const pulsar_kv_pool *p, const int32_t *status, const void *ws, size_t ws_bytes, uint32_t n) {
     const char *f = pk_pool_fault(p);
     if (f) return pk_refuse(f);
-    if (!status || !ws || ((uintptr_t)ws & 3u)) return pk_refuse("kv pool: null status or workspace");
+    if (!status || !ws || (((uintptr_t)ws | (uintptr_t)status) & 15u))
+        return pk_refuse("kv pool: status and workspace are there and aligned to 16 bytes");
     if (ws_bytes < pulsar_kv_pool_workspace(p, n)) return pk_refuse("kv pool: workspace too small");
     return pk_err_word() ? 1 : pk_refuse("kv pool: no error word on this device");
 }
@@ -481,8 +521,9 @@ extern "C" int pulsar_kv_fork(const pulsar_kv_pool *p, const int32_t *dst, const
     uint32_t tb = (p->max_pages + PK_FORK_COLS - 1) / PK_FORK_COLS;
     if (tb > 2 * sms) tb = 2 * sms;
     const uint32_t cb = p->n_slab ? 4 * sms : 0;
-    pk_fork_apply_kernel<<<tb + cb, 256, smem, st>>>(*p, dst, src, n, tb, ws, pk_err_word());
-    return pm_ok(cudaGetLastError(), "kv fork launch");
+    return pm_ok(pk_launch_after(pk_fork_apply_kernel, tb + cb, 256, smem, st, *p, dst, src, n, tb, (const void *)ws,
+                                 pk_err_word()),
+                 "kv fork launch");
 }
 
 extern "C" int pulsar_kv_compact(const pulsar_kv_pool *p, int32_t *status, void *ws, size_t ws_bytes, void *stream) {
@@ -493,6 +534,7 @@ extern "C" int pulsar_kv_compact(const pulsar_kv_pool *p, int32_t *status, void 
     const uint32_t sms = pk_sm_count();
     uint32_t tb = (p->n_rows + 7) / 8;
     if (tb > 2 * sms) tb = 2 * sms;
-    pk_compact_apply_kernel<<<tb + 4 * sms, 256, 0, st>>>(*p, tb, (const uint32_t *)ws, pk_err_word());
-    return pm_ok(cudaGetLastError(), "kv compact launch");
+    return pm_ok(pk_launch_after(pk_compact_apply_kernel, tb + 4 * sms, 256, 0, st, *p, tb, (const uint32_t *)ws,
+                                 pk_err_word()),
+                 "kv compact launch");
 }
