@@ -360,11 +360,12 @@ __device__ void pk_copy_pages(const pulsar_kv_pool &P, const int32_t *from, cons
     }
 }
 
-/* The first `table_blocks` CTAs rewrite the tables, 8 columns each: a CTA
- * reads its columns of every source row into shared memory before it writes
- * any row, so rows may trade places without a second buffer.  The other CTAs
- * copy pages: sources are live and targets were free, so the two kinds and
- * the copies among themselves do not touch. */
+/* The first `table_blocks` CTAs rewrite the tables, up to PK_FORK_COLS
+ * columns at a time (one, while there are CTAs enough): a CTA reads its
+ * columns of every source row into shared memory before it writes any row, so
+ * rows may trade places without a second buffer.  The other CTAs copy pages:
+ * sources are live and targets were free, so the two kinds and the copies
+ * among themselves do not touch. */
 __global__ void __launch_bounds__(256) pk_fork_apply_kernel(pulsar_kv_pool P, const int32_t *dst, const int32_t *src,
                                                             uint32_t n, uint32_t table_blocks, const void *wsp,
                                                             uint32_t *err) {
@@ -378,30 +379,33 @@ __global__ void __launch_bounds__(256) pk_fork_apply_kernel(pulsar_kv_pool P, co
     }
     if (blockIdx.x == 0)
         for (uint32_t i = threadIdx.x; i < n; i += blockDim.x) P.len[dst[i]] = (int32_t)w.now[i];
-    const uint32_t wide = w.head[2];
-    for (uint32_t c0 = blockIdx.x * PK_FORK_COLS; c0 < wide; c0 += table_blocks * PK_FORK_COLS) {
-        for (uint32_t u = threadIdx.x; u < n * PK_FORK_COLS; u += blockDim.x) {
-            const uint32_t i = u / PK_FORK_COLS, c = c0 + u % PK_FORK_COLS;
-            const bool same = src[i] == dst[i];
-            int32_t page = -1;
-            if (c < pk_ceil(w.now[i], P.page_size) && !same) {
-                const bool copied = w.fresh[i] >= 0 && c == w.now[i] / P.page_size;
-                page = copied ? w.fresh[i] : P.table[src[i] * P.table_stride + c];
+    const uint32_t wide = w.head[2], even = pk_ceil(wide, table_blocks);
+    const uint32_t cols = even < 1 ? 1 : even < PK_FORK_COLS ? even : PK_FORK_COLS;
+    for (uint32_t c0 = blockIdx.x * cols; c0 < wide; c0 += table_blocks * cols) {
+        for (uint32_t u = threadIdx.x; u < n * cols; u += blockDim.x) {
+            const uint32_t i = u / cols, c = c0 + u % cols;
+            const int32_t s = src[i], d = dst[i], copy = w.fresh[i];
+            const uint32_t now = w.now[i], was = w.was[i];
+            const bool holds = s != d && c < pk_ceil(now, P.page_size), held = s != d && c < pk_ceil(was, P.page_size);
+            int32_t page = -1, old = -1;
+            if (holds) page = copy >= 0 && c == now / P.page_size ? copy : P.table[s * P.table_stride + c];
+            if (held) old = P.table[d * P.table_stride + c];
+            if (holds) {
                 if ((uint32_t)page >= P.n_pages) atomicOr(err, PULSAR_KV_ERR_PAGE);
                 else atomicAdd(&P.refs[page], 1);
             }
-            if (c < pk_ceil(w.was[i], P.page_size) && !same) {
-                const int32_t old = P.table[dst[i] * P.table_stride + c];
+            if (held) {
                 if ((uint32_t)old >= P.n_pages) atomicOr(err, PULSAR_KV_ERR_PAGE);
                 else atomicSub(&P.refs[old], 1);
             }
             stage[u] = page;
         }
         __syncthreads();
-        for (uint32_t u = threadIdx.x; u < n * PK_FORK_COLS; u += blockDim.x) {
-            const uint32_t i = u / PK_FORK_COLS, c = c0 + u % PK_FORK_COLS;
-            const uint32_t most = w.was[i] > w.now[i] ? w.was[i] : w.now[i];
-            if (src[i] != dst[i] && c < pk_ceil(most, P.page_size)) P.table[dst[i] * P.table_stride + c] = stage[u];
+        for (uint32_t u = threadIdx.x; u < n * cols; u += blockDim.x) {
+            const uint32_t i = u / cols, c = c0 + u % cols;
+            const uint32_t now = w.now[i], was = w.was[i];
+            if (src[i] != dst[i] && c < pk_ceil(was > now ? was : now, P.page_size))
+                P.table[dst[i] * P.table_stride + c] = stage[u];
         }
         __syncthreads();
     }
@@ -518,8 +522,7 @@ extern "C" int pulsar_kv_fork(const pulsar_kv_pool *p, const int32_t *dst, const
     pk_fork_plan_kernel<<<1, PK_PLAN, 0, st>>>(*p, dst, src, n, status, ws);
     if (!pm_ok(cudaGetLastError(), "kv fork plan launch")) return 0;
     const uint32_t sms = pk_sm_count();
-    uint32_t tb = (p->max_pages + PK_FORK_COLS - 1) / PK_FORK_COLS;
-    if (tb > 2 * sms) tb = 2 * sms;
+    const uint32_t tb = p->max_pages < 2 * sms ? p->max_pages : 2 * sms;
     const uint32_t cb = p->n_slab ? 4 * sms : 0;
     return pm_ok(pk_launch_after(pk_fork_apply_kernel, tb + cb, 256, smem, st, *p, dst, src, n, tb, (const void *)ws,
                                  pk_err_word()),
