@@ -61,23 +61,21 @@ struct pk_attend_job {
     uint32_t *err;
 };
 
-/* OCC: CTAs that an SM holds.  Three (168 registers, rings of two stages)
- * where one 16-row output tile of up to 128 columns and q's parts fit in that;
- * else two; one at 256 columns, whose rings fill the shared memory. */
-template <uint32_t CT, int DP, int R, int MT, int QP>
+template <uint32_t CT, int DP, int R, int QP>
 struct pk_shape {
     static constexpr int ELT = CT == PULSAR_TYPE_E4M3 ? 1 : 2;
     static constexpr int ROW = DP * ELT;                  /* bytes of a key in shared memory */
     static constexpr int UNITS = ROW / 16;
     static constexpr int CK = ROW >= 256 ? 16 : 32;       /* keys per chunk: about 8 KB of keys and values */
-    static constexpr int OCC = DP > 128 ? 1 : PK_OCC;
+    static constexpr int OCC = DP > 128 ? 1 : PK_OCC;     /* CTAs that an SM holds */
     static constexpr int STAGES = OCC == 3 ? 2 : 3;
     static constexpr int STAGE = 2 * CK * ROW;
     static constexpr int RING = STAGES * STAGE;           /* per warp */
-    static constexpr int PASSES = OCC == 3 && DP == 128 ? 2 : 1;       /* of the exchange at a segment's end */
-    static constexpr int QCOLS = DP / 4 / PASSES;         /* columns of a quarter in a pass */
-    static constexpr int QROW = QCOLS + 4;                /* floats; padded against bank conflicts */
-    static constexpr int JOIN = 4 * 3 * 8 * QROW * 4;     /* bytes: each quarter, from three warps */
+    static constexpr bool QSM = DP > 128;                 /* q's parts wait in shared memory, not registers */
+    static constexpr int QW = R == 1 ? 2 * QP : 4 * QP;   /* their words per lane and k-step */
+    static constexpr int XROW = 64 + 4;                   /* floats of 64 columns in the warps' meeting; no bank conflicts */
+    static constexpr int MEET = PK_WARPS * 8 * XROW * 4, QALL = QSM ? DP / 16 * QW * 128 : 0;
+    static constexpr int SIDE = MEET > QALL ? MEET : QALL; /* bytes beside the rings: both, at different times */
 };
 
 __device__ __forceinline__ uint32_t pk_saddr(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -518,15 +516,15 @@ __device__ void pk_joint_finish(const pk_attend_job &J, const pk_joint &S, uint3
 
 /* ------------------------------------------------------------ the kernel */
 
-template <uint32_t CT, int DP, int R, int MT, int QP>
-__global__ void __launch_bounds__(PK_WARPS * 32, pk_shape<CT, DP, R, MT, QP>::OCC) pk_attend_kernel(const __grid_constant__ pk_attend_job J) {
-    typedef pk_shape<CT, DP, R, MT, QP> S;
+template <uint32_t CT, int DP, int R, int QP>
+__global__ void __launch_bounds__(PK_WARPS * 32, pk_shape<CT, DP, R, QP>::OCC) pk_attend_kernel(const __grid_constant__ pk_attend_job J) {
+    typedef pk_shape<CT, DP, R, QP> S;
     constexpr bool BF = CT == PULSAR_TYPE_BF16;
     constexpr bool F8 = CT == PULSAR_TYPE_E4M3;
     constexpr int CK = S::CK, KS = DP / 16, NT = DP / 8, KT = CK / 8;
-    constexpr int LR = MT * R, HEADS = 8 * LR;            /* a lane's query rows; a tile's */
-    constexpr bool QSM = MT > 1 || DP > 128;              /* q's parts wait in shared memory, not registers */
-    constexpr int QW = R == 1 ? 2 * QP : 4 * QP;            /* words per lane and k-step */
+    constexpr int HEADS = 8 * R;                          /* query rows of a tile; a lane's are R */
+    constexpr bool QSM = S::QSM;
+    constexpr int QW = S::QW;
     constexpr int PP = QP == 3 ? 3 : 2;                   /* parts of p */
     constexpr int PW = R == 1 ? (PP == 3 ? 6 : 4) : 4 * PP;
     constexpr bool REST = R == 1 ? QP == 3 : QP > 1;      /* lower parts of q have sums of their own */
@@ -534,12 +532,10 @@ __global__ void __launch_bounds__(PK_WARPS * 32, pk_shape<CT, DP, R, MT, QP>::OC
 
     extern __shared__ __align__(128) uint8_t smem[];
     uint8_t *ring = smem + (threadIdx.x >> 5) * S::RING;
-    float *join = (float *)(smem + PK_WARPS * S::RING);
-    uint32_t *upto = (uint32_t *)join;                    /* in the beginning */
-    /* QSM: [MT][KS][QW / 2][32][2], in the same bytes: q is done with when a segment's warps meet */
-    uint32_t *qsm = (uint32_t *)join;
-    static_assert(!QSM || MT * KS * QW * 128 <= S::JOIN, "q's parts fit beside the ring");
-    static_assert((PK_WARPS * 32 + PK_WARPS) * 4 <= S::JOIN, "the line's sums fit");
+    float *side = (float *)(smem + PK_WARPS * S::RING);
+    uint32_t *upto = (uint32_t *)side;                    /* in the beginning */
+    uint32_t *qsm = (uint32_t *)side;                     /* QSM: [KS][QW / 2][32][2], until a segment's warps meet */
+    static_assert((PK_WARPS * 32 + PK_WARPS) * 4 <= S::SIDE, "the line's sums fit");
     __shared__ float wml[PK_WARPS][HEADS][2];             /* each warp's maximum and sum */
     __shared__ float fml[HEADS][2];
     __shared__ uint32_t vmask[PK_WARPS][S::STAGES];       /* keys of a stage that are there */
@@ -719,12 +715,12 @@ __global__ void __launch_bounds__(PK_WARPS * 32, pk_shape<CT, DP, R, MT, QP>::OC
         constexpr int KN = QSM ? KS / PK_WARPS : KS;
         const uint32_t k0 = QSM ? w * KN : 0;
         uint32_t qr[QSM ? 1 : KS][QW];
-        float unit[LR];                                   /* score units: log2, the power of two taken from q */
-        int32_t slo[LR], shi[LR];
+        float unit[R];                                   /* score units: log2, the power of two taken from q */
+        int32_t slo[R], shi[R];
         {
-            float x[LR][KN][4];
+            float x[R][KN][4];
 #pragma unroll
-            for (int y = 0; y < LR; y++) {
+            for (int y = 0; y < R; y++) {
                 const uint32_t v = v0 + y * 8 + g;
                 const bool have = v < J.rows;
                 const uint32_t i = have ? v / J.group : 0, h = cons.hk * J.group + (have ? v % J.group : 0);
@@ -741,9 +737,9 @@ __global__ void __launch_bounds__(PK_WARPS * 32, pk_shape<CT, DP, R, MT, QP>::OC
             if (done == 0) /* behind q's loads in the queue, not before them */
 #pragma unroll 1
                 for (uint32_t st = 0; st < S::STAGES - 1; st++) issue(st);
-            float most[LR];
+            float most[R];
 #pragma unroll
-            for (int y = 0; y < LR; y++) {
+            for (int y = 0; y < R; y++) {
                 most[y] = 0.0f;
 #pragma unroll
                 for (int n = 0; n < KN; n++)
@@ -761,7 +757,7 @@ __global__ void __launch_bounds__(PK_WARPS * 32, pk_shape<CT, DP, R, MT, QP>::OC
             if (!BF) {
                 if (QSM) __syncthreads();
 #pragma unroll
-                for (int y = 0; y < LR; y++) {
+                for (int y = 0; y < R; y++) {
                     if (QSM)
 #pragma unroll
                         for (uint32_t k = 0; k < PK_WARPS; k++) most[y] = fmaxf(most[y], wml[k][y * 8 + g][0]);
@@ -777,35 +773,27 @@ __global__ void __launch_bounds__(PK_WARPS * 32, pk_shape<CT, DP, R, MT, QP>::OC
                 }
             }
 #pragma unroll
-            for (int mt = 0; mt < MT; mt++)
+            for (int n = 0; n < KN; n++) {
+                uint32_t p[QW];
 #pragma unroll
-                for (int n = 0; n < KN; n++) {
-                    uint32_t p[QW];
-                    if constexpr (R == 1) {
-#pragma unroll
-                        for (int e = 0; e < QW; e++) p[e] = pk_split<BF, true>(x[0][n][2 * (e & 1)], x[0][n][2 * (e & 1) + 1]);
-                    } else {
-#pragma unroll
-                        for (int q = 0; q < QP; q++)
-#pragma unroll
-                            for (int e = 0; e < 4; e++) {
-                                float *z = x[mt * R + (e & 1) * (R - 1)][n] + (e & 2);
-                                p[4 * q + e] = pk_split<BF, true>(z[0], z[1]);
-                            }
-                    }
-#pragma unroll
-                    for (int e = 0; e < QW; e++) {
-                        if constexpr (QSM) qsm[(((mt * KS + k0 + n) * (QW / 2) + e / 2) * 32 + lane) * 2 + (e & 1)] = p[e];
-                        else qr[n][e] = p[e];
-                    }
+                for (int e = 0; e < QW; e++) {
+                    /* R = 1: parts of (row g, low columns), (row g, high); R = 2: (g, low), (g + 8, low), (g, high), (g + 8, high) */
+                    float *z = R == 1 ? x[0][n] + 2 * (e & 1) : x[(e & 1) * (R - 1)][n] + (e & 2);
+                    p[e] = pk_split<BF, true>(z[0], z[1]);
                 }
+#pragma unroll
+                for (int e = 0; e < QW; e++) {
+                    if constexpr (QSM) qsm[(((k0 + n) * (QW / 2) + e / 2) * 32 + lane) * 2 + (e & 1)] = p[e];
+                    else qr[n][e] = p[e];
+                }
+            }
         }
         if constexpr (QSM) __syncthreads();
-        auto q_words = [&](int mt, int ks, uint32_t *a) {
+        auto q_words = [&](int ks, uint32_t *a) {
 #pragma unroll
             for (int e = 0; e < QW; e += 2) {
                 if constexpr (QSM) {
-                    const uint2 z = ((const uint2 *)qsm)[((mt * KS + ks) * (QW / 2) + e / 2) * 32 + lane];
+                    const uint2 z = ((const uint2 *)qsm)[(ks * (QW / 2) + e / 2) * 32 + lane];
                     a[e] = z.x;
                     a[e + 1] = z.y;
                 } else {
@@ -815,18 +803,16 @@ __global__ void __launch_bounds__(PK_WARPS * 32, pk_shape<CT, DP, R, MT, QP>::OC
             }
         };
 
-        float o[MT][NT][4], m[LR], l[LR];
+        float o[NT][4], m[R], l[R];
 #pragma unroll
-        for (int y = 0; y < LR; y++) {
+        for (int y = 0; y < R; y++) {
             m[y] = -INFINITY;
             l[y] = 0.0f;
         }
 #pragma unroll
-        for (int mt = 0; mt < MT; mt++)
+        for (int t = 0; t < NT; t++)
 #pragma unroll
-            for (int t = 0; t < NT; t++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) o[mt][t][e] = 0.0f;
+            for (int e = 0; e < 4; e++) o[t][e] = 0.0f;
 
         /* ---- the warp's chunks of this segment */
         const uint32_t end = done + (uint32_t)(to - from);
@@ -850,65 +836,44 @@ __global__ void __launch_bounds__(PK_WARPS * 32, pk_shape<CT, DP, R, MT, QP>::OC
             const int32_t key0 = (cons.row.c0 + from + (int32_t)(next - done)) * CK;
 
             /* scores: keys are the columns */
-            constexpr int CHAINS = MT == 1 && KT == 2 ? 2 : 1; /* two columns of sums alone would wait on themselves */
-            float s[MT][KT][4], rest[REST ? MT : 1][KT][4], odd[CHAINS == 2 ? KT : 1][4];
+            constexpr int CHAINS = KT == 2 ? 2 : 1; /* two columns of sums alone would wait on themselves */
+            float s[KT][4], rest[REST ? KT : 1][4], odd[CHAINS == 2 ? KT : 1][4];
 #pragma unroll
-            for (int mt = 0; mt < MT; mt++)
+            for (int t = 0; t < KT; t++)
 #pragma unroll
-                for (int t = 0; t < KT; t++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        s[mt][t][e] = 0.0f;
-                        if constexpr (CHAINS == 2) odd[t][e] = 0.0f;
-                        if constexpr (REST) rest[mt][t][e] = 0.0f;
-                    }
-            auto score = [&](int mt, int t, int ks, const uint32_t *a, uint32_t b0, uint32_t b1) {
-                float *sum = CHAINS == 2 && (ks & 1) ? odd[CHAINS == 2 ? t : 0] : s[mt][t];
+                for (int e = 0; e < 4; e++) {
+                    s[t][e] = 0.0f;
+                    if constexpr (CHAINS == 2) odd[t][e] = 0.0f;
+                    if constexpr (REST) rest[t][e] = 0.0f;
+                }
+            auto score = [&](int t, int ks, const uint32_t *a, uint32_t b0, uint32_t b1) {
+                float *sum = CHAINS == 2 && (ks & 1) ? odd[CHAINS == 2 ? t : 0] : s[t];
                 if constexpr (R == 1) pk_mma<BF>(sum, a[0], QP > 1 ? a[QW > 2 ? 2 : 0] : 0, a[1], QP > 1 ? a[QW > 2 ? 3 : 1] : 0, b0, b1);
                 else pk_mma<BF>(sum, a[0], a[1], a[2], a[3], b0, b1);
-                if constexpr (R == 1 && QP == 3) pk_mma<BF>(rest[mt][t], a[4], 0, a[5], 0, b0, b1);
-                if constexpr (R == 2 && QP > 1) pk_mma<BF>(rest[mt][t], a[4], a[5], a[6], a[7], b0, b1);
-                if constexpr (R == 2 && QP > 2) pk_mma<BF>(rest[mt][t], a[8], a[9], a[10], a[11], b0, b1);
+                if constexpr (R == 1 && QP == 3) pk_mma<BF>(rest[REST ? t : 0], a[4], 0, a[5], 0, b0, b1);
+                if constexpr (R == 2 && QP > 1) pk_mma<BF>(rest[REST ? t : 0], a[4], a[5], a[6], a[7], b0, b1);
+                if constexpr (R == 2 && QP > 2) pk_mma<BF>(rest[REST ? t : 0], a[8], a[9], a[10], a[11], b0, b1);
             };
             constexpr int KQ = F8 && KT == 2 ? 2 : 1; /* k-steps per load: 16-key e4m3 chunks take two */
 #pragma unroll
             for (int ks = 0; ks < KS; ks += KQ) {
-                uint32_t a[MT][KQ][QW];
+                uint32_t a[KQ][QW], b[4];
 #pragma unroll
-                for (int mt = 0; mt < MT; mt++)
-#pragma unroll
-                    for (int q = 0; q < KQ; q++) q_words(mt, ks + q, a[mt][q]);
+                for (int q = 0; q < KQ; q++) q_words(ks + q, a[q]);
                 if constexpr (!F8) {
                     /* matrices (keys 0-7, d 0-7), (0-7, 8-15), (8-15, 0-7), (8-15, 8-15) */
 #pragma unroll
                     for (int t = 0; t < KT; t += 2) {
-                        uint32_t b[4];
                         pk_ldm4(b, unit_at(kx, 2 * ks) + t * 8 * S::ROW);
-#pragma unroll
-                        for (int mt = 0; mt < MT; mt++) {
-                            score(mt, t, ks, a[mt][0], b[0], b[1]);
-                            score(mt, t + 1, ks, a[mt][0], b[2], b[3]);
-                        }
-                    }
-                } else if constexpr (KT == 4) {
-                    /* a matrix is 8 keys x 16 bytes */
-                    uint32_t b[4];
-                    pk_ldm4(b, unit_at(kx, ks));
-#pragma unroll
-                    for (int t = 0; t < 4; t++) {
-                        const uint32_t b0 = pk_e4m3x2(b[t]), b1 = pk_e4m3x2(b[t] >> 16);
-#pragma unroll
-                        for (int mt = 0; mt < MT; mt++) score(mt, t, ks, a[mt][0], b0, b1);
+                        score(t, ks, a[0], b[0], b[1]);
+                        score(t + 1, ks, a[0], b[2], b[3]);
                     }
                 } else {
-                    uint32_t b[4];
+                    /* a matrix is 8 keys x 16 bytes: four groups of keys, or two groups and two k-steps */
                     pk_ldm4(b, unit_at(kx, ks));
 #pragma unroll
-                    for (int t = 0; t < 4; t++) {
-                        const uint32_t b0 = pk_e4m3x2(b[t]), b1 = pk_e4m3x2(b[t] >> 16);
-#pragma unroll
-                        for (int mt = 0; mt < MT; mt++) score(mt, t & 1, t >> 1, a[mt][KQ - 1 < (t >> 1) ? 0 : t >> 1], b0, b1);
-                    }
+                    for (int t = 0; t < 4; t++)
+                        score(t % KT, ks + t / KT, a[KQ == 2 ? t / KT : 0], pk_e4m3x2(b[t]), pk_e4m3x2(b[t] >> 16));
                 }
             }
 
@@ -917,26 +882,25 @@ __global__ void __launch_bounds__(PK_WARPS * 32, pk_shape<CT, DP, R, MT, QP>::OC
              * Weights are relative to m less LIFT: at most 2^15, so that f16 holds them, and small ones stay
              * clear of its subnormals.  p's parts are the left factors of the output products in the layout that
              * they already have. */
-            float top[LR];
+            float top[R];
             bool moved = false;
 #pragma unroll
-            for (int y = 0; y < LR; y++) {
+            for (int y = 0; y < R; y++) {
                 constexpr uint32_t ALL = CK == 32 ? ~0u : (1u << (CK & 31)) - 1u;
-                const int mt = y / R, r = y % R;
                 const bool whole = there == ALL && key0 >= slo[y] && key0 + CK <= shi[y];
                 top[y] = -INFINITY;
 #pragma unroll
                 for (int t = 0; t < KT; t++)
 #pragma unroll
                     for (int e = 0; e < 2; e++) {
-                        float &x = s[mt][t][2 * r + e];
-                        if constexpr (CHAINS == 2) x += odd[t][2 * r + e];
+                        float &x = s[t][2 * y + e];
+                        if constexpr (CHAINS == 2) x += odd[t][2 * y + e];
                         if constexpr (R == 1 && QP > 1) {
-                            float low = s[mt][t][e + 2];
+                            float low = s[t][e + 2];
                             if constexpr (CHAINS == 2) low += odd[t][e + 2];
-                            x = pk_fold(x, QP == 3 ? low + rest[0][t][e] : low);
+                            x = pk_fold(x, QP == 3 ? low + rest[REST ? t : 0][e] : low);
                         }
-                        if constexpr (R == 2 && QP > 1) x = pk_fold(x, rest[mt][t][2 * r + e]);
+                        if constexpr (R == 2 && QP > 1) x = pk_fold(x, rest[REST ? t : 0][2 * y + e]);
                         x *= unit[y];
                         if (!whole) {
                             const int32_t k = t * 8 + 2 * (int32_t)c + e;
@@ -948,12 +912,12 @@ __global__ void __launch_bounds__(PK_WARPS * 32, pk_shape<CT, DP, R, MT, QP>::OC
 #pragma unroll
             for (int o2 = 1; o2 < 4; o2 <<= 1)
 #pragma unroll
-                for (int y = 0; y < LR; y++) top[y] = fmaxf(top[y], __shfl_xor_sync(~0u, top[y], o2));
+                for (int y = 0; y < R; y++) top[y] = fmaxf(top[y], __shfl_xor_sync(~0u, top[y], o2));
 #pragma unroll
-            for (int y = 0; y < LR; y++) moved |= top[y] > m[y] + SLACK;
+            for (int y = 0; y < R; y++) moved |= top[y] > m[y] + SLACK;
             if (__any_sync(~0u, moved)) {
 #pragma unroll
-                for (int y = 0; y < LR; y++) {
+                for (int y = 0; y < R; y++) {
                     const float to = top[y] > m[y] + SLACK ? top[y] : m[y];
                     const float keep = to == m[y] ? 1.0f : pk_exp2(m[y] - to);
                     m[y] = to;
@@ -962,65 +926,61 @@ __global__ void __launch_bounds__(PK_WARPS * 32, pk_shape<CT, DP, R, MT, QP>::OC
                     for (int t = 0; t < NT; t++) {
                         if constexpr (R == 1) {
 #pragma unroll
-                            for (int e = 0; e < 4; e++) o[y][t][e] *= keep;
+                            for (int e = 0; e < 4; e++) o[t][e] *= keep;
                         } else {
-                            o[y / R][t][2 * (y % R)] *= keep;
-                            o[y / R][t][2 * (y % R) + 1] *= keep;
+                            o[t][2 * y] *= keep;
+                            o[t][2 * y + 1] *= keep;
                         }
                     }
                 }
             }
-            uint32_t pa[MT][KT / 2][PW];
+            uint32_t pa[KT / 2][PW];
 #pragma unroll
-            for (int y = 0; y < LR; y++) {
+            for (int y = 0; y < R; y++) {
                 const float zero = (m[y] == -INFINITY ? 0.0f : m[y]) - LIFT; /* nothing seen yet: every weight is 0 */
 #pragma unroll
                 for (int t = 0; t < KT; t++)
 #pragma unroll
                     for (int e = 0; e < 2; e++) {
-                        float &x = s[y / R][t][2 * (y % R) + e];
+                        float &x = s[t][2 * y + e];
                         x = pk_exp2(x - zero);
                         l[y] += x;
                     }
             }
 #pragma unroll
-            for (int mt = 0; mt < MT; mt++)
-#pragma unroll
-                for (int kt = 0; kt < KT / 2; kt++) {
-                    uint32_t *a = pa[mt][kt];
-                    if constexpr (R == 1) {
-                        float *p0 = s[mt][2 * kt], *p1 = s[mt][2 * kt + 1];
-                        a[0] = pk_split<BF, false>(p0[0], p0[1]);
-                        a[2] = pk_split<BF, false>(p1[0], p1[1]);
-                        a[1] = pk_split<BF, false>(p0[0], p0[1]);
-                        a[3] = pk_split<BF, false>(p1[0], p1[1]);
-                        if constexpr (PP == 3) {
-                            a[4] = pk_split<BF, false>(p0[0], p0[1]);
-                            a[5] = pk_split<BF, false>(p1[0], p1[1]);
-                        }
-                    } else {
-#pragma unroll
-                        for (int q = 0; q < PP; q++)
-#pragma unroll
-                            for (int e = 0; e < 4; e++) {
-                                float *z = s[mt][2 * kt + (e >> 1)] + 2 * (e & 1);
-                                a[4 * q + e] = pk_split<BF, false>(z[0], z[1]);
-                            }
+            for (int kt = 0; kt < KT / 2; kt++) {
+                uint32_t *a = pa[kt];
+                float *p0 = s[2 * kt], *p1 = s[2 * kt + 1];
+                if constexpr (R == 1) {
+                    a[0] = pk_split<BF, false>(p0[0], p0[1]);
+                    a[2] = pk_split<BF, false>(p1[0], p1[1]);
+                    a[1] = pk_split<BF, false>(p0[0], p0[1]);
+                    a[3] = pk_split<BF, false>(p1[0], p1[1]);
+                    if constexpr (PP == 3) {
+                        a[4] = pk_split<BF, false>(p0[0], p0[1]);
+                        a[5] = pk_split<BF, false>(p1[0], p1[1]);
                     }
+                } else {
+#pragma unroll
+                    for (int q = 0; q < PP; q++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            float *z = (e < 2 ? p0 : p1) + 2 * (e & 1);
+                            a[4 * q + e] = pk_split<BF, false>(z[0], z[1]);
+                        }
                 }
+            }
             /* output tiles t and t + 1; a part's products for all tiles before the next part's, which add to the same sums */
             auto weigh = [&](int t, int kt, const uint32_t *b) {
                 constexpr int TIMES = R == 1 ? PP - 1 : PP;
 #pragma unroll
                 for (int q = 0; q < TIMES; q++)
 #pragma unroll
-                    for (int mt = 0; mt < MT; mt++)
-#pragma unroll
-                        for (int x = 0; x < 2; x++) {
-                            const uint32_t *a = pa[mt][kt] + 4 * q;
-                            if (R == 1 && q == 1) pk_mma<BF>(o[mt][t + x], a[0], 0, a[PW > 5 ? 1 : 0], 0, b[2 * x], b[2 * x + 1]);
-                            else pk_mma<BF>(o[mt][t + x], a[0], a[1], a[2], a[3], b[2 * x], b[2 * x + 1]);
-                        }
+                    for (int x = 0; x < 2; x++) {
+                        const uint32_t *a = pa[kt] + 4 * q;
+                        if (R == 1 && q == 1) pk_mma<BF>(o[t + x], a[0], 0, a[PW > 5 ? 1 : 0], 0, b[2 * x], b[2 * x + 1]);
+                        else pk_mma<BF>(o[t + x], a[0], a[1], a[2], a[3], b[2 * x], b[2 * x + 1]);
+                    }
             };
 #pragma unroll
             for (int kt = 0; kt < KT / 2; kt++) {
@@ -1047,10 +1007,10 @@ __global__ void __launch_bounds__(PK_WARPS * 32, pk_shape<CT, DP, R, MT, QP>::OC
 
         /* ---- the segment's end */
         const uint32_t took = (uint32_t)(to - from);
-        constexpr int QT = NT / 4, RUN = F8 ? 4 : 2;      /* tiles of a quarter of the columns; a lane's run of columns */
+        constexpr int RUN = F8 ? 4 : 2;                   /* a lane's run of columns */
         /* RUN neighbouring columns of row y at tile t: folded parts, times by */
         auto columns = [&](int y, int t, float by, float *x) {
-            const float *a = o[y / R][t], *b2 = o[y / R][F8 ? t + 1 : t];
+            const float *a = o[t], *b2 = o[F8 ? t + 1 : t];
             if constexpr (R == 1) {
                 x[0] = pk_fold(a[0], a[2]);
                 x[RUN - 2 > 0 ? 2 : 1] = pk_fold(a[1], a[3]);
@@ -1059,25 +1019,25 @@ __global__ void __launch_bounds__(PK_WARPS * 32, pk_shape<CT, DP, R, MT, QP>::OC
                     x[RUN - 1] = pk_fold(b2[1], b2[3]);
                 }
             } else {
-                x[0] = a[2 * (y % R)];
-                x[RUN - 2 > 0 ? 2 : 1] = a[2 * (y % R) + 1];
+                x[0] = a[2 * y];
+                x[RUN - 2 > 0 ? 2 : 1] = a[2 * y + 1];
                 if constexpr (F8) {
-                    x[1] = b2[2 * (y % R)];
-                    x[RUN - 1] = b2[2 * (y % R) + 1];
+                    x[1] = b2[2 * y];
+                    x[RUN - 1] = b2[2 * y + 1];
                 }
             }
 #pragma unroll
             for (int e = 0; e < RUN; e++) x[e] *= by;
         };
 #pragma unroll
-        for (int y = 0; y < LR; y++) {
+        for (int y = 0; y < R; y++) {
             l[y] += __shfl_xor_sync(~0u, l[y], 1);
             l[y] += __shfl_xor_sync(~0u, l[y], 2);
         }
         const float drop = BF ? 1.0f : 1.0f / 128.0f;     /* 2^-LIFT */
         if (solo) {
 #pragma unroll
-            for (int y = 0; y < LR; y++) {
+            for (int y = 0; y < R; y++) {
                 const uint32_t v = v0 + y * 8 + g;
                 if (v >= J.rows) continue;
                 const float by = drop * pk_finish(J, cons.b, cons.row.len, cons.hk, v, m[y], l[y] * drop, c == 0);
@@ -1090,16 +1050,15 @@ __global__ void __launch_bounds__(PK_WARPS * 32, pk_shape<CT, DP, R, MT, QP>::OC
                 }
             }
         } else {
-            /* the four warps meet: maxima, then each quarter of the columns goes to one warp */
+            /* the four warps meet: maxima, then the sums of 64 columns at a time */
             const bool cut = from != 0 || to != cons.row.n;
             float *part = J.parts + (uint64_t)(2 * blockIdx.x + (done != 0)) * (HEADS * (DP + 2));
 #pragma unroll
-            for (int y = 0; y < LR; y++)
+            for (int y = 0; y < R; y++)
                 if (c == 0) *(float2 *)wml[w][y * 8 + g] = make_float2(m[y], l[y] * drop);
             __syncthreads();
 #pragma unroll
-            for (int y = 0; y < LR; y++) {
-                if (y) __syncthreads(); /* the previous rows' sums are out of `join` */
+            for (int y = 0; y < R; y++) {
                 float top = -INFINITY, sum = 0.0f;
 #pragma unroll
                 for (uint32_t k = 0; k < PK_WARPS; k++) top = fmaxf(top, wml[k][y * 8 + g][0]);
@@ -1112,56 +1071,35 @@ __global__ void __launch_bounds__(PK_WARPS * 32, pk_shape<CT, DP, R, MT, QP>::OC
                     if (!cut && v < J.rows) top = pk_finish(J, cons.b, cons.row.len, cons.hk, v, top, sum);
                     *(float2 *)fml[y * 8 + g] = make_float2(top, sum); /* uncut: [0] is the output's factor */
                 }
-                auto place = [&](uint32_t owner, uint32_t source, int tq) {
-                    return join + ((owner * 3 + source) * 8 + g) * S::QROW + tq * 8 + RUN * c;
-                };
 #pragma unroll
-                for (int pass = 0; pass < S::PASSES; pass++) {
-                    constexpr int PT = QT / S::PASSES;    /* tiles of a quarter in a pass */
-                    if (pass) __syncthreads();
+                for (int c0 = 0; c0 < DP; c0 += 64) {
+                    if (y || c0) __syncthreads(); /* the previous columns have been read */
 #pragma unroll
-                    for (uint32_t q = 0; q < 4; q++)
-                        if (q != w)
-#pragma unroll
-                            for (int t = 0; t < PT; t += RUN / 2) {
-                                float x[RUN], *d = place(q, w < q ? w : w - 1, t);
-                                columns(y, q * QT + pass * PT + t, keep, x);
-                                if constexpr (F8) *(float4 *)d = make_float4(x[0], x[1], x[RUN - 2], x[RUN - 1]);
-                                else *(float2 *)d = make_float2(x[0], x[1]);
-                            }
+                    for (int t = 0; t < 8; t += RUN / 2) {
+                        float x[RUN], *d = side + (w * 8 + g) * S::XROW + t * 8 + RUN * c;
+                        columns(y, c0 / 8 + t, keep, x);
+                        if constexpr (F8) *(float4 *)d = make_float4(x[0], x[1], x[RUN - 2], x[RUN - 1]);
+                        else *(float2 *)d = make_float2(x[0], x[1]);
+                    }
                     __syncthreads();
+                    /* four columns of a row a thread: out, or into the workspace */
+                    static_assert(PK_WARPS * 32 == 8 * 64 / 4, "one run of four columns a thread");
+                    const uint32_t head = y * 8 + tid / 16, col = c0 + tid % 16 * 4;
+                    float4 z = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-                    for (uint32_t q = 0; q < 4; q++)
-                        if (q == w)
-#pragma unroll
-                            for (int t = 0; t < PT; t += RUN / 2) {
-                                float own[RUN], x[RUN], *d = place(q, 0, t);
-                                columns(y, q * QT + pass * PT + t, keep, own);
-#pragma unroll
-                                for (int e = 0; e < RUN; e++) {
-                                    x[e] = 0.0f;
-#pragma unroll
-                                    for (uint32_t k = 0; k < 4; k++) x[e] += k == q ? own[e] : place(q, k < q ? k : k - 1, t)[e];
-                                }
-#pragma unroll
-                                for (int e = 0; e < RUN; e++) d[e] = x[e];
-                            }
-                    __syncthreads();
-
-                    /* out, or into the workspace */
-                    constexpr uint32_t C4 = S::QCOLS;     /* runs of 4 columns of a row in a pass, all quarters */
-                    for (uint32_t i = tid; i < 8 * C4; i += PK_WARPS * 32) {
-                        const uint32_t hh = i / C4, q = i % C4 / (C4 / 4), in = i % (C4 / 4) * 4;
-                        const uint32_t col = q * (DP / 4) + pass * S::QCOLS + in, head = y * 8 + hh;
-                        const float4 x = *(const float4 *)(join + ((q * 3) * 8 + hh) * S::QROW + in);
-                        if (cut) {
-                            __stcg((float4 *)(part + 2 * HEADS + head * DP + col), x);
-                            if (col == 0) __stcg((float2 *)(part + 2 * head), make_float2(fml[head][0], fml[head][1]));
-                        } else if (v0 + head < J.rows && col < J.D.head_dim) {
-                            const float by = fml[head][0];
-                            const float z[4] = {x.x * by, x.y * by, x.z * by, x.w * by};
-                            pk_put<4>(J, cons.b, cons.hk, v0 + head, col, z);
-                        }
+                    for (uint32_t k = 0; k < PK_WARPS; k++) {
+                        const float4 v = *(const float4 *)(side + (k * 8 + tid / 16) * S::XROW + tid % 16 * 4);
+                        z.x += v.x;
+                        z.y += v.y;
+                        z.z += v.z;
+                        z.w += v.w;
+                    }
+                    if (cut) {
+                        __stcg((float4 *)(part + 2 * HEADS + head * DP + col), z);
+                        if (col == 0) __stcg((float2 *)(part + 2 * head), make_float2(fml[head][0], fml[head][1]));
+                    } else if (v0 + head < J.rows && col < J.D.head_dim) {
+                        const float by = fml[head][0], q4[4] = {z.x * by, z.y * by, z.z * by, z.w * by};
+                        pk_put<4>(J, cons.b, cons.hk, v0 + head, col, q4);
                     }
                 }
             }
@@ -1192,7 +1130,7 @@ __global__ void __launch_bounds__(PK_WARPS * 32, pk_shape<CT, DP, R, MT, QP>::OC
                     }
                 }
             }
-            __syncthreads(); /* wml, fml, join and qsm are free again */
+            __syncthreads(); /* wml, fml and side are free again */
         }
         done += took;
         if (done < slice) cons.step(J, cached, (int32_t)took);
@@ -1204,37 +1142,34 @@ __global__ void __launch_bounds__(PK_WARPS * 32, pk_shape<CT, DP, R, MT, QP>::OC
     if (also) pk_joint_finish<DP, HEADS, PARTS>(J, joint, &last, fml, (float *)smem);
 }
 
-template <uint32_t CT, int DP, int R, int MT, int QP>
+template <uint32_t CT, int DP, int R, int QP>
 static int pk_attend_launch(const pk_attend_job &J, uint32_t grid, cudaStream_t st) {
-    typedef pk_shape<CT, DP, R, MT, QP> S;
+    typedef pk_shape<CT, DP, R, QP> S;
     static uint64_t done = 0;
-    constexpr uint32_t smem = PK_WARPS * S::RING + S::JOIN;
-    auto kernel = pk_attend_kernel<CT, DP, R, MT, QP>;
+    constexpr uint32_t smem = PK_WARPS * S::RING + S::SIDE;
+    auto kernel = pk_attend_kernel<CT, DP, R, QP>;
     if (!pm_smem_attr(kernel, smem, &done)) return 0;
     kernel<<<grid, PK_WARPS * 32, smem, st>>>(J);
     return pm_ok(cudaGetLastError(), "kv attend launch");
 }
 
-/* one translation unit per cache type (kv_attend_*.cu); r, mt and qp as the
- * kernel's, wide: q has more bits than one part holds */
+/* one translation unit per cache type (kv_attend_*.cu); r as the kernel's R,
+ * wide: q has more bits than one part holds */
 typedef int (*pk_attend_fn)(const pk_attend_job &, uint32_t, cudaStream_t);
-pk_attend_fn pk_attend_bf16(int dp, int r, int mt, bool wide);
-pk_attend_fn pk_attend_f16(int dp, int r, int mt, bool wide);
-pk_attend_fn pk_attend_e4m3(int dp, int r, int mt, bool wide);
+pk_attend_fn pk_attend_bf16(int dp, int r, bool wide);
+pk_attend_fn pk_attend_f16(int dp, int r, bool wide);
+pk_attend_fn pk_attend_e4m3(int dp, int r, bool wide);
 
 template <uint32_t CT, int DP>
-static pk_attend_fn pk_attend_pick_at(int r, int mt, bool wide) {
+static pk_attend_fn pk_attend_pick_at(int r, bool wide) {
     constexpr int MOST = CT == PULSAR_TYPE_BF16 ? 3 : 2; /* parts of wide q */
-    if (r == 1) return wide ? pk_attend_launch<CT, DP, 1, 1, MOST> : pk_attend_launch<CT, DP, 1, 1, 1>;
-    if (wide) return pk_attend_launch<CT, DP, 2, 1, MOST>;
-    if constexpr (DP <= 128)
-        if (mt == 2) return pk_attend_launch<CT, DP, 2, 2, 1>;
-    return pk_attend_launch<CT, DP, 2, 1, 1>;
+    if (r == 1) return wide ? pk_attend_launch<CT, DP, 1, MOST> : pk_attend_launch<CT, DP, 1, 1>;
+    return wide ? pk_attend_launch<CT, DP, 2, MOST> : pk_attend_launch<CT, DP, 2, 1>;
 }
 
 template <uint32_t CT>
-static pk_attend_fn pk_attend_pick(int dp, int r, int mt, bool wide) {
-    if (dp == 64) return pk_attend_pick_at<CT, 64>(r, mt, wide);
-    if (dp == 128) return pk_attend_pick_at<CT, 128>(r, mt, wide);
-    return pk_attend_pick_at<CT, 256>(r, mt, wide);
+static pk_attend_fn pk_attend_pick(int dp, int r, bool wide) {
+    if (dp == 64) return pk_attend_pick_at<CT, 64>(r, wide);
+    if (dp == 128) return pk_attend_pick_at<CT, 128>(r, wide);
+    return pk_attend_pick_at<CT, 256>(r, wide);
 }
