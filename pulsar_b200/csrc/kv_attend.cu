@@ -41,10 +41,10 @@ static int pk_attend_prepare(const pulsar_kv_desc *d, const pulsar_kv_attend_arg
         if (d->page_size == 1u << s) J->page_shift = s;
     const uint32_t qe = pk_type_bytes(a->q_type);
     J->pairs = (((uintptr_t)a->q | a->q_stride * qe) % (2 * qe)) == 0;
-    const uint32_t elt = pk_type_bytes(d->dtype), ck = (uint32_t)p->dp * elt >= 256 ? 16 : 32;
+    const uint32_t ck = PK_CK;
     J->least = 128 / ck;
     /* CTAs that are resident together (pk_shape's OCC) */
-    p->workers = pk_sm_count() * (p->dp == 256 ? 1 : PK_OCC);
+    p->workers = pk_sm_count() * (p->dp == 256 ? 1 : 2);
     if (p->workers > PK_MAX_WORKERS) p->workers = PK_MAX_WORKERS;
     /* no more CTAs than the longest rows could feed; no more rows in a launch
      * than a line of less than 2^32 chunks holds */

@@ -16,7 +16,7 @@
  * own running maximum, sum and output tile, and meet at a segment's end; a
  * segment that a slice cuts is joined through the workspace by the CTA that
  * arrives last, in the order of the slices (a fixed order: the same call
- * gives the same bits), 32 parts at a time.  Many short segments (16 chunks
+ * gives the same bits), 32 parts at a time.  Many short segments (8 chunks
  * or fewer on average, more of them than CTAs): a worker is a warp, which
  * takes whole segments and meets nobody.
  *
@@ -38,9 +38,7 @@
 #include "pk_common.h"
 
 #define PK_WARPS 4u
-#ifndef PK_OCC
-#define PK_OCC 2
-#endif
+#define PK_CK 32              /* keys per chunk: a lane each */
 #define PK_GROUP 32u          /* parts joined at a time */
 #define PK_MAX_WORKERS 1024u  /* 2 x 2 counters of each fill PULSAR_KV_WS_ZEROED / 2 */
 #define PK_LOG2E 1.4426950408889634f
@@ -66,10 +64,13 @@ struct pk_shape {
     static constexpr int ELT = CT == PULSAR_TYPE_E4M3 ? 1 : 2;
     static constexpr int ROW = DP * ELT;                  /* bytes of a key in shared memory */
     static constexpr int UNITS = ROW / 16;
-    static constexpr int CK = ROW >= 256 ? 16 : 32;       /* keys per chunk: about 8 KB of keys and values */
-    static constexpr int OCC = DP > 128 ? 1 : PK_OCC;     /* CTAs that an SM holds */
-    static constexpr int STAGES = OCC == 3 ? 2 : 3;
-    static constexpr int STAGE = 2 * CK * ROW;
+    /* A stage of the ring is a chunk's keys and values; at rows of 256 bytes or more its keys or its values,
+     * which take turns: stages stay at 4 to 16 KB, and a chunk, whose bookkeeping and softmax cost the same
+     * for any number of keys, stays at PK_CK. */
+    static constexpr bool SPLIT = ROW >= 256;
+    static constexpr int STAGES = 3;
+    static constexpr int OCC = DP > 128 ? 1 : 2;          /* CTAs that an SM holds */
+    static constexpr int STAGE = (SPLIT ? 1 : 2) * PK_CK * ROW;
     static constexpr int RING = STAGES * STAGE;           /* per warp */
     static constexpr bool QSM = DP > 128;                 /* q's parts wait in shared memory, not registers */
     static constexpr int QW = R == 1 ? 2 * QP : 4 * QP;   /* their words per lane and k-step */
@@ -521,7 +522,7 @@ __global__ void __launch_bounds__(PK_WARPS * 32, pk_shape<CT, DP, R, QP>::OCC) p
     typedef pk_shape<CT, DP, R, QP> S;
     constexpr bool BF = CT == PULSAR_TYPE_BF16;
     constexpr bool F8 = CT == PULSAR_TYPE_E4M3;
-    constexpr int CK = S::CK, KS = DP / 16, NT = DP / 8, KT = CK / 8;
+    constexpr int CK = PK_CK, KS = DP / 16, NT = DP / 8, KT = CK / 8;
     constexpr int HEADS = 8 * R;                          /* query rows of a tile; a lane's are R */
     constexpr bool QSM = S::QSM;
     constexpr int QW = S::QW;
@@ -563,15 +564,15 @@ __global__ void __launch_bounds__(PK_WARPS * 32, pk_shape<CT, DP, R, QP>::OCC) p
 
     /* ---- the worker's slice of it */
     const uint32_t total = all * J.segs, segs = B * J.segs;
-    const bool brief = all <= 16u * B;                    /* 16 chunks a segment or fewer, on average */
+    const bool brief = all <= 8u * B;                     /* 8 chunks a segment or fewer, on average */
     const bool solo = !QSM && brief && segs > gridDim.x;
     const uint32_t workers = solo ? gridDim.x * PK_WARPS : gridDim.x, me = solo ? blockIdx.x * PK_WARPS + w : blockIdx.x;
     uint32_t per = (total + workers - 1) / workers;
     /* Few segments: each is cut evenly among CTAs of its own, so that no CTA takes parts of two.  That makes
-     * slices longer by segs / (CTAs - segs); a second segment in a slice costs its CTA about 27 chunks' time
+     * slices longer by segs / (CTAs - segs); a second segment in a slice costs its CTA about 14 chunks' time
      * (q, the warps' meeting, the join: 5 us). */
-    const bool own = !solo && segs < workers && (uint64_t)per * segs < 27ull * (workers - segs);
-    /* a segment of up to 16 chunks is not cut to fill idle SMs: joining it costs more than reading it */
+    const bool own = !solo && segs < workers && (uint64_t)per * segs < 14ull * (workers - segs);
+    /* a segment of up to 8 chunks is not cut to fill idle SMs: joining it costs more than reading it */
     const uint32_t least = !brief ? J.least : B == 1 ? all : (all + B - 1) / B;
     if (own) per = (total + workers - segs - 1) / (workers - segs);
     if (!solo) per = per < least ? least : (per + PK_WARPS - 1) & ~(PK_WARPS - 1);
@@ -632,10 +633,11 @@ __global__ void __launch_bounds__(PK_WARPS * 32, pk_shape<CT, DP, R, QP>::OCC) p
     const uint32_t kbase = pk_saddr(ring);
 
     /* the page of each lane's key of prod's chunk is loaded a chunk ahead */
-    uint32_t page = 0, slot = 0;
-    bool real = false;
+    uint32_t page = 0, slot = 0, there = 0;
+    bool real = false, values = false;                    /* values: prod's chunk has its keys issued (SPLIT) */
+    uint64_t at_key = 0;                                  /* byte offset of the lane's key */
     auto fetch = [&]() {
-        const int32_t j = (prod.row.c0 + prod.pos) * CK + (int32_t)(lane % CK);
+        const int32_t j = (prod.row.c0 + prod.pos) * CK + (int32_t)lane;
         real = j >= prod.lo && j < prod.hi;
         if (real) {
             const uint32_t pi = J.page_shift >= 0 ? (uint32_t)j >> J.page_shift : (uint32_t)j / J.D.page_size;
@@ -645,54 +647,62 @@ __global__ void __launch_bounds__(PK_WARPS * 32, pk_shape<CT, DP, R, QP>::OCC) p
     };
     constexpr uint32_t RPI = 32 / S::UNITS;               /* keys per copy instruction of a warp */
     const uint32_t cu = lane % S::UNITS, cr = lane / S::UNITS; /* a lane's 16 bytes and first key in it */
-    const bool in_page = J.D.page_size % CK == 0;         /* a chunk is part of one page */
-    const uint64_t key_step = (uint64_t)RPI * J.D.tok_stride * S::ELT;
+    const bool runs = J.D.page_size % 16 == 0;            /* 16 aligned keys are in one page */
+    const uint64_t tok_bytes = J.D.tok_stride * S::ELT;
     const uint64_t k_to_v = (uint64_t)((const uint8_t *)J.D.v - (const uint8_t *)J.D.k);
     if (ahead < slice) fetch();
 
     auto issue = [&](uint32_t st) {
         if (ahead < slice) {
-            if (real && page >= J.D.n_pages) {
-                real = false;
-                atomicOr(J.err, PULSAR_KV_ERR_PAGE);
+            if (!S::SPLIT || !values) {
+                if (real && page >= J.D.n_pages) {
+                    real = false;
+                    atomicOr(J.err, PULSAR_KV_ERR_PAGE);
+                }
+                there = __ballot_sync(~0u, real);
+                if (lane == 0) vmask[w][st] = there;
+                at_key = real ? ((uint64_t)page * J.D.page_stride + prod.hk * J.D.head_stride) * S::ELT + slot * tok_bytes : 0;
             }
-            const uint32_t there = __ballot_sync(~0u, real);
-            if (lane == 0) vmask[w][st] = CK == 32 ? there : there & ((1u << (CK & 31)) - 1u);
-            const uint64_t off = (uint64_t)page * J.D.page_stride + prod.hk * J.D.head_stride;
+            const uint8_t *base = (const uint8_t *)J.D.k + cu * 16 + (S::SPLIT && values ? k_to_v : 0);
             const uint32_t dst = kbase + st * S::STAGE + cr * S::ROW;
-            if (there == ~0u && in_page) {
-                /* one page, every key: addresses go up by a constant */
-                if (cu < units) {
-                    const uint8_t *k = (const uint8_t *)J.D.k +
-                                       (off + (slot - lane % CK + cr) * J.D.tok_stride) * S::ELT + cu * 16;
+            if (there == ~0u && runs) {
+                /* every key: within 16 of them addresses go up by a constant */
 #pragma unroll
-                    for (uint32_t i = 0; i < CK / RPI; i++) {
-                        const uint32_t r = i * RPI + cr;
-                        const uint32_t d = dst + i * RPI * S::ROW + (S::ROW >= 128 ? cu ^ (r & 7u) : cu ^ ((r >> 1) & 3u)) * 16;
-                        pk_cp16(d, k, true);
-                        pk_cp16(d + CK * S::ROW, k + k_to_v, true);
-                        k += key_step;
+                for (uint32_t h = 0; h < CK; h += 16) {
+                    const uint32_t lo32 = __shfl_sync(~0u, (uint32_t)at_key, h), hi32 = __shfl_sync(~0u, (uint32_t)(at_key >> 32), h);
+                    if (cu < units) {
+                        const uint8_t *k = base + ((uint64_t)hi32 << 32 | lo32) + cr * tok_bytes;
+#pragma unroll
+                        for (uint32_t i = 0; i < 16 / RPI; i++) {
+                            const uint32_t r = h + i * RPI + cr;
+                            const uint32_t d = dst + (h + i * RPI) * S::ROW + (S::ROW >= 128 ? cu ^ (r & 7u) : cu ^ ((r >> 1) & 3u)) * 16;
+                            pk_cp16(d, k, true);
+                            if constexpr (!S::SPLIT) pk_cp16(d + CK * S::ROW, k + k_to_v, true);
+                            k += RPI * tok_bytes;
+                        }
                     }
                 }
             } else if (there) {
-                const uint64_t at = real ? (off + slot * J.D.tok_stride) * S::ELT : 0;
-                const uint32_t lo32 = (uint32_t)at, hi32 = (uint32_t)(at >> 32);
 #pragma unroll 1
                 for (uint32_t i = 0; i < CK / RPI; i++) {
                     const uint32_t r = i * RPI + cr;
-                    const uint64_t o = (uint64_t)__shfl_sync(~0u, hi32, r) << 32 | __shfl_sync(~0u, lo32, r);
+                    const uint32_t lo32 = __shfl_sync(~0u, (uint32_t)at_key, r), hi32 = __shfl_sync(~0u, (uint32_t)(at_key >> 32), r);
+                    const uint8_t *k = base + ((uint64_t)hi32 << 32 | lo32);
                     const uint32_t d = dst + i * RPI * S::ROW + (S::ROW >= 128 ? cu ^ (r & 7u) : cu ^ ((r >> 1) & 3u)) * 16;
                     const bool ok = there >> r & 1u;
                     if (cu < units) {
-                        pk_cp16(d, (const uint8_t *)J.D.k + o + cu * 16, ok);
-                        pk_cp16(d + CK * S::ROW, (const uint8_t *)J.D.v + o + cu * 16, ok);
+                        pk_cp16(d, k, ok);
+                        if constexpr (!S::SPLIT) pk_cp16(d + CK * S::ROW, k + k_to_v, ok);
                     }
                 }
             }
-            ahead += stride;
-            if (ahead < slice) {
-                prod.step(J, cached, (int32_t)stride);
-                fetch();
+            if (S::SPLIT) values = !values;
+            if (!values) {
+                ahead += stride;
+                if (ahead < slice) {
+                    prod.step(J, cached, (int32_t)stride);
+                    fetch();
+                }
             }
         }
         pk_cp_commit();
@@ -814,66 +824,68 @@ __global__ void __launch_bounds__(PK_WARPS * 32, pk_shape<CT, DP, R, QP>::OCC) p
 #pragma unroll
             for (int e = 0; e < 4; e++) o[t][e] = 0.0f;
 
+        /* the next stage, with the one after next issued behind it; *mask: which of its keys are there */
+        auto turn = [&](uint32_t *mask) {
+            pk_cp_wait<S::STAGES - 2>();
+            __syncwarp();
+            issue(stage == 0 ? S::STAGES - 1 : stage - 1);
+            const uint32_t at = kbase + stage * S::STAGE;
+            if (mask) *mask = vmask[w][stage];
+            stage = stage + 1 == S::STAGES ? 0 : stage + 1;
+            return at;
+        };
+
         /* ---- the warp's chunks of this segment */
         const uint32_t end = done + (uint32_t)(to - from);
 #pragma unroll 1
         for (; next < end; next += stride) {
-            pk_cp_wait<S::STAGES - 2>();
-            __syncwarp();
-            issue(stage == 0 ? S::STAGES - 1 : stage - 1);
-            const uint32_t there = vmask[w][stage];
-            const uint32_t ka = kbase + stage * S::STAGE;
-            stage = stage + 1 == S::STAGES ? 0 : stage + 1;
-            if (!there) continue;
+            uint32_t mask;
+            const uint32_t ka = turn(&mask);
+            if (!mask) {
+                if (S::SPLIT) turn(nullptr);
+                continue;
+            }
             /* the lane's ldmatrix rows; 16-byte unit u of row r sits at unit u ^ swizzle(r), the swizzle within
              * 128 aligned bytes, so that unit u + v (no carry) is an exclusive or away */
             auto unit_at = [](uint32_t x, int u) { return (x ^ ((u & 7) * 16)) + (u >> 3) * 128; };
-            const uint32_t kr = F8 ? (KT == 4 ? lane : lane & 15u) : (lane >> 4) * 8 + (lane & 7u);
-            const uint32_t ku = F8 ? (KT == 4 ? 0u : lane >> 4) : (lane >> 3) & 1u;
+            const uint32_t kr = F8 ? lane : (lane >> 4) * 8 + (lane & 7u), ku = F8 ? 0u : (lane >> 3) & 1u;
             const uint32_t kx = ka + kr * S::ROW + (S::ROW >= 128 ? ku ^ (kr & 7u) : ku ^ ((kr >> 1) & 3u)) * 16;
-            const uint32_t vr = lane & 15u, vu = lane >> 4;
-            const uint32_t vx = ka + CK * S::ROW + vr * S::ROW + (S::ROW >= 128 ? vu ^ (vr & 7u) : vu ^ ((vr >> 1) & 3u)) * 16;
             const int32_t key0 = (cons.row.c0 + from + (int32_t)(next - done)) * CK;
 
             /* scores: keys are the columns */
-            constexpr int CHAINS = KT == 2 ? 2 : 1; /* two columns of sums alone would wait on themselves */
-            float s[KT][4], rest[REST ? KT : 1][4], odd[CHAINS == 2 ? KT : 1][4];
+            float s[KT][4], rest[REST ? KT : 1][4];
 #pragma unroll
             for (int t = 0; t < KT; t++)
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
                     s[t][e] = 0.0f;
-                    if constexpr (CHAINS == 2) odd[t][e] = 0.0f;
                     if constexpr (REST) rest[t][e] = 0.0f;
                 }
-            auto score = [&](int t, int ks, const uint32_t *a, uint32_t b0, uint32_t b1) {
-                float *sum = CHAINS == 2 && (ks & 1) ? odd[CHAINS == 2 ? t : 0] : s[t];
+            auto score = [&](int t, const uint32_t *a, uint32_t b0, uint32_t b1) {
+                float *sum = s[t];
                 if constexpr (R == 1) pk_mma<BF>(sum, a[0], QP > 1 ? a[QW > 2 ? 2 : 0] : 0, a[1], QP > 1 ? a[QW > 2 ? 3 : 1] : 0, b0, b1);
                 else pk_mma<BF>(sum, a[0], a[1], a[2], a[3], b0, b1);
                 if constexpr (R == 1 && QP == 3) pk_mma<BF>(rest[REST ? t : 0], a[4], 0, a[5], 0, b0, b1);
                 if constexpr (R == 2 && QP > 1) pk_mma<BF>(rest[REST ? t : 0], a[4], a[5], a[6], a[7], b0, b1);
                 if constexpr (R == 2 && QP > 2) pk_mma<BF>(rest[REST ? t : 0], a[8], a[9], a[10], a[11], b0, b1);
             };
-            constexpr int KQ = F8 && KT == 2 ? 2 : 1; /* k-steps per load: 16-key e4m3 chunks take two */
 #pragma unroll
-            for (int ks = 0; ks < KS; ks += KQ) {
-                uint32_t a[KQ][QW], b[4];
-#pragma unroll
-                for (int q = 0; q < KQ; q++) q_words(ks + q, a[q]);
+            for (int ks = 0; ks < KS; ks++) {
+                uint32_t a[QW], b[4];
+                q_words(ks, a);
                 if constexpr (!F8) {
                     /* matrices (keys 0-7, d 0-7), (0-7, 8-15), (8-15, 0-7), (8-15, 8-15) */
 #pragma unroll
                     for (int t = 0; t < KT; t += 2) {
                         pk_ldm4(b, unit_at(kx, 2 * ks) + t * 8 * S::ROW);
-                        score(t, ks, a[0], b[0], b[1]);
-                        score(t + 1, ks, a[0], b[2], b[3]);
+                        score(t, a, b[0], b[1]);
+                        score(t + 1, a, b[2], b[3]);
                     }
                 } else {
-                    /* a matrix is 8 keys x 16 bytes: four groups of keys, or two groups and two k-steps */
+                    /* a matrix is 8 keys x 16 bytes */
                     pk_ldm4(b, unit_at(kx, ks));
 #pragma unroll
-                    for (int t = 0; t < 4; t++)
-                        score(t % KT, ks + t / KT, a[KQ == 2 ? t / KT : 0], pk_e4m3x2(b[t]), pk_e4m3x2(b[t] >> 16));
+                    for (int t = 0; t < KT; t++) score(t, a, pk_e4m3x2(b[t]), pk_e4m3x2(b[t] >> 16));
                 }
             }
 
@@ -886,28 +898,30 @@ __global__ void __launch_bounds__(PK_WARPS * 32, pk_shape<CT, DP, R, QP>::OCC) p
             bool moved = false;
 #pragma unroll
             for (int y = 0; y < R; y++) {
-                constexpr uint32_t ALL = CK == 32 ? ~0u : (1u << (CK & 31)) - 1u;
-                const bool whole = there == ALL && key0 >= slo[y] && key0 + CK <= shi[y];
-                top[y] = -INFINITY;
 #pragma unroll
                 for (int t = 0; t < KT; t++)
 #pragma unroll
                     for (int e = 0; e < 2; e++) {
                         float &x = s[t][2 * y + e];
-                        if constexpr (CHAINS == 2) x += odd[t][2 * y + e];
                         if constexpr (R == 1 && QP > 1) {
-                            float low = s[t][e + 2];
-                            if constexpr (CHAINS == 2) low += odd[t][e + 2];
+                            const float low = s[t][e + 2];
                             x = pk_fold(x, QP == 3 ? low + rest[REST ? t : 0][e] : low);
                         }
                         if constexpr (R == 2 && QP > 1) x = pk_fold(x, rest[REST ? t : 0][2 * y + e]);
                         x *= unit[y];
-                        if (!whole) {
-                            const int32_t k = t * 8 + 2 * (int32_t)c + e;
-                            if (!(there >> k & 1u) || key0 + k < slo[y] || key0 + k >= shi[y]) x = -INFINITY;
-                        }
-                        top[y] = fmaxf(top[y], x);
                     }
+                if (__builtin_expect(mask != ~0u || key0 < slo[y] || key0 + CK > shi[y], 0))
+#pragma unroll
+                    for (int t = 0; t < KT; t++)
+#pragma unroll
+                        for (int e = 0; e < 2; e++) {
+                            const int32_t k = t * 8 + 2 * (int32_t)c + e;
+                            if (!(mask >> k & 1u) || key0 + k < slo[y] || key0 + k >= shi[y]) s[t][2 * y + e] = -INFINITY;
+                        }
+                float half[KT];
+#pragma unroll
+                for (int t = 0; t < KT; t++) half[t] = fmaxf(s[t][2 * y], s[t][2 * y + 1]);
+                top[y] = fmaxf(fmaxf(half[0], half[1]), fmaxf(half[2], half[3]));
             }
 #pragma unroll
             for (int o2 = 1; o2 < 4; o2 <<= 1)
@@ -915,7 +929,7 @@ __global__ void __launch_bounds__(PK_WARPS * 32, pk_shape<CT, DP, R, QP>::OCC) p
                 for (int y = 0; y < R; y++) top[y] = fmaxf(top[y], __shfl_xor_sync(~0u, top[y], o2));
 #pragma unroll
             for (int y = 0; y < R; y++) moved |= top[y] > m[y] + SLACK;
-            if (__any_sync(~0u, moved)) {
+            if (__builtin_expect(__any_sync(~0u, moved), 0)) {
 #pragma unroll
                 for (int y = 0; y < R; y++) {
                     const float to = top[y] > m[y] + SLACK ? top[y] : m[y];
@@ -944,8 +958,9 @@ __global__ void __launch_bounds__(PK_WARPS * 32, pk_shape<CT, DP, R, QP>::OCC) p
                     for (int e = 0; e < 2; e++) {
                         float &x = s[t][2 * y + e];
                         x = pk_exp2(x - zero);
-                        l[y] += x;
                     }
+                l[y] += (s[0][2 * y] + s[0][2 * y + 1] + (s[1][2 * y] + s[1][2 * y + 1])) +
+                        (s[2][2 * y] + s[2][2 * y + 1] + (s[3][2 * y] + s[3][2 * y + 1]));
             }
 #pragma unroll
             for (int kt = 0; kt < KT / 2; kt++) {
@@ -970,39 +985,39 @@ __global__ void __launch_bounds__(PK_WARPS * 32, pk_shape<CT, DP, R, QP>::OCC) p
                         }
                 }
             }
-            /* output tiles t and t + 1; a part's products for all tiles before the next part's, which add to the same sums */
-            auto weigh = [&](int t, int kt, const uint32_t *b) {
-                constexpr int TIMES = R == 1 ? PP - 1 : PP;
+            const uint32_t vr = lane & 15u, vu = lane >> 4;
+            const uint32_t vx = (S::SPLIT ? turn(nullptr) : ka + CK * S::ROW) + vr * S::ROW +
+                                (S::ROW >= 128 ? vu ^ (vr & 7u) : vu ^ ((vr >> 1) & 3u)) * 16;
 #pragma unroll
-                for (int q = 0; q < TIMES; q++)
+            for (int kt = 0; kt < KT / 2; kt++)
 #pragma unroll
-                    for (int x = 0; x < 2; x++) {
-                        const uint32_t *a = pa[kt] + 4 * q;
-                        if (R == 1 && q == 1) pk_mma<BF>(o[t + x], a[0], 0, a[PW > 5 ? 1 : 0], 0, b[2 * x], b[2 * x + 1]);
-                        else pk_mma<BF>(o[t + x], a[0], a[1], a[2], a[3], b[2 * x], b[2 * x + 1]);
-                    }
-            };
-#pragma unroll
-            for (int kt = 0; kt < KT / 2; kt++) {
-                /* matrices (keys 0-7, unit u), (keys 8-15, u), (0-7, u + 1), (8-15, u + 1) */
-#pragma unroll
-                for (int u = 0; u < S::UNITS; u += 2) {
-                    uint32_t b[4];
-                    pk_ldm4t(b, unit_at(vx, u) + kt * 16 * S::ROW);
+                for (int t0 = 0; t0 < NT; t0 += 4) {
+                    /* four output tiles' right factors, from matrices (keys 0-7, unit u), (keys 8-15, u),
+                     * (0-7, u + 1), (8-15, u + 1) */
+                    uint32_t b[8];
                     if constexpr (!F8) {
-                        weigh(u, kt, b);
+                        pk_ldm4t(b, unit_at(vx, t0) + kt * 16 * S::ROW);
+                        pk_ldm4t(b + 4, unit_at(vx, t0 + 2) + kt * 16 * S::ROW);
                     } else {
                         /* a 16-bit column is two values: the even ones to tile 2u, the odd ones to 2u + 1 */
+                        uint32_t v[4];
+                        pk_ldm4t(v, unit_at(vx, t0 / 2) + kt * 16 * S::ROW);
 #pragma unroll
-                        for (int y = 0; y < 2; y++) {
-                            const uint32_t x0 = b[2 * y], x1 = b[2 * y + 1];
-                            const uint32_t z[4] = {pk_e4m3x2(__byte_perm(x0, 0, 0x0020)), pk_e4m3x2(__byte_perm(x1, 0, 0x0020)),
-                                                   pk_e4m3x2(__byte_perm(x0, 0, 0x0031)), pk_e4m3x2(__byte_perm(x1, 0, 0x0031))};
-                            weigh(2 * (u + y), kt, z);
+                        for (int x = 0; x < 4; x++) {
+                            b[4 * (x >> 1) + (x & 1)] = pk_e4m3x2(__byte_perm(v[x], 0, 0x0020));
+                            b[4 * (x >> 1) + 2 + (x & 1)] = pk_e4m3x2(__byte_perm(v[x], 0, 0x0031));
                         }
                     }
+                    /* a part's products for all tiles before the next part's, which add to the same sums */
+#pragma unroll
+                    for (int q = 0; q < (R == 1 ? PP - 1 : PP); q++)
+#pragma unroll
+                        for (int x = 0; x < 4; x++) {
+                            const uint32_t *a = pa[kt] + 4 * q;
+                            if (R == 1 && q == 1) pk_mma<BF>(o[t0 + x], a[0], 0, a[PW > 5 ? 1 : 0], 0, b[2 * x], b[2 * x + 1]);
+                            else pk_mma<BF>(o[t0 + x], a[0], a[1], a[2], a[3], b[2 * x], b[2 * x + 1]);
+                        }
                 }
-            }
         }
 
         /* ---- the segment's end */
