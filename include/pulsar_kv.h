@@ -92,8 +92,10 @@ int pulsar_kv_append(const pulsar_kv_desc *d, const pulsar_kv_append_args *a, vo
  * q, out: [n_rows * n_q] tokens of n_head heads of head_dim values of
  * q_type, q_stride / out_stride values apart.  n_head is a multiple of
  * n_kv; query head h reads key head h / (n_head / n_kv).  Keys beyond a
- * token's span have no influence, whatever their bytes are.
- * ws: pulsar_kv_attend_workspace bytes; its first PULSAR_KV_WS_ZEROED bytes
+ * token's span have no influence, whatever their bytes are; an infinite or
+ * NaN score or value that is seen gives what the formula gives, or NaN.
+ * ws: pulsar_kv_attend_workspace bytes (with a NULL: enough for any
+ * arguments over this cache), aligned to 16; its first PULSAR_KV_WS_ZEROED bytes
  * are zero before the first call and are zero again after every call.  One
  * ws serves any sequence of calls on one stream. */
 typedef struct pulsar_kv_attend_args {
@@ -155,7 +157,7 @@ int pulsar_kv_compact(const pulsar_kv_pool *p, int32_t *status, void *ws, size_t
 #define PULSAR_KV_MAX_FORK 4096u
 size_t pulsar_kv_pool_workspace(const pulsar_kv_pool *p, uint32_t n);
 
-/* reads and clears the family's error word on the current device (synchronous) */
+/* reads and clears the family's error word on the current device (waits for the device) */
 uint32_t pulsar_kv_error(void);
 
 #ifdef __cplusplus

@@ -134,11 +134,12 @@ _SIGS = {
     "pulsar_moe_layer_ws_view": [ctypes.POINTER(LayerDesc), _U32, _P, ctypes.POINTER(WsView)],
     "pulsar_quantize_rows": [_P, _P, _P, _U32, _U64, _U32, _P],
     "pulsar_repack_q2k_tiles": [_P, _P, _U32, _U32, _U32, _U64, _U64, _P],
-    "pulsar_kv_append": [ctypes.POINTER(KvDesc), ctypes.POINTER(KvAppendArgs), _P],
-    "pulsar_kv_attend": [ctypes.POINTER(KvDesc), ctypes.POINTER(KvAttendArgs), _P, ctypes.c_size_t, _P],
-    "pulsar_kv_grow": [ctypes.POINTER(KvPoolDesc), _P, _P, _U32, _P, _P, ctypes.c_size_t, _P],
-    "pulsar_kv_fork": [ctypes.POINTER(KvPoolDesc), _P, _P, _U32, _P, _P, ctypes.c_size_t, _P],
-    "pulsar_kv_compact": [ctypes.POINTER(KvPoolDesc), _P, _P, ctypes.c_size_t, _P],
+    # descriptors go by address: a ctypes pointer object costs a call more than an integer
+    "pulsar_kv_append": [_P, _P, _P],
+    "pulsar_kv_attend": [_P, _P, _P, ctypes.c_size_t, _P],
+    "pulsar_kv_grow": [_P, _P, _P, _U32, _P, _P, ctypes.c_size_t, _P],
+    "pulsar_kv_fork": [_P, _P, _P, _U32, _P, _P, ctypes.c_size_t, _P],
+    "pulsar_kv_compact": [_P, _P, _P, ctypes.c_size_t, _P],
 }
 
 
@@ -176,9 +177,9 @@ def lib() -> ctypes.CDLL:
         L.pulsar_row_bytes.restype = _U64
         L.pulsar_b200_abi_error.argtypes = []
         L.pulsar_b200_abi_error.restype = _U32
-        L.pulsar_kv_attend_workspace.argtypes = [ctypes.POINTER(KvDesc), ctypes.POINTER(KvAttendArgs)]
+        L.pulsar_kv_attend_workspace.argtypes = [_P, _P]
         L.pulsar_kv_attend_workspace.restype = ctypes.c_size_t
-        L.pulsar_kv_pool_workspace.argtypes = [ctypes.POINTER(KvPoolDesc), _U32]
+        L.pulsar_kv_pool_workspace.argtypes = [_P, _U32]
         L.pulsar_kv_pool_workspace.restype = ctypes.c_size_t
         L.pulsar_kv_error.argtypes = []
         L.pulsar_kv_error.restype = _U32

@@ -94,12 +94,17 @@ __global__ void __launch_bounds__(256, V == 8 && !NEAR && HU > 1 ? 3 : 4) /* 64 
                     if (second) r1[u] = *(const pk_vec<T, V> *)(from + u * D.head_dim + o1);
             }
         const uint32_t now = t;
-        const int32_t p = seq < 0 ? -1 : pos, row = seq;
+        int32_t p = seq < 0 ? -1 : pos;
+        const int32_t row = seq;
         const bool more = A.n_tok - t > step;
         t = more ? t + step : A.n_tok;
         if (more) {
             pos = __ldg(A.pos + t);
             seq = __ldg(A.seq + t);
+        }
+        if (p >= 0 && A.rot_dim && (uint32_t)p >= A.n_pos) { /* no angles: nothing of the token is written */
+            atomicOr(err, PULSAR_KV_ERR_SPAN);
+            p = -1;
         }
         if (p < 0) continue;
         uint64_t to;
@@ -120,10 +125,6 @@ __global__ void __launch_bounds__(256, V == 8 && !NEAR && HU > 1 ? 3 : 4) /* 64 
         }
         pk_vec<float, P> c, s;
         if (turn) {
-            if ((uint32_t)p >= A.n_pos) {
-                atomicOr(err, PULSAR_KV_ERR_SPAN);
-                continue;
-            }
             const float *cs = A.cos_sin + (uint64_t)p * A.rot_dim + angle;
             c = *(const pk_vec<float, P> *)cs;
             s = *(const pk_vec<float, P> *)(cs + half);

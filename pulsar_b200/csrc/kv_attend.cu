@@ -10,6 +10,21 @@ struct pk_attend_plan {
     size_t bytes;            /* of the workspace */
 };
 
+static uint32_t pk_attend_width(const pulsar_kv_desc *d) {
+    return d->head_dim <= 64 ? 64 : d->head_dim <= 128 ? 128 : 256;
+}
+
+/* CTAs that are resident together (pk_shape's OCC) */
+static uint32_t pk_attend_workers(uint32_t dp) {
+    const uint32_t n = pk_sm_count() * (dp == 256 ? 1 : 2);
+    return n < PK_MAX_WORKERS ? n : PK_MAX_WORKERS;
+}
+
+/* a worker has two parts of `heads` rows */
+static size_t pk_attend_bytes(uint32_t workers, uint32_t heads, uint32_t dp) {
+    return PULSAR_KV_WS_ZEROED + 4ull * workers * 2 * heads * (dp + 2);
+}
+
 static int pk_attend_prepare(const pulsar_kv_desc *d, const pulsar_kv_attend_args *a, pk_attend_job *J,
                              pk_attend_plan *p) {
     const char *f = pk_desc_fault(d);
@@ -25,7 +40,7 @@ static int pk_attend_prepare(const pulsar_kv_desc *d, const pulsar_kv_attend_arg
     J->A = *a;
     J->group = a->n_head / d->n_kv;
     J->rows = a->n_q * J->group;
-    p->dp = d->head_dim <= 64 ? 64 : d->head_dim <= 128 ? 128 : 256;
+    p->dp = (int)pk_attend_width(d);
     /* q in one part: the cache's own 16-bit type, or bf16 (8 bits) beside f16 and e4m3 */
     p->wide = a->q_type == PULSAR_TYPE_F32 || (d->dtype == PULSAR_TYPE_BF16 && a->q_type == PULSAR_TYPE_F16);
     /* a tile of 16 query rows, or of 8 where there are no more.  (32, with two
@@ -36,16 +51,12 @@ static int pk_attend_prepare(const pulsar_kv_desc *d, const pulsar_kv_attend_arg
     J->tiles = (J->rows + heads - 1) / heads;
     if ((uint64_t)J->tiles * d->n_kv > 0x7fffffffull) return pk_refuse("kv attend: too many heads and tokens");
     J->segs = J->tiles * d->n_kv;
-    J->page_shift = -1;
-    for (int s = 0; s < 31; s++)
-        if (d->page_size == 1u << s) J->page_shift = s;
+    J->page_shift = d->page_size & (d->page_size - 1) ? -1 : __builtin_ctz(d->page_size);
     const uint32_t qe = pk_type_bytes(a->q_type);
     J->pairs = (((uintptr_t)a->q | a->q_stride * qe) % (2 * qe)) == 0;
     const uint32_t ck = PK_CK;
     J->least = 128 / ck;
-    /* CTAs that are resident together (pk_shape's OCC) */
-    p->workers = pk_sm_count() * (p->dp == 256 ? 1 : 2);
-    if (p->workers > PK_MAX_WORKERS) p->workers = PK_MAX_WORKERS;
+    p->workers = pk_attend_workers(p->dp);
     /* no more CTAs than the longest rows could feed; no more rows in a launch
      * than a line of less than 2^32 chunks holds */
     uint64_t keys = (uint64_t)d->max_pages * d->page_size;
@@ -54,7 +65,7 @@ static int pk_attend_prepare(const pulsar_kv_desc *d, const pulsar_kv_attend_arg
     if (row > 0x7fffffffull) return pk_refuse("kv attend: a row too long for its heads");
     p->rows = 0xffffffffull / row < a->n_rows ? (uint32_t)(0xffffffffull / row) : a->n_rows;
     if (p->workers > row * p->rows) p->workers = (uint32_t)(row * p->rows);
-    p->bytes = PULSAR_KV_WS_ZEROED + 4ull * p->workers * 2 * heads * (p->dp + 2);
+    p->bytes = pk_attend_bytes(p->workers, heads, p->dp);
     return 1;
 }
 static_assert(4 * 2 * 2 * PK_MAX_WORKERS <= PULSAR_KV_WS_ZEROED, "the counters are in the zeroed bytes");
@@ -62,6 +73,11 @@ static_assert(4 * 2 * 2 * PK_MAX_WORKERS <= PULSAR_KV_WS_ZEROED, "the counters a
 extern "C" size_t pulsar_kv_attend_workspace(const pulsar_kv_desc *d, const pulsar_kv_attend_args *a) {
     pk_attend_job J;
     pk_attend_plan p;
+    if (!a) {
+        if (const char *f = pk_desc_fault(d)) return (size_t)pk_refuse(f);
+        const uint32_t dp = pk_attend_width(d);
+        return pk_attend_bytes(pk_attend_workers(dp), 16, dp);
+    }
     return pk_attend_prepare(d, a, &J, &p) ? p.bytes : 0;
 }
 

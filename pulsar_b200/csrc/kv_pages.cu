@@ -25,7 +25,8 @@ uint32_t *pk_err_word() {
 extern "C" uint32_t pulsar_kv_error(void) {
     uint32_t v = 0, zero = 0;
     uint32_t *w = pk_err_word();
-    if (!w || !pm_ok(cudaMemcpy(&v, w, 4, cudaMemcpyDeviceToHost), "kv error word") ||
+    /* the calls' streams need not be ones that a copy waits for */
+    if (!w || !pm_ok(cudaDeviceSynchronize(), "kv error word") || !pm_ok(cudaMemcpy(&v, w, 4, cudaMemcpyDeviceToHost), "kv error word") ||
         (v && !pm_ok(cudaMemcpy(w, &zero, 4, cudaMemcpyHostToDevice), "kv error word")))
         return 0xffffffffu;
     return v;

@@ -32,6 +32,10 @@ def kv_error() -> int:
     return int(lib().pulsar_kv_error())
 
 
+_device = torch._C._cuda_getDevice
+_raw_stream = torch._C._cuda_getCurrentRawStream  # current_stream() builds an object: 3 us a call
+
+
 def _need(ok: bool, what: str) -> None:
     if not ok:
         raise ValueError(what)
@@ -39,9 +43,11 @@ def _need(ok: bool, what: str) -> None:
 
 def _stream(stream, dev):
     """the cudaStream_t to launch on: dev is the buffers' device index"""
-    if stream is None:
-        return torch._C._cuda_getCurrentRawStream(dev)  # current_stream() builds an object: 3 us a call
-    return stream.cuda_stream
+    if _device() != dev:
+        raise ValueError("the buffers' device is not the current one")
+    # torch's default stream goes by the runtime's handle for it (1): 0 would be the calling thread's own,
+    # which is ordered with it, but by an event each way
+    return (_raw_stream(dev) if stream is None else stream.cuda_stream) or 1
 
 
 def _i32(t, n, dev, what):
@@ -77,17 +83,17 @@ def _tokens(t, n, n_q, n_head, d):
 def rope_table(n_pos: int, rot_dim: int, base: float = 10000.0, scaling: dict | None = None,
                device="cuda") -> torch.Tensor:
     """f32 [n_pos][2][rot_dim / 2]: cosines and sines of p * f_i, f_i =
-    base^(-2 i / rot_dim), computed in 64 bits.  scaling, for contexts
-    beyond the trained one (all with "factor" s):
+    base^(-2 i / rot_dim), computed in 64 bits.  scaling, for contexts s =
+    "factor" times the trained one:
       kind "linear": f_i / s
-      kind "ntk":    base * s^(rot_dim / (rot_dim - 2))
-      kind "yarn":   between f_i (fast pairs) and f_i / s (slow ones): with
-        r_i = trained * f_i / (2 pi) turns over the trained context
-        ("trained"), the share of f_i is (r_i's pair index ramp) between the
-        pairs that turn "fast" (32) and "slow" (1) times, and cosines and
-        sines are times 1 + 0.1 ln s ("mscale" overrides)
-      kind "bands":  f_i where the wavelength is below trained / "high" (4),
-        f_i / s above trained / "low" (1), a linear blend in turns between
+      kind "ntk":    base * s^(rot_dim / (rot_dim - 2)) in place of base
+      kind "yarn":   f_i up to the pair that turns "fast" (32) times over the
+        trained context ("trained"), f_i / s from the one that turns "slow"
+        (1) times, a linear ramp over the pairs between; cosines and sines
+        are times "mscale" (1 + 0.1 ln s)
+      kind "bands":  f_i for pairs that turn "high" (4) times or more over the
+        trained context, f_i / s for "low" (1) times or fewer, a blend linear
+        in the turns between
     """
     _need(rot_dim >= 2 and rot_dim % 2 == 0 and n_pos >= 1, "rope_table: an even rot_dim and at least one position")
     half = rot_dim // 2
@@ -130,16 +136,19 @@ class PagedKv:
     """One layer's cache: k, v [n_pages][n_kv][page_size][head_dim] (any
     strides whose head rows are contiguous and 16-byte aligned), bf16, f16 or
     float8_e4m3fn; table int32 [n_rows][max_pages].  k_scale, v_scale: f32
-    [n_kv], e4m3 only."""
+    [n_kv], e4m3 only.  ws: attend's workspace (workspace()), which any number
+    of layers share on one stream; without one the first attend() makes one.
+    An object serves one thread, and its workspace one stream, at a time."""
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, k_scale: torch.Tensor | None = None,
-                 v_scale: torch.Tensor | None = None):
+                 v_scale: torch.Tensor | None = None, ws: torch.Tensor | None = None):
         _need(k.is_cuda and k.dim() == 4 and k.shape == v.shape and k.stride() == v.stride() and k.dtype == v.dtype
               and v.device == k.device, "PagedKv: k and v alike, [n_pages][n_kv][page_size][head_dim] on one GPU")
         _need(k.dtype in TYPES and k.dtype != torch.float32, "PagedKv: caches are bf16, f16 or float8_e4m3fn")
         _need(k.stride(3) == 1, "PagedKv: a head's values are contiguous")
         _need(table.dim() == 2 and table.dtype == torch.int32 and table.device == k.device and table.stride(1) == 1,
               "PagedKv: table is int32 [n_rows][max_pages] beside the cache")
+        _need(table.shape[0] == 1 or table.stride(0) >= table.shape[1], "PagedKv: table rows overlap")
         for s in (k_scale, v_scale):
             _need(s is None or (s.dtype == torch.float32 and s.device == k.device and s.is_contiguous()
                                 and s.numel() == k.shape[1]), "PagedKv: scales are f32 [n_kv] beside the cache")
@@ -154,11 +163,14 @@ class PagedKv:
         d.n_pages, d.n_kv, d.page_size, d.head_dim = k.shape
         d.n_rows, d.max_pages = table.shape
         d.dtype = TYPES[k.dtype]
-        self._desc, self._pdesc = d, ctypes.pointer(d)
+        self._desc, self._pdesc = d, ctypes.addressof(d)
         self._args, self._append = KvAttendArgs(), KvAppendArgs()
-        self._pargs, self._pappend = ctypes.pointer(self._args), ctypes.pointer(self._append)
-        self._ws, self._sized = None, None
+        self._pargs, self._pappend = ctypes.addressof(self._args), ctypes.addressof(self._append)
+        self._ws = None
+        if ws is not None:
+            self._take(ws)
         self._lib = lib()
+        self._c_append, self._c_attend = self._lib.pulsar_kv_append, self._lib.pulsar_kv_attend
 
     def append(self, q, k, v, seq, pos, cos_sin, q_out, interleaved: bool = False, stream=None):
         """Turn q [T][n_head][D] into q_out and write turned k and v [T][n_kv][D]
@@ -187,7 +199,8 @@ class PagedKv:
                 raise ValueError("append: cos_sin is f32 [n_pos][2][rot_dim / 2]")
             a.cos_sin, a.n_pos, a.rot_dim = cos_sin.data_ptr(), cos_sin.shape[0], 2 * cos_sin.shape[2]
         a.n_tok, a.x_type, a.interleaved = n_tok, TYPES[k.dtype], int(interleaved)
-        check(self._lib.pulsar_kv_append(self._pdesc, self._pappend, _stream(stream, self._index)), "kv_append")
+        if not self._c_append(self._pdesc, self._pappend, _stream(stream, self._index)):
+            raise KernelError("kv_append")
         return q_out
 
     def attend(self, q, lens, out, scale: float | None = None, window: int = 0, sinks=None, lse=None, seq=None,
@@ -197,8 +210,8 @@ class PagedKv:
         new ones among them) in table row seq[b] (None: b).  Token i of n_q
         sees lens[b] - (n_q - 1 - i) keys, the last `window` of them if that is
         not 0.  sinks f32 [n_head]; lse f32 [B][n_q][n_head].  scale: D^-1/2
-        unless given.  ws: a zeroed workspace (workspace()); without one the
-        object keeps its own, which serves one stream at a time."""
+        unless given.  ws: another workspace than the object's, zeroed before
+        its first use (workspace())."""
         a, dev, D = self._args, self.device, self.head_dim
         shape, dtype = q.shape, q.dtype
         kind = TYPES.get(dtype, 3)
@@ -227,22 +240,26 @@ class PagedKv:
             raise ValueError("attend: window is 0 (none) or a number of keys")
         a.scale = D ** -0.5 if scale is None else scale
         a.n_rows, a.n_q, a.n_head, a.window, a.q_type = n, n_q, n_head, window, kind
-        if ws is None:
-            size = (n, n_q, n_head, kind, window)
-            if self._sized != size:
-                need = self.workspace_bytes()
-                if self._ws is None or self._ws.numel() < need:
-                    self._ws = torch.zeros(need, dtype=torch.uint8, device=dev)
-                self._sized, self._where = size, (self._ws.data_ptr(), self._ws.numel())
-            where = self._where
-        else:
+        if ws is not None:
             where = ws.data_ptr(), ws.numel()
-        check(self._lib.pulsar_kv_attend(self._pdesc, self._pargs, *where, _stream(stream, self._index)), "kv_attend")
+        else:
+            if self._ws is None:
+                self._take(self.workspace())
+            where = self._where
+        if not self._c_attend(self._pdesc, self._pargs, *where, _stream(stream, self._index)):
+            raise KernelError("kv_attend")
         return out
 
-    def workspace_bytes(self) -> int:
-        """bytes that the last attend() call's arguments need"""
-        return int(self._lib.pulsar_kv_attend_workspace(self._pdesc, self._pargs))
+    def workspace(self) -> torch.Tensor:
+        """a zeroed workspace for attend() over caches of this shape, whatever its arguments (about 5 MB)"""
+        n = int(self._lib.pulsar_kv_attend_workspace(self._pdesc, None))
+        _need(n > 0, "PagedKv: shape refused")
+        return torch.zeros(n, dtype=torch.uint8, device=self.device)
+
+    def _take(self, ws: torch.Tensor) -> None:
+        _need(ws.dtype == torch.uint8 and ws.device == self.device and ws.is_contiguous(),
+              "PagedKv: a workspace is contiguous bytes beside the cache")
+        self._ws, self._where = ws, (ws.data_ptr(), ws.numel())
 
 
 # ------------------------------------------------------------------ all layers
@@ -269,12 +286,13 @@ class KvPool:
         p.table_stride = table.shape[1]
         p.n_rows, p.max_pages = table.shape
         p.n_pages, p.page_size, p.n_slab = data.shape[2], data.shape[4], 2 * data.shape[0]
-        self._desc, self._p = p, ctypes.pointer(p)
+        self._desc, self._p = p, ctypes.addressof(p)
         self._lib = lib()
         need = int(self._lib.pulsar_kv_pool_workspace(self._p, n_rows))
         _need(need > 0, "KvPool: shape refused")
         self._ws = torch.empty(need, dtype=torch.uint8, device=self.device)
         self._where = self._ws.data_ptr(), need
+        self._attend_ws = None
         #: what the last grow, fork and compact did (pulsar_kv.h's status words)
         self.status = torch.zeros((3, 4), dtype=torch.int32, device=self.device)
         self._status = [self.status[i].data_ptr() for i in range(3)]
@@ -287,7 +305,12 @@ class KvPool:
                    torch.zeros(n_pages, **i32))
 
     def layer(self, i: int, k_scale=None, v_scale=None) -> PagedKv:
-        return PagedKv(self.data[i, 0], self.data[i, 1], self.table, k_scale, v_scale)
+        """layer i's cache; the layers share one attend workspace"""
+        kv = PagedKv(self.data[i, 0], self.data[i, 1], self.table, k_scale, v_scale, self._attend_ws)
+        if self._attend_ws is None:
+            self._attend_ws = kv.workspace()
+            kv._take(self._attend_ws)
+        return kv
 
     def grow(self, n_new: torch.Tensor, rows: torch.Tensor | None = None, stream=None) -> None:
         """rows[i] (None: i) gets n_new[i] more tokens and the pages for them"""

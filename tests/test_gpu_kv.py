@@ -102,6 +102,15 @@ CASES = [
     ([40] * 70, 1, 4, 2, 32, 16, 0, False, BF16, F16),
     ([130, 131], 64, 4, 1, 64, 16, 0, False, F32, F16),
     ([30] * 3 + [1] * 9 + [2500], 1, 64, 8, 64, 16, 128, True, BF16, BF16),
+    # the workers' three ways of sharing a call: whole short segments a warp, segments cut among CTAs, equal slices;
+    # batches beyond what a CTA keeps of the lengths
+    ([20 + 3 * i % 90 for i in range(200)], 1, 24, 2, 64, 16, 0, False, BF16, F16),
+    ([1 + 7 * i % 40 for i in range(300)], 1, 2, 1, 128, 16, 0, True, F32, F16),
+    ([i % 5 for i in range(5000)], 1, 1, 1, 16, 4, 0, False, BF16, BF16),
+    ([250 + 61 * i % 2250 for i in range(40)], 1, 8, 8, 64, 16, 0, False, F16, F16),
+    ([250 + 61 * i % 2250 for i in range(40)], 1, 80, 8, 128, 32, 0, False, BF16, BF16),
+    ([900 + 331 * i % 2000 for i in range(30)], 2, 10, 10, 256, 16, 700, False, F32, E4M3),
+    ([100000], 1, 2, 1, 128, 64, 0, False, F32, BF16),
 ]
 
 
@@ -199,6 +208,23 @@ def test_attend_past_32_bits(kv):
     kv.PagedKv(k, v, table[:, :].flip(1).contiguous()).append(None, x, x, torch.zeros_like(pos), pos, None, None)
     got = k[n_pages - 1, :, :3].float()
     assert (got - x.transpose(0, 1)).abs().max() <= 2.0 ** -4 * x.abs().max()
+
+
+@pytest.mark.parametrize("rows", [None, [3, 0, 3, 9, 1, 2, 3, 4, 5, 9, 7, 8, 0]])
+def test_attend_in_several_launches(kv, rows):
+    """rows so long (by the table's width) that the call takes a few of them at a time"""
+    D, page, n_kv, n = 16, 1 << 20, 8, 10
+    gen = torch.Generator(device="cuda").manual_seed(12)
+    k, v = (values((3, n_kv, page, D), F32, gen).to(E4M3) for _ in range(2))
+    table = torch.full((n, 2047), -1, dtype=torch.int32, device="cuda")
+    table[:, 0] = torch.arange(n, device="cuda", dtype=torch.int32) % 3
+    lens = [40 + 9 * i for i in range(n if rows is None else len(rows))]
+    q = values((len(lens), 1, n_kv, D), BF16, gen)
+    out, lse = torch.zeros_like(q), torch.zeros((len(lens), 1, n_kv), device="cuda")
+    seq = None if rows is None else torch.tensor(rows, dtype=torch.int32, device="cuda")
+    kv.PagedKv(k, v, table).attend(q, torch.tensor(lens, dtype=torch.int32, device="cuda"), out, lse=lse, seq=seq)
+    small = torch.stack([t[:, :, :200].contiguous() for t in (k, v)])
+    held(out, lse, kv_ref.attend(q, small[0], small[1], table[:, :1], lens, seq=rows), BF16, E4M3, 200, D)
 
 
 def test_attend_streams_and_graph(kv):
@@ -341,8 +367,10 @@ def test_append_in_place_strided_and_told(kv):
     assert kv.kv_error() == kv.ERR_ROW
     c.append(q[:1], k[:1], v[:1], one, one, kv.rope_table(1, D), q[:1].clone())
     assert kv.kv_error() == 0
+    kept = ck.clone(), cv.clone()
     c.append(q[:1], k[:1], v[:1], one, one + 1, kv.rope_table(1, D), q[:1].clone())  # past the angles
     assert kv.kv_error() == kv.ERR_SPAN
+    assert torch.equal(ck, kept[0]) and torch.equal(cv, kept[1])
     table[0, 0] = 4
     c.append(None, k[:1], v[:1], one, one, None, None)
     assert kv.kv_error() == kv.ERR_PAGE

@@ -100,6 +100,10 @@ def test_refusals_before_any_launch(L):
     need = L.pulsar_kv_attend_workspace(ref(desc()), ref(attend_args()))
     assert need >= 32768
     assert L.pulsar_kv_attend(ref(desc()), ref(attend_args()), 4096, need - 1, None) == 0
+    assert L.pulsar_kv_attend(ref(desc()), ref(attend_args()), 4104, big, None) == 0
+    # enough for any arguments: the widest tiles of as many workers
+    for kw in (dict(), dict(n_head=64, q_stride=64 * 64, out_stride=64 * 64), dict(n_q=9, q_type=0), dict(window=3)):
+        assert L.pulsar_kv_attend_workspace(ref(desc()), None) >= L.pulsar_kv_attend_workspace(ref(desc()), ref(attend_args(**kw)))
 
 
 def test_pool_refusals_before_any_launch(L):
