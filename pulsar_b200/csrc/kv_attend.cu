@@ -11,12 +11,15 @@ struct pk_attend_plan {
 };
 
 static uint32_t pk_attend_width(const pulsar_kv_desc *d) {
-    return d->head_dim <= 64 ? 64 : d->head_dim <= 128 ? 128 : 256;
+    return d->head_dim <= 64    ? 64
+           : d->head_dim <= 128 ? 128
+           : d->head_dim <= 192 && d->dtype != PULSAR_TYPE_E4M3 ? 192 : 256;
 }
 
-/* CTAs that are resident together (pk_shape's OCC) */
-static uint32_t pk_attend_workers(uint32_t dp) {
-    const uint32_t n = pk_sm_count() * (dp == 256 ? 1 : 2);
+/* two CTAs an SM (pk_shape's OCC; one where q's parts at 256 columns leave no
+ * room for two) */
+static uint32_t pk_attend_workers() {
+    const uint32_t n = pk_sm_count() * 2;
     return n < PK_MAX_WORKERS ? n : PK_MAX_WORKERS;
 }
 
@@ -54,9 +57,9 @@ static int pk_attend_prepare(const pulsar_kv_desc *d, const pulsar_kv_attend_arg
     J->page_shift = d->page_size & (d->page_size - 1) ? -1 : __builtin_ctz(d->page_size);
     const uint32_t qe = pk_type_bytes(a->q_type);
     J->pairs = (((uintptr_t)a->q | a->q_stride * qe) % (2 * qe)) == 0;
-    const uint32_t ck = PK_CK;
+    const uint32_t ck = PK_CK(p->dp * pk_type_bytes(d->dtype));
     J->least = 128 / ck;
-    p->workers = pk_attend_workers(p->dp);
+    p->workers = pk_attend_workers();
     /* no more CTAs than the longest rows could feed; no more rows in a launch
      * than a line of less than 2^32 chunks holds */
     uint64_t keys = (uint64_t)d->max_pages * d->page_size;
@@ -76,7 +79,7 @@ extern "C" size_t pulsar_kv_attend_workspace(const pulsar_kv_desc *d, const puls
     if (!a) {
         if (const char *f = pk_desc_fault(d)) return (size_t)pk_refuse(f);
         const uint32_t dp = pk_attend_width(d);
-        return pk_attend_bytes(pk_attend_workers(dp), 16, dp);
+        return pk_attend_bytes(pk_attend_workers(), 16, dp);
     }
     return pk_attend_prepare(d, a, &J, &p) ? p.bytes : 0;
 }

@@ -37,8 +37,10 @@
 #pragma once
 #include "pk_common.h"
 
-#define PK_WARPS 4u
-#define PK_CK 32              /* keys per chunk: a lane each */
+#define PK_WARPS 4
+/* keys per chunk, by the bytes of a row in shared memory: 32 while their keys fit 8 KB */
+#define PK_CK(row_bytes) ((row_bytes) > 256 ? 16 : 32)
+#define PK_SM_BYTES (228 * 1024) /* shared memory of an SM; each CTA takes 1 KB more than it asks for */
 #define PK_GROUP 32u          /* parts joined at a time */
 #define PK_MAX_WORKERS 1024u  /* 2 x 2 counters of each fill PULSAR_KV_WS_ZEROED / 2 */
 #define PK_LOG2E 1.4426950408889634f
@@ -64,19 +66,19 @@ struct pk_shape {
     static constexpr int ELT = CT == PULSAR_TYPE_E4M3 ? 1 : 2;
     static constexpr int ROW = DP * ELT;                  /* bytes of a key in shared memory */
     static constexpr int UNITS = ROW / 16;
+    static constexpr int CK = PK_CK(ROW);
     /* A stage of the ring is a chunk's keys and values; at rows of 256 bytes or more its keys or its values,
-     * which take turns: stages stay at 4 to 16 KB, and a chunk, whose bookkeeping and softmax cost the same
-     * for any number of keys, stays at PK_CK. */
+     * which take turns: stages stay at 4 to 8 KB. */
     static constexpr bool SPLIT = ROW >= 256;
     static constexpr int STAGES = 3;
-    static constexpr int OCC = DP > 128 ? 1 : 2;          /* CTAs that an SM holds */
-    static constexpr int STAGE = (SPLIT ? 1 : 2) * PK_CK * ROW;
+    static constexpr int STAGE = (SPLIT ? 1 : 2) * CK * ROW;
     static constexpr int RING = STAGES * STAGE;           /* per warp */
     static constexpr bool QSM = DP > 128;                 /* q's parts wait in shared memory, not registers */
     static constexpr int QW = R == 1 ? 2 * QP : 4 * QP;   /* their words per lane and k-step */
     static constexpr int XROW = 64 + 4;                   /* floats of 64 columns in the warps' meeting; no bank conflicts */
     static constexpr int MEET = PK_WARPS * 8 * XROW * 4, QALL = QSM ? DP / 16 * QW * 128 : 0;
     static constexpr int SIDE = MEET > QALL ? MEET : QALL; /* bytes beside the rings: both, at different times */
+    static constexpr int OCC = 2 * (PK_WARPS * RING + SIDE + 4096) <= PK_SM_BYTES ? 2 : 1; /* CTAs that an SM holds */
 };
 
 __device__ __forceinline__ uint32_t pk_saddr(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -522,7 +524,7 @@ __global__ void __launch_bounds__(PK_WARPS * 32, pk_shape<CT, DP, R, QP>::OCC) p
     typedef pk_shape<CT, DP, R, QP> S;
     constexpr bool BF = CT == PULSAR_TYPE_BF16;
     constexpr bool F8 = CT == PULSAR_TYPE_E4M3;
-    constexpr int CK = PK_CK, KS = DP / 16, NT = DP / 8, KT = CK / 8;
+    constexpr int CK = S::CK, KS = DP / 16, NT = DP / 8, KT = CK / 8;
     constexpr int HEADS = 8 * R;                          /* query rows of a tile; a lane's are R */
     constexpr bool QSM = S::QSM;
     constexpr int QW = S::QW;
@@ -637,7 +639,7 @@ __global__ void __launch_bounds__(PK_WARPS * 32, pk_shape<CT, DP, R, QP>::OCC) p
     bool real = false, values = false;                    /* values: prod's chunk has its keys issued (SPLIT) */
     uint64_t at_key = 0;                                  /* byte offset of the lane's key */
     auto fetch = [&]() {
-        const int32_t j = (prod.row.c0 + prod.pos) * CK + (int32_t)lane;
+        const int32_t j = (prod.row.c0 + prod.pos) * CK + (int32_t)(lane % CK);
         real = j >= prod.lo && j < prod.hi;
         if (real) {
             const uint32_t pi = J.page_shift >= 0 ? (uint32_t)j >> J.page_shift : (uint32_t)j / J.D.page_size;
@@ -647,7 +649,8 @@ __global__ void __launch_bounds__(PK_WARPS * 32, pk_shape<CT, DP, R, QP>::OCC) p
     };
     constexpr uint32_t RPI = 32 / S::UNITS;               /* keys per copy instruction of a warp */
     const uint32_t cu = lane % S::UNITS, cr = lane / S::UNITS; /* a lane's 16 bytes and first key in it */
-    const bool runs = J.D.page_size % 16 == 0;            /* 16 aligned keys are in one page */
+    const bool runs = J.D.page_size % 8 == 0;             /* 8 aligned keys are in one page */
+    const bool copies = cr < RPI && cu < units;
     const uint64_t tok_bytes = J.D.tok_stride * S::ELT;
     const uint64_t k_to_v = (uint64_t)((const uint8_t *)J.D.v - (const uint8_t *)J.D.k);
     if (ahead < slice) fetch();
@@ -666,14 +669,14 @@ __global__ void __launch_bounds__(PK_WARPS * 32, pk_shape<CT, DP, R, QP>::OCC) p
             const uint8_t *base = (const uint8_t *)J.D.k + cu * 16 + (S::SPLIT && values ? k_to_v : 0);
             const uint32_t dst = kbase + st * S::STAGE + cr * S::ROW;
             if (there == ~0u && runs) {
-                /* every key: within 16 of them addresses go up by a constant */
+                /* every key: within 8 of them addresses go up by a constant */
 #pragma unroll
-                for (uint32_t h = 0; h < CK; h += 16) {
+                for (uint32_t h = 0; h < CK; h += 8) {
                     const uint32_t lo32 = __shfl_sync(~0u, (uint32_t)at_key, h), hi32 = __shfl_sync(~0u, (uint32_t)(at_key >> 32), h);
-                    if (cu < units) {
+                    if (copies) {
                         const uint8_t *k = base + ((uint64_t)hi32 << 32 | lo32) + cr * tok_bytes;
 #pragma unroll
-                        for (uint32_t i = 0; i < 16 / RPI; i++) {
+                        for (uint32_t i = 0; i < 8 / RPI; i++) {
                             const uint32_t r = h + i * RPI + cr;
                             const uint32_t d = dst + (h + i * RPI) * S::ROW + (S::ROW >= 128 ? cu ^ (r & 7u) : cu ^ ((r >> 1) & 3u)) * 16;
                             pk_cp16(d, k, true);
@@ -683,14 +686,14 @@ __global__ void __launch_bounds__(PK_WARPS * 32, pk_shape<CT, DP, R, QP>::OCC) p
                     }
                 }
             } else if (there) {
-#pragma unroll 1
+#pragma unroll 4
                 for (uint32_t i = 0; i < CK / RPI; i++) {
-                    const uint32_t r = i * RPI + cr;
+                    const uint32_t r = i * RPI + (cr < RPI ? cr : 0);
                     const uint32_t lo32 = __shfl_sync(~0u, (uint32_t)at_key, r), hi32 = __shfl_sync(~0u, (uint32_t)(at_key >> 32), r);
                     const uint8_t *k = base + ((uint64_t)hi32 << 32 | lo32);
                     const uint32_t d = dst + i * RPI * S::ROW + (S::ROW >= 128 ? cu ^ (r & 7u) : cu ^ ((r >> 1) & 3u)) * 16;
                     const bool ok = there >> r & 1u;
-                    if (cu < units) {
+                    if (copies) {
                         pk_cp16(d, k, ok);
                         if constexpr (!S::SPLIT) pk_cp16(d + CK * S::ROW, k + k_to_v, ok);
                     }
@@ -921,7 +924,7 @@ __global__ void __launch_bounds__(PK_WARPS * 32, pk_shape<CT, DP, R, QP>::OCC) p
                 float half[KT];
 #pragma unroll
                 for (int t = 0; t < KT; t++) half[t] = fmaxf(s[t][2 * y], s[t][2 * y + 1]);
-                top[y] = fmaxf(fmaxf(half[0], half[1]), fmaxf(half[2], half[3]));
+                top[y] = fmaxf(fmaxf(half[0], half[1]), fmaxf(half[KT - 2], half[KT - 1]));
             }
 #pragma unroll
             for (int o2 = 1; o2 < 4; o2 <<= 1)
@@ -959,8 +962,9 @@ __global__ void __launch_bounds__(PK_WARPS * 32, pk_shape<CT, DP, R, QP>::OCC) p
                         float &x = s[t][2 * y + e];
                         x = pk_exp2(x - zero);
                     }
-                l[y] += (s[0][2 * y] + s[0][2 * y + 1] + (s[1][2 * y] + s[1][2 * y + 1])) +
-                        (s[2][2 * y] + s[2][2 * y + 1] + (s[3][2 * y] + s[3][2 * y + 1]));
+#pragma unroll
+                for (int t = 0; t < KT; t += 2)
+                    l[y] += s[t][2 * y] + s[t][2 * y + 1] + (s[t + 1][2 * y] + s[t + 1][2 * y + 1]);
             }
 #pragma unroll
             for (int kt = 0; kt < KT / 2; kt++) {
@@ -1164,7 +1168,8 @@ static int pk_attend_launch(const pk_attend_job &J, uint32_t grid, cudaStream_t 
     constexpr uint32_t smem = PK_WARPS * S::RING + S::SIDE;
     auto kernel = pk_attend_kernel<CT, DP, R, QP>;
     if (!pm_smem_attr(kernel, smem, &done)) return 0;
-    kernel<<<grid, PK_WARPS * 32, smem, st>>>(J);
+    const uint32_t most = S::OCC * pk_sm_count(); /* one wave */
+    kernel<<<grid < most ? grid : most, PK_WARPS * 32, smem, st>>>(J);
     return pm_ok(cudaGetLastError(), "kv attend launch");
 }
 
@@ -1186,5 +1191,7 @@ template <uint32_t CT>
 static pk_attend_fn pk_attend_pick(int dp, int r, bool wide) {
     if (dp == 64) return pk_attend_pick_at<CT, 64>(r, wide);
     if (dp == 128) return pk_attend_pick_at<CT, 128>(r, wide);
+    if constexpr (CT != PULSAR_TYPE_E4M3) /* rows of 192 bytes would break the swizzle's 128 */
+        if (dp == 192) return pk_attend_pick_at<CT, 192>(r, wide);
     return pk_attend_pick_at<CT, 256>(r, wide);
 }

@@ -111,6 +111,12 @@ CASES = [
     ([250 + 61 * i % 2250 for i in range(40)], 1, 80, 8, 128, 32, 0, False, BF16, BF16),
     ([900 + 331 * i % 2000 for i in range(30)], 2, 10, 10, 256, 16, 700, False, F32, E4M3),
     ([100000], 1, 2, 1, 128, 64, 0, False, F32, BF16),
+    # heads of 129 to 192, pages of multiples of 8 and of none
+    ([700, 33, 2041], 2, 12, 2, 192, 24, 0, False, F32, BF16),
+    ([190, 65, 16, 15], 1, 3, 3, 176, 8, 50, True, F16, F16),
+    ([500, 77, 31], 1, 20, 2, 256, 10, 0, False, BF16, BF16),
+    ([900, 9], 1, 5, 1, 144, 3, 0, True, F32, F16),
+    ([1200, 640], 3, 16, 2, 64, 8, 0, False, F32, E4M3),
 ]
 
 
