@@ -12,6 +12,7 @@ struct pk_attend_plan {
 
 static uint32_t pk_attend_width(const pulsar_kv_desc *d) {
     return d->head_dim <= 64    ? 64
+           : d->head_dim <= 96  ? 96
            : d->head_dim <= 128 ? 128
            : d->head_dim <= 192 && d->dtype != PULSAR_TYPE_E4M3 ? 192 : 256;
 }
@@ -57,14 +58,14 @@ static int pk_attend_prepare(const pulsar_kv_desc *d, const pulsar_kv_attend_arg
     J->page_shift = d->page_size & (d->page_size - 1) ? -1 : __builtin_ctz(d->page_size);
     const uint32_t qe = pk_type_bytes(a->q_type);
     J->pairs = (((uintptr_t)a->q | a->q_stride * qe) % (2 * qe)) == 0;
-    const uint32_t ck = PK_CK(p->dp * pk_type_bytes(d->dtype));
+    const uint32_t ck = PK_CK((p->dp == 96 ? 128 : p->dp) * pk_type_bytes(d->dtype));
     J->least = 128 / ck;
     p->workers = pk_attend_workers();
     /* no more CTAs than the longest rows could feed; no more rows in a launch
      * than a line of less than 2^32 chunks holds */
     uint64_t keys = (uint64_t)d->max_pages * d->page_size;
     if (a->window && keys > (uint64_t)a->window + a->n_q - 1) keys = (uint64_t)a->window + a->n_q - 1;
-    const uint64_t row = (uint64_t)J->segs * (keys / ck + 2);
+    const uint64_t row = (uint64_t)J->segs * (keys / ck + 2 + 3); /* 3: the kernel's cost of a segment */
     if (row > 0x7fffffffull) return pk_refuse("kv attend: a row too long for its heads");
     p->rows = 0xffffffffull / row < a->n_rows ? (uint32_t)(0xffffffffull / row) : a->n_rows;
     if (p->workers > row * p->rows) p->workers = (uint32_t)(row * p->rows);

@@ -64,14 +64,14 @@ struct pk_attend_job {
 template <uint32_t CT, int DP, int R, int QP>
 struct pk_shape {
     static constexpr int ELT = CT == PULSAR_TYPE_E4M3 ? 1 : 2;
-    static constexpr int ROW = DP * ELT;                  /* bytes of a key in shared memory */
+    static constexpr int ROW = (DP == 96 ? 128 : DP) * ELT; /* bytes of a key in shared memory: whole 64s or 128s */
     static constexpr int UNITS = ROW / 16;
     static constexpr int CK = PK_CK(ROW);
     /* A stage of the ring is a chunk's keys and values; at rows of 256 bytes or more its keys or its values,
-     * which take turns: stages stay at 4 to 8 KB. */
+     * which take turns: stages stay at 4 to 8 KB, a warp's ring at 18 to 24. */
     static constexpr bool SPLIT = ROW >= 256;
-    static constexpr int STAGES = 3;
     static constexpr int STAGE = (SPLIT ? 1 : 2) * CK * ROW;
+    static constexpr int STAGES = STAGE <= 4096 ? 6 : 3;
     static constexpr int RING = STAGES * STAGE;           /* per warp */
     static constexpr bool QSM = DP > 128;                 /* q's parts wait in shared memory, not registers */
     static constexpr int QW = R == 1 ? 2 * QP : 4 * QP;   /* their words per lane and k-step */
@@ -275,14 +275,18 @@ __device__ __forceinline__ uint32_t pk_prefix(uint32_t mine, uint32_t *upto) {
 
 /* a warp finds the sequence that holds unit `at` of the line: upto[t] are the
  * units of one segment each up to the rows of thread t (`run` rows a
- * thread); before = those of all earlier rows */
+ * thread), to which every segment adds `extra`; before = the units of all
+ * earlier rows without that */
 template <int CK>
 __device__ __forceinline__ uint32_t pk_locate(const pk_attend_job &J, const int2 *cached, const uint32_t *upto,
-                                              uint32_t run, uint32_t per, uint32_t at, uint32_t *before) {
+                                              uint32_t run, uint32_t per, uint32_t extra, uint32_t at, uint32_t *before) {
     const uint32_t lane = threadIdx.x & 31u;
     uint32_t t = 0;
 #pragma unroll
-    for (uint32_t k = 0; k < PK_WARPS; k++) t += __popc(__ballot_sync(~0u, upto[k * 32 + lane] * J.segs <= at));
+    for (uint32_t k = 0; k < PK_WARPS; k++) {
+        const uint32_t x = k * 32 + lane, rows = (x + 1) * run < J.A.n_rows ? (x + 1) * run : J.A.n_rows;
+        t += __popc(__ballot_sync(~0u, (upto[x] + extra * rows) * J.segs <= at));
+    }
     uint32_t sum = t ? upto[t - 1] : 0;
     if (run == 1) {
         *before = sum;
@@ -298,7 +302,7 @@ __device__ __forceinline__ uint32_t pk_locate(const pk_attend_job &J, const int2
             const uint32_t y = __shfl_up_sync(~0u, x, o);
             if (lane >= o) x += y;
         }
-        const uint32_t hit = __ballot_sync(~0u, in && (sum + x) * J.segs > at);
+        const uint32_t hit = __ballot_sync(~0u, in && (sum + x + extra * (r + 1)) * J.segs > at);
         if (hit || r0 + 32 >= (t + 1) * run || r0 + 32 >= J.A.n_rows) {
             const uint32_t k = hit ? __ffs(hit) - 1 : 0;
             *before = sum + __shfl_sync(~0u, x - n, k);
@@ -427,8 +431,9 @@ template <int DP, int HEADS, int PARTS>
 __device__ void pk_join(const pk_attend_job &J, const pk_joint &S, uint32_t first, uint32_t step, uint32_t count,
                         bool final, float (*ml)[2], float *room) {
     constexpr uint32_t FLOATS = HEADS * (DP + 2), THREADS = PK_WARPS * 32;
-    constexpr int NX = HEADS * DP / 4 / THREADS; /* runs of four columns a thread sums */
-    static_assert(NX * 4 * THREADS == HEADS * DP && PARTS > 0, "tiles are whole numbers of threads");
+    constexpr uint32_t RUNS = HEADS * DP / 4;                 /* of four columns */
+    constexpr int NX = (RUNS + THREADS - 1) / THREADS;        /* that a thread sums */
+    static_assert(PARTS > 0, "a part fits");
     float4 acc[NX];
 #pragma unroll
     for (int n = 0; n < NX; n++) acc[n] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -464,7 +469,9 @@ __device__ void pk_join(const pk_attend_job &J, const pk_joint &S, uint32_t firs
         __syncthreads();
 #pragma unroll
         for (int n = 0; n < NX; n++) {
-            const float keep = room[2 * ((n * THREADS + threadIdx.x) / (DP / 4)) + 1];
+            const uint32_t x = n * THREADS + threadIdx.x;
+            if (RUNS % THREADS && x >= RUNS) break;
+            const float keep = room[2 * (x / (DP / 4)) + 1];
             acc[n].x *= keep;
             acc[n].y *= keep;
             acc[n].z *= keep;
@@ -475,6 +482,7 @@ __device__ void pk_join(const pk_attend_job &J, const pk_joint &S, uint32_t firs
 #pragma unroll
             for (int n = 0; n < NX; n++) {
                 const uint32_t x = n * THREADS + threadIdx.x;
+                if (RUNS % THREADS && x >= RUNS) break;
                 const float by = room[k * FLOATS + 2 * (x / (DP / 4))];
                 const float4 v = *(const float4 *)(room + k * FLOATS + 2 * HEADS + 4 * x);
                 acc[n].x += v.x * by;
@@ -493,6 +501,7 @@ __device__ void pk_join(const pk_attend_job &J, const pk_joint &S, uint32_t firs
 #pragma unroll
     for (int n = 0; n < NX; n++) {
         const uint32_t x = n * THREADS + threadIdx.x, head = x / (DP / 4), col = x % (DP / 4) * 4, v = S.v0 + head;
+        if (RUNS % THREADS && x >= RUNS) break;
         if (!final) {
             __stcg((float4 *)(J.parts + S.slot(first) * (uint64_t)FLOATS + 2 * HEADS + 4 * x), acc[n]);
         } else if (v < J.rows && col < J.D.head_dim) {
@@ -568,8 +577,11 @@ __global__ void __launch_bounds__(PK_WARPS * 32, pk_shape<CT, DP, R, QP>::OCC) p
     const uint32_t total = all * J.segs, segs = B * J.segs;
     const bool brief = all <= 8u * B;                     /* 8 chunks a segment or fewer, on average */
     const bool solo = !QSM && brief && segs > gridDim.x;
+    /* a warp's slice is cut by cost: beside its chunks a segment costs about three (q, the results) */
+    const uint32_t extra = solo ? 3 : 0;
     const uint32_t workers = solo ? gridDim.x * PK_WARPS : gridDim.x, me = solo ? blockIdx.x * PK_WARPS + w : blockIdx.x;
-    uint32_t per = (total + workers - 1) / workers;
+    const uint32_t cost = total + extra * segs;
+    uint32_t per = (cost + workers - 1) / workers;
     /* Few segments: each is cut evenly among CTAs of its own, so that no CTA takes parts of two.  That makes
      * slices longer by segs / (CTAs - segs); a second segment in a slice costs its CTA about 14 chunks' time
      * (q, the warps' meeting, the join: 5 us). */
@@ -585,7 +597,7 @@ __global__ void __launch_bounds__(PK_WARPS * 32, pk_shape<CT, DP, R, QP>::OCC) p
         mine = 0;
         for (uint32_t r = tid * run; r < (tid + 1) * run && r < B; r++) mine += pk_units<CK>(J, cached, r, per);
         if (me >= pk_prefix(mine, upto) * J.segs) return; /* more CTAs than pieces */
-        cons.b = pk_locate<CK>(J, cached, upto, run, per, me, &at);
+        cons.b = pk_locate<CK>(J, cached, upto, run, per, 0, me, &at);
         cons.row = pk_row_of<CK>(J, B <= PK_CACHED ? cached[cons.b] : pk_len_of(J, cons.b, false));
         pieces = ((uint32_t)cons.row.n + per - 1) / per;
         in = (me - at * J.segs) / pieces;
@@ -595,33 +607,40 @@ __global__ void __launch_bounds__(PK_WARPS * 32, pk_shape<CT, DP, R, QP>::OCC) p
         hi = lo + each + (piece < more);
         cons.pos = (int32_t)lo;
     } else {
+        /* where the line position x lies: sequence, segment, chunk; solo: the first segment that begins at or
+         * behind it.  Returns the chunk's place on the line. */
+        auto place = [&](uint32_t x, uint32_t &b, uint32_t &seg, int32_t &pos) {
+            b = pk_locate<CK>(J, cached, upto, run, 1, extra, x, &at);
+            const uint32_t n = pk_units<CK>(J, cached, b, 1), off = x - (at + extra * b) * J.segs;
+            if (solo) {
+                seg = (off + n + extra - 1) / (n + extra);
+                pos = 0;
+                return at * J.segs + seg * n;
+            }
+            seg = off / n;
+            pos = (int32_t)(off - seg * n);
+            return x;
+        };
         lo = per * me;
-        if (per && lo / per != me) lo = total;            /* past 2^32: past the end */
-        hi = total - lo < per || lo >= total ? total : lo + per;
-        if (lo < total) {
-            cons.b = pk_locate<CK>(J, cached, upto, run, 1, lo, &at);
-            cons.row = pk_row_of<CK>(J, B <= PK_CACHED ? cached[cons.b] : pk_len_of(J, cons.b, false));
-            in = (lo - at * J.segs) / (uint32_t)cons.row.n;
-            cons.pos = (int32_t)(lo - at * J.segs - in * (uint32_t)cons.row.n);
+        hi = total;
+        if ((per && lo / per != me) || lo >= cost) {      /* past 2^32: past the end */
+            lo = total;
+        } else {
+            uint32_t b2, seg2;
+            int32_t pos2;
+            if (cost - lo > per) hi = solo ? place(lo + per, b2, seg2, pos2) : lo + per;
+            lo = place(lo, cons.b, in, cons.pos);
+            if (in == J.segs) { /* solo: behind the row's last segment */
+                in = 0;
+                cons.b++;
+            }
+            if (lo < hi) cons.row = pk_row_of<CK>(J, B <= PK_CACHED ? cached[cons.b] : pk_len_of(J, cons.b, false));
         }
     }
     if (lo < hi) {
         cons.hk = J.tiles == 1 ? in : in / J.tiles;
         cons.tile = in - cons.hk * J.tiles;
         cons.enter(J);
-        if (solo) {
-            /* whole segments: those that begin in [lo, hi) */
-            if (cons.pos) {
-                const int32_t rest = cons.row.n - cons.pos;
-                lo += rest;
-                cons.step(J, cached, rest);
-            }
-            if (hi < total) {
-                const uint32_t b2 = pk_locate<CK>(J, cached, upto, run, 1, hi, &at);
-                const uint32_t n2 = pk_units<CK>(J, cached, b2, 1);
-                hi = at * J.segs + (hi - at * J.segs + n2 - 1) / n2 * n2;
-            }
-        }
     }
     __syncthreads(); /* `upto` has been read */
     if (lo >= hi) return; /* a CTA's four warps alike, but for solo ones, which meet no more */
@@ -1094,7 +1113,7 @@ __global__ void __launch_bounds__(PK_WARPS * 32, pk_shape<CT, DP, R, QP>::OCC) p
                 for (int c0 = 0; c0 < DP; c0 += 64) {
                     if (y || c0) __syncthreads(); /* the previous columns have been read */
 #pragma unroll
-                    for (int t = 0; t < 8; t += RUN / 2) {
+                    for (int t = 0; t < (NT - c0 / 8 < 8 ? NT - c0 / 8 : 8); t += RUN / 2) {
                         float x[RUN], *d = side + (w * 8 + g) * S::XROW + t * 8 + RUN * c;
                         columns(y, c0 / 8 + t, keep, x);
                         if constexpr (F8) *(float4 *)d = make_float4(x[0], x[1], x[RUN - 2], x[RUN - 1]);
@@ -1113,7 +1132,8 @@ __global__ void __launch_bounds__(PK_WARPS * 32, pk_shape<CT, DP, R, QP>::OCC) p
                         z.z += v.z;
                         z.w += v.w;
                     }
-                    if (cut) {
+                    if (DP % 64 && col >= DP) {
+                    } else if (cut) {
                         __stcg((float4 *)(part + 2 * HEADS + head * DP + col), z);
                         if (col == 0) __stcg((float2 *)(part + 2 * head), make_float2(fml[head][0], fml[head][1]));
                     } else if (v0 + head < J.rows && col < J.D.head_dim) {
@@ -1190,6 +1210,7 @@ static pk_attend_fn pk_attend_pick_at(int r, bool wide) {
 template <uint32_t CT>
 static pk_attend_fn pk_attend_pick(int dp, int r, bool wide) {
     if (dp == 64) return pk_attend_pick_at<CT, 64>(r, wide);
+    if (dp == 96) return pk_attend_pick_at<CT, 96>(r, wide);
     if (dp == 128) return pk_attend_pick_at<CT, 128>(r, wide);
     if constexpr (CT != PULSAR_TYPE_E4M3) /* rows of 192 bytes would break the swizzle's 128 */
         if (dp == 192) return pk_attend_pick_at<CT, 192>(r, wide);
