@@ -53,6 +53,7 @@ __global__ void __launch_bounds__(256, V == 8 && !NEAR && HU > 1 ? 3 : 4) /* 64 
     typedef typename pk_type<X>::t T;
     constexpr int P = NEAR ? V / 2 : V;                    /* pairs of an item */
     const uint32_t it = blockIdx.x * blockDim.x + threadIdx.x;
+    pk_enter();
     if (it >= G.items) return;
     const uint32_t n_turn = (G.q + G.kv) * G.head;
     const bool is_v = it >= n_turn;
@@ -178,8 +179,7 @@ static int pk_append_grid(const pulsar_kv_desc *d, const pulsar_kv_append_args *
      * its item of more of them), a token a thread where there are fewer */
     const uint32_t y = (a->n_tok + block.y - 1) / block.y, most = (16 * pk_sm_count() + grid.x - 1) / grid.x;
     grid.y = y < most ? y : most;
-    pk_append_kernel<X, V, NEAR, HU><<<grid, block, 0, st>>>(*d, *a, g, pk_err_word());
-    return pm_ok(cudaGetLastError(), "kv append launch");
+    return pm_ok(pk_launch(pk_append_kernel<X, V, NEAR, HU>, grid, block, 0, st, *d, *a, g, pk_err_word()), "kv append launch");
 }
 
 template <uint32_t X, int V>

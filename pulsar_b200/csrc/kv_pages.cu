@@ -32,28 +32,6 @@ extern "C" uint32_t pulsar_kv_error(void) {
     return v;
 }
 
-/* An apply kernel is launched while its plan still runs: its CTAs take their
- * places and wait there (in the hardware, for the plan's end and its writes),
- * which saves the launch's latency. */
-__device__ __forceinline__ void pk_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-__device__ __forceinline__ void pk_await() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-
-template <class... A>
-static cudaError_t pk_launch_after(void (*kernel)(A...), uint32_t grid, uint32_t block, uint32_t smem, cudaStream_t st,
-                                   A... args) {
-    cudaLaunchAttribute early;
-    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    early.val.programmaticStreamSerializationAllowed = 1;
-    cudaLaunchConfig_t c = {};
-    c.gridDim = grid;
-    c.blockDim = block;
-    c.dynamicSmemBytes = smem;
-    c.stream = st;
-    c.attrs = &early;
-    c.numAttrs = 1;
-    return cudaLaunchKernelEx(&c, kernel, args...);
-}
-
 #define PK_PLAN 1024u /* threads of a plan CTA */
 #define PK_FORK_COLS 8u
 
@@ -137,6 +115,7 @@ __global__ void __launch_bounds__(PK_PLAN) pk_grow_kernel(pulsar_kv_pool P, cons
     __shared__ pk_scan scan;
     __shared__ uint32_t bad, marks[PK_MARKS];
     __shared__ unsigned long long wanted; /* need_all could wrap: nothing is taken from it unless this fits */
+    pk_enter();
     uint32_t *mark = P.n_rows <= PK_MARKS ? marks : ws, *off = ws + P.n_rows;
     const uint32_t tid = threadIdx.x;
     const uint32_t cap = P.max_pages * P.page_size;
@@ -232,10 +211,10 @@ __global__ void __launch_bounds__(PK_PLAN) pk_fork_plan_kernel(pulsar_kv_pool P,
                                                                void *wsp) {
     __shared__ pk_scan scan;
     __shared__ uint32_t bad, wide, marks[PK_MARKS];
+    pk_enter();
     pk_fork_ws w = pk_fork_layout(wsp, P.n_rows, n);
     const uint32_t tid = threadIdx.x;
     const uint32_t cap = P.max_pages * P.page_size;
-    pk_dependents();
     if (2 * P.n_rows <= PK_MARKS) {
         w.mark = marks;
         w.first = marks + P.n_rows;
@@ -372,7 +351,7 @@ __global__ void __launch_bounds__(256) pk_fork_apply_kernel(pulsar_kv_pool P, co
                                                             uint32_t *err) {
     extern __shared__ int32_t stage[]; /* [n][PK_FORK_COLS] */
     const pk_fork_ws w = pk_fork_layout((void *)wsp, P.n_rows, n);
-    pk_await();
+    pk_enter();
     if (!w.head[0]) return;
     if (blockIdx.x >= table_blocks) {
         pk_copy_pages(P, w.pair, w.pair + 1, 2, w.head[1], blockIdx.x - table_blocks, gridDim.x - table_blocks, err);
@@ -420,9 +399,9 @@ __global__ void __launch_bounds__(PK_PLAN) pk_compact_plan_kernel(pulsar_kv_pool
     const uint32_t half = P.n_pages / 2 + 1;
     uint32_t *head = ws;
     int32_t *from = (int32_t *)ws + 4, *to = from + half, *map = to + half;
+    pk_enter();
     const auto none = [](uint32_t) { return 0u; };
     const auto every = [](uint32_t total) { return total; };
-    pk_dependents();
     const uint32_t live = pk_choose(P.refs, 0, P.n_pages, true, scan, none, [](uint32_t, uint32_t) {});
     const uint32_t moves = pk_choose(P.refs, 0, live, false, scan, every,
                                      [&](uint32_t page, uint32_t rank) { to[rank] = (int32_t)page; });
@@ -440,7 +419,7 @@ __global__ void __launch_bounds__(PK_PLAN) pk_compact_plan_kernel(pulsar_kv_pool
 
 __global__ void __launch_bounds__(256) pk_compact_apply_kernel(pulsar_kv_pool P, uint32_t table_blocks,
                                                                const uint32_t *ws, uint32_t *err) {
-    pk_await();
+    pk_enter();
     const uint32_t half = P.n_pages / 2 + 1, moves = ws[0], live = ws[1];
     const int32_t *from = (const int32_t *)ws + 4, *to = from + half, *map = to + half;
     if (blockIdx.x >= table_blocks) {
@@ -507,8 +486,8 @@ extern "C" int pulsar_kv_grow(const pulsar_kv_pool *p, const int32_t *rows, cons
                               int32_t *status, void *ws, size_t ws_bytes, void *stream) {
     if (!pk_pool_check(p, status, ws, ws_bytes, n)) return 0;
     if (!n_new || !n || n > p->n_rows) return pk_refuse("kv grow: between 1 and n_rows rows, each with a count");
-    pk_grow_kernel<<<1, PK_PLAN, 0, pk_stream(stream)>>>(*p, rows, n_new, n, status, (uint32_t *)ws);
-    return pm_ok(cudaGetLastError(), "kv grow launch");
+    return pm_ok(pk_launch(pk_grow_kernel, 1, PK_PLAN, 0, pk_stream(stream), *p, rows, n_new, n, status, (uint32_t *)ws),
+                 "kv grow launch");
 }
 
 extern "C" int pulsar_kv_fork(const pulsar_kv_pool *p, const int32_t *dst, const int32_t *src, uint32_t n,
@@ -520,25 +499,25 @@ extern "C" int pulsar_kv_fork(const pulsar_kv_pool *p, const int32_t *dst, const
     const uint32_t smem = n * PK_FORK_COLS * 4u;
     if (!pm_smem_attr(pk_fork_apply_kernel, smem, &done)) return 0;
     const cudaStream_t st = pk_stream(stream);
-    pk_fork_plan_kernel<<<1, PK_PLAN, 0, st>>>(*p, dst, src, n, status, ws);
-    if (!pm_ok(cudaGetLastError(), "kv fork plan launch")) return 0;
+    if (!pm_ok(pk_launch(pk_fork_plan_kernel, 1, PK_PLAN, 0, st, *p, dst, src, n, status, ws), "kv fork plan launch"))
+        return 0;
     const uint32_t sms = pk_sm_count();
     const uint32_t tb = p->max_pages < 2 * sms ? p->max_pages : 2 * sms;
     const uint32_t cb = p->n_slab ? 4 * sms : 0;
-    return pm_ok(pk_launch_after(pk_fork_apply_kernel, tb + cb, 256, smem, st, *p, dst, src, n, tb, (const void *)ws,
-                                 pk_err_word()),
+    return pm_ok(pk_launch(pk_fork_apply_kernel, tb + cb, 256, smem, st, *p, dst, src, n, tb, (const void *)ws,
+                           pk_err_word()),
                  "kv fork launch");
 }
 
 extern "C" int pulsar_kv_compact(const pulsar_kv_pool *p, int32_t *status, void *ws, size_t ws_bytes, void *stream) {
     if (!pk_pool_check(p, status, ws, ws_bytes, 0)) return 0;
     const cudaStream_t st = pk_stream(stream);
-    pk_compact_plan_kernel<<<1, PK_PLAN, 0, st>>>(*p, status, (uint32_t *)ws);
-    if (!pm_ok(cudaGetLastError(), "kv compact plan launch")) return 0;
+    if (!pm_ok(pk_launch(pk_compact_plan_kernel, 1, PK_PLAN, 0, st, *p, status, (uint32_t *)ws), "kv compact plan launch"))
+        return 0;
     const uint32_t sms = pk_sm_count();
     uint32_t tb = (p->n_rows + 7) / 8;
     if (tb > 2 * sms) tb = 2 * sms;
-    return pm_ok(pk_launch_after(pk_compact_apply_kernel, tb + 4 * sms, 256, 0, st, *p, tb, (const uint32_t *)ws,
-                                 pk_err_word()),
+    return pm_ok(pk_launch(pk_compact_apply_kernel, tb + 4 * sms, 256, 0, st, *p, tb, (const uint32_t *)ws,
+                           pk_err_word()),
                  "kv compact launch");
 }

@@ -557,6 +557,7 @@ __global__ void __launch_bounds__(PK_WARPS * 32, pk_shape<CT, DP, R, QP>::OCC) p
     const uint32_t tid = threadIdx.x, lane = tid & 31u, w = tid >> 5;
     const uint32_t g = lane >> 2, c = lane & 3u;          /* row and column pair of a fragment */
 
+    pk_enter();
     /* ---- the line's length */
     const uint32_t B = J.A.n_rows;
     const uint32_t run = (B + PK_WARPS * 32 - 1) / (PK_WARPS * 32);
@@ -1189,8 +1190,7 @@ static int pk_attend_launch(const pk_attend_job &J, uint32_t grid, cudaStream_t 
     auto kernel = pk_attend_kernel<CT, DP, R, QP>;
     if (!pm_smem_attr(kernel, smem, &done)) return 0;
     const uint32_t most = S::OCC * pk_sm_count(); /* one wave */
-    kernel<<<grid < most ? grid : most, PK_WARPS * 32, smem, st>>>(J);
-    return pm_ok(cudaGetLastError(), "kv attend launch");
+    return pm_ok(pk_launch(kernel, grid < most ? grid : most, PK_WARPS * 32, smem, st, J), "kv attend launch");
 }
 
 /* one translation unit per cache type (kv_attend_*.cu); r as the kernel's R,

@@ -53,6 +53,32 @@ static inline const char *pk_desc_fault(const pulsar_kv_desc *d) {
     return nullptr;
 }
 
+/* ------------------------------------------------------ launches */
+
+/* A kernel of the family may be launched while the one before it in its
+ * stream, if that is of the family too, still runs: its CTAs take the places
+ * that come free and wait at pk_enter (in the hardware, for the end and the
+ * writes of what came before), which saves the launch's latency.  Each kernel
+ * enters before its first access to global memory. */
+__device__ __forceinline__ void pk_enter() {
+    asm volatile("griddepcontrol.wait;\n\tgriddepcontrol.launch_dependents;" ::: "memory");
+}
+
+template <class... P, class... A>
+static cudaError_t pk_launch(void (*kernel)(P...), dim3 grid, dim3 block, uint32_t smem, cudaStream_t st, A... args) {
+    cudaLaunchAttribute early;
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t c = {};
+    c.gridDim = grid;
+    c.blockDim = block;
+    c.dynamicSmemBytes = smem;
+    c.stream = st;
+    c.attrs = &early;
+    c.numAttrs = 1;
+    return cudaLaunchKernelEx(&c, kernel, (P)args...);
+}
+
 /* ------------------------------------------------------ values by type */
 
 template <uint32_t T> struct pk_type;
