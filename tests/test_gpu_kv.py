@@ -516,3 +516,39 @@ def test_pool_calls_in_a_graph(kv):
         assert model.fork(parents, [0, 1, 2, 3])[0] == 0 and model.grow([0, 1, 2, 3], [1] * 4) == 0
         same(pool, model)
     pool.check()
+
+
+def test_chained_calls_see_each_other(kv):
+    """growth, append, attention and forks one behind the other on a stream, nothing between them (the kernels
+    overlap): the same bits as with the device waited for after every call"""
+    D, n_kv, H, rows, page = 64, 2, 8, 24, 8
+    gen = torch.Generator(device="cuda").manual_seed(40)
+    steps = 40
+    x = values((steps, rows, (H + 2 * n_kv) * D), BF16, gen)
+    ids = torch.arange(rows, dtype=torch.int32, device="cuda")
+    one = torch.ones(rows, dtype=torch.int32, device="cuda")
+    perm = torch.stack([torch.randint(0, rows, (rows,), generator=gen, device="cuda") for _ in range(steps)]).to(torch.int32)
+    cs = kv.rope_table(steps + 1, D)
+
+    def run(wait):
+        pool = kv.KvPool.empty(1, 600, page, n_kv, D, rows, 8)
+        layer, outs = pool.layer(0), []
+        turned = torch.zeros((rows, H, D), dtype=BF16, device="cuda")
+        pos = [torch.full((rows,), t, dtype=torch.int32, device="cuda") for t in range(steps)]
+        cut = [[z.unflatten(1, (-1, D)) for z in x[t].split([H * D, n_kv * D, n_kv * D], 1)] for t in range(steps)]
+        outs = [torch.zeros((rows, H, D), dtype=BF16, device="cuda") for _ in range(steps)]
+        torch.cuda.synchronize()
+        for t in range(steps):
+            for f in (lambda: pool.grow(one, ids), lambda: layer.append(*cut[t], ids, pos[t], cs, turned),
+                      lambda: layer.attend(turned, pool.lens, outs[t]), lambda: pool.fork(perm[t], ids),
+                      lambda: pool.compact() if t % 5 == 4 else None):
+                f()
+                if wait:
+                    torch.cuda.synchronize()
+        torch.cuda.synchronize()
+        pool.check()
+        return torch.stack(outs), pool.table.clone(), pool.refs.clone()
+
+    a, b = run(True), run(False)
+    assert torch.isfinite(a[0]).all() and kv.kv_error() == 0
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
