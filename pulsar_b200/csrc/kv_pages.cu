@@ -107,7 +107,8 @@ __device__ uint32_t pk_choose(const int32_t *refs, uint32_t lo, uint32_t hi, boo
     return total;
 }
 
-/* words of row marks that a plan keeps in shared memory; longer tables use the workspace */
+/* words that a plan keeps in shared memory (row marks, offsets, ranks: what it looks up at random); more rows than
+ * that use the workspace */
 #define PK_MARKS 8192u
 
 __device__ __forceinline__ uint32_t pk_ceil(uint32_t a, uint32_t b) { return (a + b - 1u) / b; }
@@ -122,7 +123,8 @@ __global__ void __launch_bounds__(PK_PLAN) pk_grow_kernel(pulsar_kv_pool P, cons
     __shared__ uint32_t bad, marks[PK_MARKS];
     __shared__ unsigned long long wanted; /* need_all could wrap: nothing is taken from it unless this fits */
     pk_enter();
-    uint32_t *mark = P.n_rows <= PK_MARKS ? marks : ws, *off = ws + P.n_rows;
+    const bool near = (uint64_t)P.n_rows + n <= PK_MARKS;
+    uint32_t *mark = near ? marks : ws, *off = mark + P.n_rows;
     const uint32_t tid = threadIdx.x;
     const uint32_t cap = P.max_pages * P.page_size;
     if (tid == 0) {
@@ -221,9 +223,10 @@ __global__ void __launch_bounds__(PK_PLAN) pk_fork_plan_kernel(pulsar_kv_pool P,
     pk_fork_ws w = pk_fork_layout(wsp, P.n_rows, n);
     const uint32_t tid = threadIdx.x;
     const uint32_t cap = P.max_pages * P.page_size;
-    if (2 * P.n_rows <= PK_MARKS) {
+    if (2ull * P.n_rows + n <= PK_MARKS) {
         w.mark = marks;
         w.first = marks + P.n_rows;
+        w.rank = w.first + P.n_rows; /* the apply kernel does not read these */
     }
     if (tid == 0) bad = wide = 0;
     for (uint32_t r = tid; r < P.n_rows; r += PK_PLAN) {

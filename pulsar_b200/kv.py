@@ -149,6 +149,7 @@ class PagedKv:
         _need(table.dim() == 2 and table.dtype == torch.int32 and table.device == k.device and table.stride(1) == 1,
               "PagedKv: table is int32 [n_rows][max_pages] beside the cache")
         _need(table.shape[0] == 1 or table.stride(0) >= table.shape[1], "PagedKv: table rows overlap")
+        _need(k.dtype == torch.float8_e4m3fn or (k_scale is None and v_scale is None), "PagedKv: scales belong to e4m3 caches")
         for s in (k_scale, v_scale):
             _need(s is None or (s.dtype == torch.float32 and s.device == k.device and s.is_contiguous()
                                 and s.numel() == k.shape[1]), "PagedKv: scales are f32 [n_kv] beside the cache")

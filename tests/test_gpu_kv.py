@@ -450,6 +450,77 @@ def test_pages_follow_the_model(kv, page, n_pages, n_rows, width, seed):
     assert kv.kv_error() == 0
 
 
+@pytest.mark.parametrize("n_rows", [4000, 9000])
+def test_pages_of_many_rows(kv, n_rows):
+    """more rows than a plan keeps in shared memory (fork's marks, growth's too)"""
+    import random
+    rng = random.Random(n_rows)
+    pool = kv.KvPool.empty(1, 3 * n_rows, 2, 1, 16, n_rows, 4, dtype=F16)
+    model = kv_ref.Pages(n_rows, 4, 3 * n_rows, 2)
+    for step in range(4):
+        rows = rng.sample(range(n_rows), n_rows if step == 0 else 2500)
+        n_new = [rng.randint(0, 1 if step else 3) for _ in rows]
+        assert model.grow(rows, n_new) == 0
+        pool.grow(i32(n_new), i32(rows))
+        dst = rng.sample(range(n_rows), 900)
+        src = [rng.choice((-1, rng.randrange(n_rows), dst[0], dst[1])) for _ in dst]
+        assert model.fork(src, dst)[0] == 0
+        pool.fork(i32(src), i32(dst))
+        pool.check()
+        same(pool, model)
+    model.compact()
+    pool.compact()
+    same(pool, model)
+    # a row named twice is found among many
+    rows[-1] = rows[0]
+    pool.grow(i32(n_new), i32(rows))
+    assert int(pool.status[0, 0]) == 3
+    dst[-1] = dst[0]
+    pool.fork(i32(src), i32(dst))
+    assert int(pool.status[1, 0]) == 3
+    same(pool, model)
+
+
+def test_python_refusals(kv):
+    """what the wrappers refuse before a launch"""
+    gen = torch.Generator(device="cuda").manual_seed(50)
+    k, v, table = cache([20, 9], 2, 64, 8, BF16, gen)
+    c = kv.PagedKv(k, v, table)
+    n = torch.tensor([20, 9], dtype=torch.int32, device="cuda")
+    q = values((2, 4, 64), BF16, gen)
+    out = torch.zeros_like(q)
+    bad = [dict(q=q.double()), dict(out=out.float()), dict(q=q[:, :, :32], out=out[:, :, :32]), dict(lens=n.long()),
+           dict(lens=n[:1]), dict(lens=n.cpu()), dict(q=q.transpose(0, 1), out=out.transpose(0, 1)), dict(window=-1),
+           dict(sinks=torch.zeros(3, device="cuda")), dict(lse=torch.zeros(2, device="cuda")), dict(q=q.cpu()),
+           dict(seq=n.cpu()), dict(q=q[:, ::2], out=out[:, ::2])]
+    for kw in bad:
+        a = dict(q=q, lens=n, out=out)
+        a.update(kw)
+        with pytest.raises(ValueError):
+            c.attend(a.pop("q"), a.pop("lens"), a.pop("out"), **a)
+    with pytest.raises(kv.KernelError):
+        c.attend(q[:, :3].contiguous(), n, out[:, :3].contiguous())       # 3 query heads over 2 key heads
+    with pytest.raises(kv.KernelError):
+        c.attend(q.repeat(2, 1, 1), n.repeat(2), out.repeat(2, 1, 1))      # more rows than the table
+    with pytest.raises(kv.KernelError):
+        c.attend(q, n, out, ws=torch.zeros(64, dtype=torch.uint8, device="cuda"))
+    x, pos = values((2, 2, 64), BF16, gen), torch.zeros(2, dtype=torch.int32, device="cuda")
+    cs = kv.rope_table(4, 64)
+    for a in ((None, x.float(), x, pos, pos, cs, None), (None, x, x[:1], pos, pos, cs, None), (None, x, x, pos.long(), pos, cs, None),
+              (None, x, x, pos, pos, cs.half(), None), (q[:, :, :32], x, x, pos, pos, cs, q), (q, x, x, pos, pos, cs, q[:1])):
+        with pytest.raises(ValueError):
+            c.append(*a)
+    with pytest.raises(kv.KernelError):
+        c.append(None, x, x, pos, pos, kv.rope_table(4, 128), None)        # wider than the head
+    for a in ((k.float(), v.float(), table), (k, v[:1], table), (k, v, table.long()), (k, v, table[:1].expand(2, -1)),
+              (k.transpose(2, 3), v.transpose(2, 3), table), (k, v, table, torch.ones(2, device="cuda"))):
+        with pytest.raises(ValueError):
+            kv.PagedKv(*a)
+    empty = torch.zeros((0, 4, 64), dtype=BF16, device="cuda")
+    assert c.attend(empty, n[:0], empty.clone()).numel() == 0 and c.append(None, x[:0], x[:0], pos[:0], pos[:0], cs, None) is None
+    assert kv.kv_error() == 0
+
+
 def test_pages_refusals_change_nothing(kv):
     pool = kv.KvPool.empty(1, 6, 4, 1, 16, 4, 3)
     pool.grow(i32([6, 3]), i32([0, 2]))
