@@ -220,8 +220,10 @@ template <int CK, int HEADS>
 struct pk_cursor {
     uint32_t b, hk, tile;
     int32_t pos, lo, hi;
+    uint64_t head; /* byte offset of the key head */
     pk_row row;
     __device__ __forceinline__ void enter(const pk_attend_job &J) {
+        head = hk * J.D.head_stride * (J.D.dtype == PULSAR_TYPE_E4M3 ? 1 : 2);
         uint32_t i0 = 0, i1 = 0;
         if (J.A.n_q > 1) {
             const uint32_t v0 = tile * HEADS, v1 = v0 + HEADS < J.rows ? v0 + HEADS - 1 : J.rows - 1;
@@ -677,7 +679,18 @@ __global__ void __launch_bounds__(PK_WARPS * 32, pk_shape<CT, DP, R, QP>::OCC) p
     const uint32_t cu = lane % S::UNITS, cr = lane / S::UNITS; /* a lane's 16 bytes and first key in it */
     const bool runs = J.D.page_size % 8 == 0;             /* 8 aligned keys are in one page */
     const bool copies = cr < RPI && cu < units;
-    const uint64_t tok_bytes = J.D.tok_stride * S::ELT;
+    const uint32_t tok_bytes = (uint32_t)J.D.tok_stride * S::ELT;
+    const uint64_t page_bytes = J.D.page_stride * S::ELT;
+    /* what does not change of the copies' addresses: a lane's first source less its key's offset, its targets in
+     * the first 8 keys of a stage */
+    const uint64_t lane_at = (uint64_t)J.D.k + (uint64_t)cr * tok_bytes + cu * 16;
+    const uint64_t key_step = (uint64_t)RPI * tok_bytes;
+    uint32_t lane_to[8 / RPI];
+#pragma unroll
+    for (uint32_t i = 0; i < 8 / RPI; i++) {
+        const uint32_t r = i * RPI + cr;
+        lane_to[i] = kbase + r * S::ROW + (S::ROW >= 128 ? cu ^ (r & 7u) : cu ^ ((r >> 1) & 3u)) * 16;
+    }
     const uint64_t k_to_v = (uint64_t)((const uint8_t *)J.D.v - (const uint8_t *)J.D.k);
     if (ahead < slice) fetch();
 
@@ -690,40 +703,39 @@ __global__ void __launch_bounds__(PK_WARPS * 32, pk_shape<CT, DP, R, QP>::OCC) p
                 }
                 there = __ballot_sync(~0u, real);
                 if (lane == 0) vmask[w][st] = there;
-                at_key = real ? ((uint64_t)page * J.D.page_stride + prod.hk * J.D.head_stride) * S::ELT + slot * tok_bytes : 0;
+                at_key = real ? page * page_bytes + prod.head + (uint64_t)slot * tok_bytes : 0;
             }
-            const uint8_t *base = (const uint8_t *)J.D.k + cu * 16 + (S::SPLIT && values ? k_to_v : 0);
-            const uint32_t dst = kbase + st * S::STAGE + cr * S::ROW;
+            const uint64_t base = lane_at + (S::SPLIT && values ? k_to_v : 0);
+            const uint32_t to = st * S::STAGE;
             if (there == ~0u && runs) {
                 /* every key: within 8 of them addresses go up by a constant */
 #pragma unroll
                 for (uint32_t h = 0; h < CK; h += 8) {
                     const uint32_t lo32 = __shfl_sync(~0u, (uint32_t)at_key, h), hi32 = __shfl_sync(~0u, (uint32_t)(at_key >> 32), h);
                     if (copies) {
-                        const uint8_t *k = base + ((uint64_t)hi32 << 32 | lo32) + cr * tok_bytes;
+                        uint64_t k = base + ((uint64_t)hi32 << 32 | lo32);
 #pragma unroll
                         for (uint32_t i = 0; i < 8 / RPI; i++) {
-                            const uint32_t r = h + i * RPI + cr;
-                            const uint32_t d = dst + (h + i * RPI) * S::ROW + (S::ROW >= 128 ? cu ^ (r & 7u) : cu ^ ((r >> 1) & 3u)) * 16;
-                            pk_cp16(d, k, true);
-                            if constexpr (!S::SPLIT) pk_cp16(d + CK * S::ROW, k + k_to_v, true);
-                            k += RPI * tok_bytes;
+                            pk_cp16(lane_to[i] + to + h * S::ROW, (const void *)k, true);
+                            if constexpr (!S::SPLIT) pk_cp16(lane_to[i] + to + (h + CK) * S::ROW, (const void *)(k + k_to_v), true);
+                            k += key_step;
                         }
                     }
                 }
             } else if (there) {
-#pragma unroll 4
-                for (uint32_t i = 0; i < CK / RPI; i++) {
-                    const uint32_t r = i * RPI + (cr < RPI ? cr : 0);
-                    const uint32_t lo32 = __shfl_sync(~0u, (uint32_t)at_key, r), hi32 = __shfl_sync(~0u, (uint32_t)(at_key >> 32), r);
-                    const uint8_t *k = base + ((uint64_t)hi32 << 32 | lo32);
-                    const uint32_t d = dst + i * RPI * S::ROW + (S::ROW >= 128 ? cu ^ (r & 7u) : cu ^ ((r >> 1) & 3u)) * 16;
-                    const bool ok = there >> r & 1u;
-                    if (copies) {
-                        pk_cp16(d, k, ok);
-                        if constexpr (!S::SPLIT) pk_cp16(d + CK * S::ROW, k + k_to_v, ok);
+#pragma unroll 1
+                for (uint32_t h = 0; h < CK; h += 8)
+#pragma unroll
+                    for (uint32_t i = 0; i < 8 / RPI; i++) {
+                        const uint32_t r = h + i * RPI + (cr < RPI ? cr : 0);
+                        const uint32_t lo32 = __shfl_sync(~0u, (uint32_t)at_key, r), hi32 = __shfl_sync(~0u, (uint32_t)(at_key >> 32), r);
+                        const uint64_t k = base - (uint64_t)cr * tok_bytes + ((uint64_t)hi32 << 32 | lo32);
+                        const bool ok = there >> r & 1u;
+                        if (copies) {
+                            pk_cp16(lane_to[i] + to + h * S::ROW, (const void *)k, ok);
+                            if constexpr (!S::SPLIT) pk_cp16(lane_to[i] + to + (h + CK) * S::ROW, (const void *)(k + k_to_v), ok);
+                        }
                     }
-                }
             }
             if (S::SPLIT) values = !values;
             if (!values) {

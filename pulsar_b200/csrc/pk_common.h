@@ -49,6 +49,7 @@ static inline const char *pk_desc_fault(const pulsar_kv_desc *d) {
     const uint64_t e = pk_type_bytes(d->dtype);
     if (((uintptr_t)d->k | (uintptr_t)d->v | d->page_stride * e | d->head_stride * e | d->tok_stride * e) % 16)
         return "kv: cache pointers and strides are multiples of 16 bytes";
+    if (d->tok_stride > 0x0fffffffull) return "kv: tokens are less than 2^28 values apart";
     if (d->dtype != PULSAR_TYPE_E4M3 && (d->k_scale || d->v_scale)) return "kv: scales belong to e4m3 caches";
     return nullptr;
 }

@@ -56,7 +56,7 @@ def desc(**kw):
 DESC_FAULTS = [dict(k=None), dict(table=None), dict(dtype=0), dict(dtype=4), dict(n_pages=0), dict(page_size=0),
                dict(n_kv=0), dict(n_rows=0), dict(max_pages=0), dict(head_dim=0), dict(head_dim=72),
                dict(head_dim=272), dict(table_stride=3), dict(k=4104), dict(tok_stride=65), dict(head_stride=1020),
-               dict(k_scale=4096), dict(max_pages=1 << 28, table_stride=1 << 28)]
+               dict(k_scale=4096), dict(max_pages=1 << 28, table_stride=1 << 28), dict(tok_stride=1 << 28)]
 
 
 def append_args(**kw):
