@@ -6,9 +6,9 @@
  * for up to 16 query heads that share it, and 2 x 16 x head_dim multiply-adds
  * per key are far below what the warp matrix instructions do in that time.
  * Measured: 256 sequences of up to 4096 keys, bf16, 32 / 8 heads of 128:
- * 401 us, 6.5 TB/s (a copy's rate); 4 of up to 131071 in e4m3, 64 / 8 heads:
- * 123 us, 5.2 TB/s (the loads alone 105 us); one of 100 keys: 7.8 us, all of
- * it latency.
+ * 389 to 410 us, 6.4 to 6.7 TB/s (a copy's rate); 4 of up to 131071 in e4m3,
+ * 64 / 8 heads: 113 to 128 us, 5.0 to 5.7 TB/s (the loads alone 105 us); one
+ * of 100 keys: 7.1 us, all of it latency.
  *
  * Work.  The query rows of a key head are its n_q * (n_head / n_kv) (token,
  * head) pairs; a tile is HEADS of them.  All (sequence, key head, tile)
