@@ -93,10 +93,9 @@ int pulsar_kv_append(const pulsar_kv_desc *d, const pulsar_kv_append_args *a, vo
  * q_type, q_stride / out_stride values apart.  n_head is a multiple of
  * n_kv; query head h reads key head h / (n_head / n_kv).  Keys beyond a
  * token's span have no influence, whatever their bytes are; an infinite or
- * NaN score or value that is seen gives what the formula gives, or NaN.  (The
- * n_q tokens of a sequence share tiles: a value, not a key, that is infinite
- * or NaN and within the span of one of them may make its columns NaN in the
- * others' outputs too.)
+ * NaN score or value that is seen gives what the formula gives, or NaN.  (Where
+ * a value that some of a sequence's n_q tokens see and others do not is
+ * infinite or NaN, the outputs of those that see it are NaN throughout.)
  * ws: pulsar_kv_attend_workspace bytes (with a NULL: enough for any
  * arguments over this cache), aligned to 16; its first PULSAR_KV_WS_ZEROED bytes
  * are zero before the first call and are zero again after every call.  One

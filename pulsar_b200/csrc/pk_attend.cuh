@@ -163,6 +163,31 @@ __device__ __forceinline__ float pk_exp2(float x) {
     return r;
 }
 
+/* a warp zeroes the rows of CK values in shared memory that hold an infinity or
+ * NaN; returns which (of those that are there) */
+template <uint32_t CT, int CK, int ROW>
+__device__ __noinline__ uint32_t pk_take_odd(uint32_t rows, uint32_t there) {
+    constexpr uint32_t ONES = CT == PULSAR_TYPE_E4M3 ? 0x7f7f7f7fu : CT == PULSAR_TYPE_BF16 ? 0x7f807f80u : 0x7c007c00u;
+    const uint32_t lane = threadIdx.x & 31u, at = rows + lane % CK * ROW;
+    uint32_t hit = 0;
+#pragma unroll 1
+    for (uint32_t u = 0; u < ROW / 16; u++) {
+        const uint32_t x = at + (u ^ (lane & (ROW >= 128 ? 7u : 3u))) * 16;
+        uint32_t v[4];
+        asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(x) : "memory");
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            hit |= CT == PULSAR_TYPE_E4M3 ? __vcmpeq4(v[e] & ONES, ONES) : __vcmpeq2(v[e] & ONES, ONES);
+    }
+    const uint32_t odd = __ballot_sync(~0u, hit && (there >> lane & 1u));
+    if (odd >> lane & 1u)
+#pragma unroll 1
+        for (uint32_t u = 0; u < ROW / 16; u++)
+            asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(at + u * 16), "r"(0) : "memory");
+    __syncwarp();
+    return CK == 32 ? odd : odd & ((1u << (CK & 31)) - 1u);
+}
+
 /* the leading sum, plus the rest where the rest is a number: a key or value
  * of +-inf makes the lower parts' products NaN, the leading one's +-inf */
 __device__ __forceinline__ float pk_fold(float lead, float rest) { return isfinite(rest) ? lead + rest : lead; }
@@ -1028,8 +1053,26 @@ __global__ void __launch_bounds__(PK_WARPS * 32, pk_shape<CT, DP, R, QP>::OCC) p
                 }
             }
             const uint32_t vr = lane & 15u, vu = lane >> 4;
-            const uint32_t vx = (S::SPLIT ? turn(nullptr) : ka + CK * S::ROW) + vr * S::ROW +
-                                (S::ROW >= 128 ? vu ^ (vr & 7u) : vu ^ ((vr >> 1) & 3u)) * 16;
+            const uint32_t va = S::SPLIT ? turn(nullptr) : ka + CK * S::ROW;
+            const uint32_t vx = va + vr * S::ROW + (S::ROW >= 128 ? vu ^ (vr & 7u) : vu ^ ((vr >> 1) & 3u)) * 16;
+            if (J.A.n_q > 1) {
+                /* rows of several tokens: a value that is not a number, seen by some of them, would reach the
+                 * others as 0 * NaN.  Where the tile's spans end in this chunk, such values are taken out and
+                 * the rows that see them become NaN. */
+                bool edge = false;
+#pragma unroll
+                for (int y = 0; y < R; y++)
+                    edge |= v0 + y * 8 + g < J.rows && (key0 < slo[y] || key0 + CK > shi[y]);
+                if (__any_sync(~0u, edge)) {
+                    const uint32_t odd = pk_take_odd<CT, CK, S::ROW>(va, mask);
+#pragma unroll
+                    for (int y = 0; y < R; y++) {
+                        const int32_t a = slo[y] - key0, z = shi[y] - key0;
+                        const uint32_t from = a <= 0 ? ~0u : a >= 32 ? 0u : ~0u << a, to = z <= 0 ? 0u : z >= 32 ? ~0u : ~(~0u << z);
+                        if (odd & from & to) l[y] = __int_as_float(0x7fffffff);
+                    }
+                }
+            }
 #pragma unroll
             for (int kt = 0; kt < KT / 2; kt++)
 #pragma unroll

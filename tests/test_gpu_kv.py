@@ -193,6 +193,46 @@ def test_attend_extreme_scores(kv):
     assert torch.isnan(out[3]).all()
 
 
+@pytest.mark.parametrize("ct,H,n_kv,D,n_q,window", [(BF16, 4, 2, 128, 3, 0), (F16, 12, 1, 64, 4, 40), (E4M3, 8, 2, 80, 3, 0),
+                                                    (BF16, 3, 1, 256, 5, 33), (E4M3, 20, 2, 192, 2, 64), (F16, 2, 1, 192, 3, 0)])
+def test_drafts_do_not_share_their_faults(kv, ct, H, n_kv, D, n_q, window):
+    """NaN (e4m3: NaN, 16 bits: infinities too) in keys and values that only some of a sequence's new tokens see: the
+    others' outputs are what they are without"""
+    gen = torch.Generator(device="cuda").manual_seed(60)
+    lens, page = [70, 2, 200], 8
+    k, v, table = cache(lens, n_kv, D, page, ct, gen)
+    q = values((3, n_q, H, D), BF16, gen)
+    ks = torch.ones(n_kv, device="cuda") if ct == E4M3 else None
+    n = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    bad = torch.tensor([math.nan if ct == E4M3 else math.inf, math.nan], device="cuda").to(ct)
+    want = kv_ref.attend(q, k, v, table, lens, window=window, k_scale=ks, v_scale=ks)
+    sees = torch.ones((3, n_q), dtype=torch.bool)
+    for b, m in enumerate(lens):
+        spots = [m - 1]                                   # the last new token's own key
+        if window and m > window + n_q:
+            spots.append(m - n_q - window + 1)            # the first token's window begins there, the others' later
+        for x, j in enumerate(spots):
+            p, o = table[b, j // page].long(), j % page
+            for t in (k, v):
+                raw = t.view(torch.uint8) if ct == E4M3 else t
+                raw[p, :, o, 5 + x] = bad[x].view(torch.uint8) if ct == E4M3 else bad[x]
+        for i in range(n_q):
+            hi = m - (n_q - 1 - i)
+            lo = max(0, hi - window) if window else 0
+            sees[b, i] = any(lo <= j < hi for j in spots)
+    out = torch.zeros_like(q)
+    kv.PagedKv(k, v, table, ks, ks).attend(q, n, out, window=window)
+    got = out.cpu()
+    assert (~sees).any()
+    for b in range(3):
+        for i in range(n_q):
+            if sees[b, i]:
+                assert not torch.isfinite(got[b, i].float()).all(-1).any()
+            else:
+                w = tuple(z[b:b + 1, i:i + 1] for z in want)
+                held(got[b:b + 1, i:i + 1], None, w, BF16, ct, 200, D)
+
+
 def test_attend_past_32_bits(kv):
     """pages whose offsets pass 2^32 values, in a cache of 2^32 + values"""
     D, page, n_kv, H = 128, 64, 8, 16
