@@ -412,9 +412,19 @@ __global__ void __launch_bounds__(256) pk_fork_apply_kernel(pulsar_kv_pool P, co
 }
 
 /* A small fork in one launch: a cluster, whose first CTA plans, and which then
- * does both.  (2 x 4 beams over 8 slabs: 15.0 us in a stream against 17.4 in
- * two launches; 52 rows of 133 pages, whose tables want more SMs: 20.5 us on the device against 17.7.) */
+ * does both: it saves the host a launch and does the copies and tables slower.
+ * So it takes up to 32 rows, 512 table entries and 512 KB of copies.  Measured
+ * with a growth behind it, in a stream, one launch against two, us: 8 rows of
+ * 64 pages 10.1 / 12.8 without copies, 11.5 / 12.7 with 512 KB, 12.9 / 12.7 with 1 MB;
+ * 32 rows of 16 pages 10.2 / 12.8, 12.2 / 12.8, 13.3 / 12.6; 1024 entries and 512 KB:
+ * 8 rows 14.8 / 13.0, 32 rows 13.3 / 12.9; 2048 entries 16.0 / 12.7; 256 rows of 8 pages
+ * (in a graph, the fork alone) 21.1 / 8.8. */
 #define PK_CLUSTER 8
+#define PK_SMALL_ROWS 32u
+#define PK_SMALL_ENTRIES 512u
+#define PK_SMALL_BYTES (512u << 10)
+static_assert(4 * PK_MARKS + sizeof(pk_scan) + 64 + PK_SMALL_ROWS * PK_FORK_COLS * 4 <= 48 * 1024,
+              "a small fork needs no more shared memory than any kernel may have");
 __global__ void __cluster_dims__(PK_CLUSTER, 1, 1) __launch_bounds__(512)
     pk_fork_small_kernel(pulsar_kv_pool P, const int32_t *dst, const int32_t *src, uint32_t n, int32_t *status,
                          void *wsp, uint32_t *err) {
@@ -534,12 +544,12 @@ extern "C" int pulsar_kv_fork(const pulsar_kv_pool *p, const int32_t *dst, const
     if (!dst || !src || !n || n > p->n_rows || n > PULSAR_KV_MAX_FORK)
         return pk_refuse("kv fork: between 1 and min(n_rows, 4096) rows, each with a source");
     const uint32_t smem = n * PK_FORK_COLS * 4u;
-    if (!pm_smem_attr(pk_fork_apply_kernel, smem, &done)) return 0;
     const cudaStream_t st = pk_stream(stream);
-    /* one launch where a cluster is enough: at most 1 MB to copy, a table entry a thread */
-    if ((uint64_t)n * p->n_slab * p->page_bytes <= 1u << 20 && (uint64_t)n * p->max_pages <= 2048)
+    if (n <= PK_SMALL_ROWS && (uint64_t)n * p->max_pages <= PK_SMALL_ENTRIES &&
+        p->page_bytes <= PK_SMALL_BYTES && (uint64_t)n * p->n_slab * p->page_bytes <= PK_SMALL_BYTES)
         return pm_ok(pk_launch(pk_fork_small_kernel, PK_CLUSTER, 512, smem, st, *p, dst, src, n, status, ws, pk_err_word()),
                      "kv fork launch");
+    if (!pm_smem_attr(pk_fork_apply_kernel, smem, &done)) return 0;
     if (!pm_ok(pk_launch(pk_fork_plan_kernel, 1, PK_PLAN, 0, st, *p, dst, src, n, status, ws), "kv fork plan launch"))
         return 0;
     const uint32_t sms = pk_sm_count();

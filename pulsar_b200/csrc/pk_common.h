@@ -77,7 +77,9 @@ static cudaError_t pk_launch(void (*kernel)(P...), dim3 grid, dim3 block, uint32
     c.stream = st;
     c.attrs = &early;
     c.numAttrs = 1;
-    return cudaLaunchKernelEx(&c, kernel, (P)args...);
+    const cudaError_t e = cudaLaunchKernelEx(&c, kernel, (P)args...);
+    if (e != cudaSuccess) (void)cudaGetLastError(); /* the caller's next check of a launch is not about this one */
+    return e;
 }
 
 /* ------------------------------------------------------ values by type */

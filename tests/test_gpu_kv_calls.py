@@ -1,0 +1,49 @@
+"""Calls of the paged cache off the beaten track, against the model of the
+pages and the plain 64-bit forms."""
+import random
+
+import pytest
+
+import kv_ref
+from test_gpu_kv import F16, i32, same
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def kv():
+    from pulsar_b200 import kv as m
+    m.kv_error()
+    return m
+
+
+@pytest.mark.parametrize("n,width,layers", [(256, 4, 1), (507, 2, 1), (508, 2, 1), (600, 3, 1), (600, 2, 0), (1024, 2, 1),
+                                            (2048, 1, 1), (2048, 1, 0)])
+def test_turns_of_many_rows_of_few_pages(kv, n, width, layers):
+    """fork and free of up to 2048 rows at once, with slabs and without, against the model and by the pages' bytes"""
+    rng = random.Random(n + width + layers)
+    page, n_pages = 4, n * width + n
+    pool = kv.KvPool.empty(layers, n_pages, page, 1, 16, n, width, dtype=F16)
+    model = kv_ref.Pages(n, width, n_pages, page)
+    pool.data.copy_((torch.arange(n_pages, device="cuda") % 2000).to(F16).view(1, 1, -1, 1, 1, 1).expand_as(pool.data))
+    rows = list(range(n))
+    n_new = [rng.randint(0, width * page) for _ in rows]
+    assert model.grow(rows, n_new) == 0
+    pool.grow(i32(n_new))
+    for _ in range(2):
+        src = [-1 if rng.random() < 0.1 else rng.choice((r, rng.randrange(n))) for r in rows]
+        was = pool.data.clone()
+        st, copies = model.fork(src, rows)
+        assert st == 0
+        pool.fork(i32(src), i32(rows))
+        pool.check()
+        same(pool, model)
+        for a, b in copies:
+            was[:, :, b] = was[:, :, a]
+        assert torch.equal(pool.data, was)
+    assert model.fork([-1] * n, rows)[0] == 0
+    pool.free(i32(rows))
+    pool.check()
+    same(pool, model)
+    assert kv.kv_error() == 0
