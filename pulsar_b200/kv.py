@@ -294,6 +294,7 @@ class KvPool:
         self._ws = torch.empty(need, dtype=torch.uint8, device=self.device)
         self._where = self._ws.data_ptr(), need
         self._attend_ws = None
+        self._none = torch.full((n_rows,), -1, dtype=torch.int32, device=self.device)  # free()'s sources
         #: what the last grow, fork and compact did (pulsar_kv.h's status words)
         self.status = torch.zeros((3, 4), dtype=torch.int32, device=self.device)
         self._status = [self.status[i].data_ptr() for i in range(3)]
@@ -333,7 +334,9 @@ class KvPool:
 
     def free(self, rows: torch.Tensor, stream=None) -> None:
         """rows become empty"""
-        self.fork(torch.full_like(rows, -1), rows, stream)
+        if rows.numel() > self.n_rows:
+            raise KernelError("kv_free: more rows than the table has")
+        self.fork(self._none[:rows.numel()], rows, stream)
 
     def compact(self, stream=None) -> None:
         """live pages move to the low ids"""

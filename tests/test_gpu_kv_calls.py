@@ -47,3 +47,29 @@ def test_turns_of_many_rows_of_few_pages(kv, n, width, layers):
     pool.check()
     same(pool, model)
     assert kv.kv_error() == 0
+
+
+def allocations():
+    return torch.cuda.memory_stats()["allocation.all.allocated"]
+
+
+def test_free_on_another_stream(kv):
+    """rows freed on a stream of their own while the current one is busy, and without an allocation"""
+    pool = kv.KvPool.empty(1, 64, 4, 1, 16, 8, 8, dtype=F16)
+    model = kv_ref.Pages(8, 8, 64, 4)
+    side, n_new, gone = torch.cuda.Stream(), i32([5, 9, 1, 32, 4, 0, 7, 12]), i32([6, 1, 3])
+    pool.grow(n_new)
+    assert model.grow(list(range(8)), n_new.tolist()) == 0
+    torch.cuda.synchronize()
+    before = allocations()
+    torch.cuda._sleep(100_000_000)                       # some 50 ms
+    pool.free(gone, stream=side)
+    assert allocations() == before
+    side.synchronize()
+    assert model.fork([-1] * 3, [6, 1, 3])[0] == 0
+    same(pool, model)
+    pool.check()
+    # more rows than there are: refused, not read past the end
+    with pytest.raises(kv.KernelError):
+        pool.free(i32(list(range(8)) + [0]))
+    same(pool, model)
