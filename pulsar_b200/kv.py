@@ -294,10 +294,13 @@ class KvPool:
         self._ws = torch.empty(need, dtype=torch.uint8, device=self.device)
         self._where = self._ws.data_ptr(), need
         self._attend_ws = None
-        self._none = torch.full((n_rows,), -1, dtype=torch.int32, device=self.device)  # free()'s sources
+        self._none = torch.full((min(n_rows, MAX_FORK),), -1, dtype=torch.int32, device=self.device)  # free()'s sources
         #: what the last grow, fork and compact did (pulsar_kv.h's status words)
         self.status = torch.zeros((3, 4), dtype=torch.int32, device=self.device)
         self._status = [self.status[i].data_ptr() for i in range(3)]
+        # of a free() in pieces: those behind the first
+        self._more = torch.zeros((max(0, -(-n_rows // MAX_FORK) - 1), 4), dtype=torch.int32, device=self.device)
+        self._n_more = 0
 
     @classmethod
     def empty(cls, n_layer, n_pages, page_size, n_kv, head_dim, n_rows, max_pages, dtype=torch.bfloat16, device="cuda"):
@@ -323,20 +326,34 @@ class KvPool:
         check(self._lib.pulsar_kv_grow(self._p, r, _i32(n_new, n, self.device, "grow: n_new"), n, self._status[0],
                                        *self._where, _stream(stream, self._index)), "kv_grow")
 
-    def fork(self, src: torch.Tensor, dst: torch.Tensor, stream=None) -> None:
-        """row dst[i] becomes what row src[i] was (src -1: empty), all i at once"""
+    def _fork(self, src, dst, status, stream) -> None:
         n = src.numel()
-        if n == 0:
-            return
         check(self._lib.pulsar_kv_fork(self._p, _i32(dst, n, self.device, "fork: dst"),
-                                       _i32(src, n, self.device, "fork: src"), n, self._status[1], *self._where,
+                                       _i32(src, n, self.device, "fork: src"), n, status, *self._where,
                                        _stream(stream, self._index)), "kv_fork")
 
+    def fork(self, src: torch.Tensor, dst: torch.Tensor, stream=None) -> None:
+        """row dst[i] becomes what row src[i] was (src -1: empty), all i at once; at most 4096 (MAX_FORK) rows"""
+        if src.numel() == 0:
+            return
+        if src.numel() > MAX_FORK:
+            raise KernelError(f"kv_fork: more than {MAX_FORK} rows at once")
+        self._n_more = 0
+        self._fork(src, dst, self._status[1], stream)
+
     def free(self, rows: torch.Tensor, stream=None) -> None:
-        """rows become empty"""
-        if rows.numel() > self.n_rows:
+        """rows become empty; more than 4096 (MAX_FORK) go in pieces, each all or nothing by itself"""
+        n = rows.numel()
+        if n == 0:
+            return
+        if n > self.n_rows:
             raise KernelError("kv_free: more rows than the table has")
-        self.fork(self._none[:rows.numel()], rows, stream)
+        _i32(rows, n, self.device, "free: rows")
+        self._n_more = (n - 1) // MAX_FORK
+        for i in range(0, n, MAX_FORK):
+            piece = rows.view(-1)[i:i + MAX_FORK]
+            self._fork(self._none[:piece.numel()], piece,
+                       self._status[1] if i == 0 else self._more[i // MAX_FORK - 1].data_ptr(), stream)
 
     def compact(self, stream=None) -> None:
         """live pages move to the low ids"""
@@ -345,7 +362,8 @@ class KvPool:
 
     def check(self) -> None:
         """raise if the last grow, fork or compact was refused on the device (synchronous)"""
-        for name, s in zip(("grow", "fork", "compact"), self.status.tolist()):
+        rest = self._more[:self._n_more].tolist() if self._n_more else []
+        for name, s in zip(("grow", "fork", "compact") + ("fork",) * len(rest), self.status.tolist() + rest):
             if s[0]:
                 why = {1: "too few free pages", 2: "a row would outgrow its table"}.get(s[0], "invalid rows or lengths")
                 raise KernelError(f"kv_{name}: {why}")

@@ -73,3 +73,34 @@ def test_free_on_another_stream(kv):
     with pytest.raises(kv.KernelError):
         pool.free(i32(list(range(8)) + [0]))
     same(pool, model)
+
+
+def test_free_of_more_rows_than_a_fork_takes(kv):
+    """releases do not depend on one another: any number of rows is one call of free(); a fork says its limit"""
+    n = kv.MAX_FORK + 300
+    pool = kv.KvPool.empty(1, 3 * n, 2, 1, 16, n, 3, dtype=F16)
+    model = kv_ref.Pages(n, 3, 3 * n, 2)
+    rows = list(range(n))
+    n_new = [r % 6 for r in rows]
+    assert model.grow(rows, n_new) == 0
+    pool.grow(i32(n_new))
+    with pytest.raises(kv.KernelError, match=str(kv.MAX_FORK)):
+        pool.fork(i32(rows), i32(rows))
+    same(pool, model)
+    order = random.Random(3).sample(rows, n - 50)
+    for r in order:
+        assert model.fork([-1], [r])[0] == 0
+    pool.free(i32(order))
+    pool.check()
+    same(pool, model)
+    # what one piece refuses is told, whichever it is
+    for at in (5, kv.MAX_FORK + 5, n - 60):
+        bad = list(order)
+        bad[at] = n
+        pool.free(i32(bad))
+        with pytest.raises(kv.KernelError):
+            pool.check()
+        pool.free(i32(order))
+        pool.check()
+    same(pool, model)
+    assert kv.kv_error() == 0
