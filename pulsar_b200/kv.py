@@ -137,7 +137,9 @@ class PagedKv:
     strides whose head rows are contiguous and 16-byte aligned), bf16, f16 or
     float8_e4m3fn; table int32 [n_rows][max_pages].  k_scale, v_scale: f32
     [n_kv], e4m3 only.  ws: attend's workspace (workspace()), which any number
-    of layers share on one stream; without one the first attend() makes one.
+    of layers share on one stream; without one the object makes its own, on the
+    current stream, like any tensor (so that a call on another stream, or in a
+    capture, is ordered behind its zeros like behind the cache's bytes).
     An object serves one thread, and its workspace one stream, at a time."""
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, k_scale: torch.Tensor | None = None,
@@ -167,10 +169,8 @@ class PagedKv:
         self._desc, self._pdesc = d, ctypes.addressof(d)
         self._args, self._append = KvAttendArgs(), KvAppendArgs()
         self._pargs, self._pappend = ctypes.addressof(self._args), ctypes.addressof(self._append)
-        self._ws = None
-        if ws is not None:
-            self._take(ws)
         self._lib = lib()
+        self._take(self.workspace() if ws is None else ws)
         self._c_append, self._c_attend = self._lib.pulsar_kv_append, self._lib.pulsar_kv_attend
 
     def append(self, q, k, v, seq, pos, cos_sin, q_out, interleaved: bool = False, stream=None):
@@ -244,8 +244,6 @@ class PagedKv:
         if ws is not None:
             where = ws.data_ptr(), ws.numel()
         else:
-            if self._ws is None:
-                self._take(self.workspace())
             where = self._where
         if not self._c_attend(self._pdesc, self._pargs, *where, _stream(stream, self._index)):
             raise KernelError("kv_attend")
@@ -312,9 +310,7 @@ class KvPool:
     def layer(self, i: int, k_scale=None, v_scale=None) -> PagedKv:
         """layer i's cache; the layers share one attend workspace"""
         kv = PagedKv(self.data[i, 0], self.data[i, 1], self.table, k_scale, v_scale, self._attend_ws)
-        if self._attend_ws is None:
-            self._attend_ws = kv.workspace()
-            kv._take(self._attend_ws)
+        self._attend_ws = kv._ws
         return kv
 
     def grow(self, n_new: torch.Tensor, rows: torch.Tensor | None = None, stream=None) -> None:

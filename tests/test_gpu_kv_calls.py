@@ -5,7 +5,7 @@ import random
 import pytest
 
 import kv_ref
-from test_gpu_kv import F16, i32, same
+from test_gpu_kv import BF16, F16, cache, held, i32, same, values
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
@@ -103,4 +103,44 @@ def test_free_of_more_rows_than_a_fork_takes(kv):
         pool.free(i32(order))
         pool.check()
     same(pool, model)
+    assert kv.kv_error() == 0
+
+
+def test_first_attend_on_another_stream(kv):
+    """the first call of an object, with segments that several CTAs share, on a stream of its own while the current one
+    is busy, and in a capture that is not replayed before the next call: the bits of any other call"""
+    gen = torch.Generator(device="cuda").manual_seed(70)
+    lens, H, n_kv, D, page = [4000, 2500], 8, 2, 64, 16
+    k, v, table = cache(lens, n_kv, D, page, BF16, gen)
+    q, n = values((2, 1, H, D), BF16, gen), i32(lens)
+    first = torch.zeros_like(q)
+    c = kv.PagedKv(k, v, table)
+    c.attend(q, n, first)
+    held(first, None, kv_ref.attend(q, k, v, table, lens), BF16, BF16, max(lens), D)
+    size = c.workspace().numel()
+
+    def fresh():
+        used = torch.full((size,), 255, dtype=torch.uint8, device="cuda")  # what the allocator hands out next
+        del used
+        return kv.PagedKv(k, v, table)
+
+    side, out = torch.cuda.Stream(), torch.zeros_like(q)
+    c = fresh()
+    torch.cuda.synchronize()
+    torch.cuda._sleep(100_000_000)                       # some 50 ms
+    c.attend(q, n, out, stream=side)
+    side.synchronize()
+    assert torch.equal(out, first)
+    c, out, g = fresh(), torch.zeros_like(q), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        c.attend(q, n, out)
+    again = torch.zeros_like(q)
+    c.attend(q, n, again)
+    assert torch.equal(again, first)
+    g.replay()
+    assert torch.equal(out, first)
+    # layers of a pool share one
+    pool = kv.KvPool.empty(2, 4, 8, 1, 64, 2, 2)
+    a, b = pool.layer(0), pool.layer(1)
+    assert a._ws.data_ptr() == b._ws.data_ptr()
     assert kv.kv_error() == 0
