@@ -210,6 +210,10 @@ int pulsar_repack_q2k_tiles(void *dst, const void *src, uint32_t n_mat, uint32_t
 /* pulsar_rms_norm on an explicit stream (cudaStream_t, NULL = per-thread default) */
 int pulsar_rms_norm_stream(void *out, const void *x, const void *w, uint32_t n, uint32_t rows, float eps,
                            void *stream);
+/* pulsar_matmul_f32 and pulsar_add likewise */
+int pulsar_matmul_f32_stream(void *out, const void *w, const void *x, uint32_t in_dim, uint32_t out_dim,
+                             uint32_t n_tok, void *stream);
+int pulsar_add_stream(void *out, const void *a, const void *b, uint32_t n, void *stream);
 
 /* bytes of workspace pulsar_moe_layer needs for up to max_tok tokens */
 size_t pulsar_moe_layer_workspace(const pulsar_moe_layer_desc *d, uint32_t max_tok);

@@ -515,6 +515,14 @@ extern "C" int pulsar_add(void *out_dev, const void *a_dev, const void *b_dev, u
     return pm_ok(cudaGetLastError(), "add launch");
 }
 
+/* the same on an explicit stream (cudaStream_t, NULL = per-thread default) */
+extern "C" int pulsar_add_stream(void *out_dev, const void *a_dev, const void *b_dev, uint32_t n, void *stream) {
+    if (!out_dev || !a_dev || !b_dev || n == 0) return 0;
+    cudaStream_t st = stream ? (cudaStream_t)stream : cudaStreamPerThread;
+    pm_add_kernel<<<(n + 255) / 256, 256, 0, st>>>((float *)out_dev, (const float *)a_dev, (const float *)b_dev, n);
+    return pm_ok(cudaGetLastError(), "add launch");
+}
+
 /* kernel timeout / bad-argument word of the reference-ABI kernels: reads
  * it back (synchronously) and clears it; 0 = no error recorded */
 extern "C" uint32_t pulsar_b200_abi_error(void) {

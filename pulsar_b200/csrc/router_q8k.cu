@@ -286,13 +286,20 @@ int pm_launch_router_logits(float *logits, const float *w, const float *x, const
     return pm_launch_router_logits_q8(logits, w, x, lbias, n_expert, in_dim, n_tok, nullptr, nullptr, st);
 }
 
+/* pulsar_matmul_f32 on an explicit stream (cudaStream_t, NULL = per-thread default) */
+extern "C" int pulsar_matmul_f32_stream(void *out_dev, const void *w_dev, const void *x_dev, uint32_t in_dim,
+                                        uint32_t out_dim, uint32_t n_tok, void *stream) {
+    if (!out_dev || !w_dev || !x_dev || in_dim == 0 || out_dim == 0 || n_tok == 0) return 0;
+    cudaStream_t st = stream ? (cudaStream_t)stream : cudaStreamPerThread;
+    return pm_launch_router_logits((float *)out_dev, (const float *)w_dev, (const float *)x_dev, nullptr, out_dim,
+                                   in_dim, n_tok, st);
+}
+
 /* cu:6526 pulsar_matmul_f32: out[t][r] = W[r] . x[t], here in the fixed
  * f32 order above (deterministic) */
 extern "C" int pulsar_matmul_f32(void *out_dev, const void *w_dev, const void *x_dev, uint32_t in_dim,
                                  uint32_t out_dim, uint32_t n_tok) {
-    if (!out_dev || !w_dev || !x_dev || in_dim == 0 || out_dim == 0 || n_tok == 0) return 0;
-    return pm_launch_router_logits((float *)out_dev, (const float *)w_dev, (const float *)x_dev, nullptr, out_dim,
-                                   in_dim, n_tok, cudaStreamPerThread);
+    return pulsar_matmul_f32_stream(out_dev, w_dev, x_dev, in_dim, out_dim, n_tok, nullptr);
 }
 
 #include "pm_router.cuh"

@@ -71,9 +71,11 @@ class Decoder:
         return seq, first + torch.arange(total, dtype=torch.int32, device=dev)
 
     def forward(self, x: torch.Tensor, seq: torch.Tensor, pos: torch.Tensor, trace: list | None = None) -> torch.Tensor:
-        """the last layer's rows of new tokens x [T][n_embd] (f32) at pos[t] of sequence seq[t]; trace collects each
-        layer's (input, attention's output, row between the halves, output)"""
+        """the last layer's rows of new tokens x [T][n_embd] (f32) at pos[t] of sequence seq[t], on torch's current
+        stream (and so in a capture, behind one call outside it); trace collects each layer's (input, attention's
+        output, row between the halves, output)"""
         s, T, dev = self.spec, x.shape[0], x.device
+        st = torch.cuda.current_stream()
         q, kv, h = s.n_head * s.head_dim, s.n_kv * s.head_dim, s.moe.n_embd
         n, y = torch.empty_like(x), torch.empty_like(x)
         qkv = torch.empty((T, q + 2 * kv), dtype=torch.float32, device=dev)
@@ -85,11 +87,11 @@ class Decoder:
         for i in range(s.n_layer):
             mid, out = torch.empty_like(x), torch.empty_like(x)
             rms_norm(n, x)
-            matmul_f32(qkv, self.wqkv[i], n, h, q + 2 * kv, T)
+            matmul_f32(qkv, self.wqkv[i], n, h, q + 2 * kv, T, st)
             self.caches[i].append(qx, kx, vx, seq, pos, self.cos_sin, turned, s.interleaved)
             self.caches[i].attend(turned, seen, a, window=s.window, seq=seq)
-            matmul_f32(y, self.wo[i], a, q, h, T)
-            add(mid, x, y, T * h)
+            matmul_f32(y, self.wo[i], a, q, h, T, st)
+            add(mid, x, y, T * h, st)
             rms_norm(n, mid)
             self.moe[i].forward(n, out, ws, residual=mid)
             if trace is not None:

@@ -83,16 +83,17 @@ def add_bias_rows(x, bias, dim, rows):
     check(lib().pulsar_add_bias_rows(ptr(x), ptr(bias), dim, rows), "add_bias_rows")
 
 
-def matmul_f32(out, w, x, in_dim, out_dim, n_tok):
-    check(lib().pulsar_matmul_f32(ptr(out), ptr(w), ptr(x), in_dim, out_dim, n_tok), "matmul_f32")
+def matmul_f32(out, w, x, in_dim, out_dim, n_tok, stream=None):
+    check(lib().pulsar_matmul_f32_stream(ptr(out), ptr(w), ptr(x), in_dim, out_dim, n_tok,
+                                         None if stream is None else stream.cuda_stream), "matmul_f32")
 
 
 def swiglu(out, gate, up, n, clamp=0.0, weight=1.0, act_op=0):
     check(lib().pulsar_swiglu(ptr(out), ptr(gate), ptr(up), n, clamp, weight, act_op), "swiglu")
 
 
-def add(out, a, b, n):
-    check(lib().pulsar_add(ptr(out), ptr(a), ptr(b), n), "add")
+def add(out, a, b, n, stream=None):
+    check(lib().pulsar_add_stream(ptr(out), ptr(a), ptr(b), n, None if stream is None else stream.cuda_stream), "add")
 
 
 def rms_norm(out, x, w=None, eps=1e-6, stream=None):

@@ -1,0 +1,66 @@
+"""The decoder example off the beaten track."""
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def make():
+    import pulsar_b200 as p
+    from pulsar_b200.decoder import Decoder, DecoderSpec
+    moe = p.LayerSpec(n_embd=256, n_ff=256, n_expert=8, n_used=2, quant=p.QUANT_Q4_K)
+
+    def f(n_pages=0, max_tokens=96, **kw):
+        spec = dict(moe=moe, n_layer=2, n_head=8, n_kv=2, head_dim=32, cache=torch.float16, page_size=8)
+        spec.update(kw)
+        return Decoder(DecoderSpec(**spec), n_rows=6, max_tokens=max_tokens, seed=3, n_pages=n_pages)
+    return f
+
+
+def hidden(n, seed):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return torch.randn((n, 256), generator=g, device="cuda")
+
+
+def test_on_a_stream_and_in_a_capture(make):
+    """prompt, decode steps and a fork on a stream of their own while the default one is busy, and a decode step captured
+    and replayed: the bits of the same calls on the default stream"""
+    def run(d, between):
+        outs = [d.forward(hidden(19, 1), *d.extend([2], [19]))]
+        between()
+        outs.append(d.forward(hidden(31, 2), *d.extend([2, 0], [1, 30])))
+        d.pool.fork(torch.tensor([2, 2], dtype=torch.int32, device="cuda"), torch.tensor([1, 4], dtype=torch.int32, device="cuda"))
+        outs.append(d.forward(hidden(3, 3), *d.extend([1, 2, 4], [1, 1, 1])))
+        return outs
+
+    want = run(make(), lambda: None)
+    d, side = make(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        got = run(d, lambda: torch.cuda.default_stream().synchronize())
+    side.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+    x = hidden(3, 4)
+    torch.cuda.synchronize()
+    torch.cuda._sleep(100_000_000)                       # the default stream is busy for some 50 ms
+    with torch.cuda.stream(side):
+        seq, pos = d.extend([1, 2, 4], [1, 1, 1])
+        a = d.forward(x, seq, pos)
+    side.synchronize()
+    # the same step (its keys and values are written again) in a graph
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        b = d.forward(x, seq, pos)
+    for new in (x.clone(), hidden(3, 5)):
+        x.copy_(new)
+        b.zero_()
+        g.replay()
+        with torch.cuda.stream(side):
+            side.wait_stream(torch.cuda.default_stream())
+            c = d.forward(x, seq, pos)
+        torch.cuda.synchronize()
+        assert torch.equal(b, c)
+        if torch.equal(new, hidden(3, 4)):
+            assert torch.equal(a, b)
+    d.pool.check()
