@@ -59,7 +59,9 @@ class Decoder:
             self.wo.append(torch.randn((h, q), generator=g, device=dev) * q ** -0.5)
 
     def extend(self, rows: list[int], n_new: list[int]):
-        """room for n_new[i] more tokens of sequence rows[i]; (seq, pos) of all new tokens, int32 [sum(n_new)]"""
+        """room for n_new[i] more tokens of sequence rows[i]; (seq, pos) of all new tokens, int32 [sum(n_new)].  Where
+        the pool has no room for all of them no sequence grows and every position is -1, which makes the tokens
+        padding: forward() writes no cache for them (pool.check() raises)."""
         dev = self.pool.device
         r = torch.tensor(rows, dtype=torch.int32, device=dev)
         n = torch.tensor(n_new, dtype=torch.int32, device=dev)
@@ -68,7 +70,8 @@ class Decoder:
         seq = torch.repeat_interleave(r, n.long(), output_size=total)
         first = torch.repeat_interleave(self.pool.lens[r.long()] - n.cumsum(0, dtype=torch.int32), n.long(),
                                         output_size=total)
-        return seq, first + torch.arange(total, dtype=torch.int32, device=dev)
+        pos = first + torch.arange(total, dtype=torch.int32, device=dev)
+        return seq, torch.where(self.pool.status[0, 0] == 0, pos, -1)  # growth's status, on the device
 
     def forward(self, x: torch.Tensor, seq: torch.Tensor, pos: torch.Tensor, trace: list | None = None) -> torch.Tensor:
         """the last layer's rows of new tokens x [T][n_embd] (f32) at pos[t] of sequence seq[t], on torch's current

@@ -64,3 +64,28 @@ def test_on_a_stream_and_in_a_capture(make):
         if torch.equal(new, hidden(3, 4)):
             assert torch.equal(a, b)
     d.pool.check()
+
+
+def test_refused_growth_touches_no_cache(make):
+    """too few free pages, and rows past their table: the new tokens are padding, and no byte of any sequence's keys and
+    values changes; the next growth that has room goes on where the sequence ended"""
+    from pulsar_b200 import KernelError
+    d, free = make(n_pages=5), make()
+    beams = torch.tensor([1, 1], dtype=torch.int32, device="cuda"), torch.tensor([0, 3], dtype=torch.int32, device="cuda")
+    for x in (d, free):                                  # 2 full pages shared by three beams, 3 pages of their own
+        x.forward(hidden(21, 1), *x.extend([1], [21]))
+        x.pool.fork(*beams)
+        x.pool.check()
+    was, lens = d.pool.data.clone(), d.pool.lens.clone()
+    for rows, n_new in (([0, 1, 3], [1, 4, 2]), ([1], [90])):
+        seq, pos = d.extend(rows, n_new)
+        assert pos.tolist() == [-1] * sum(n_new)
+        trace = []
+        d.forward(hidden(sum(n_new), 2), seq, pos, trace)
+        with pytest.raises(KernelError):
+            d.pool.check()
+        assert torch.equal(d.pool.data, was) and torch.equal(d.pool.lens, lens)
+        assert all((a == 0).all() for _, a, _, _ in trace)
+    same = [x.forward(hidden(3, 4), *x.extend([0, 1, 3], [1, 1, 1])) for x in (d, free)]
+    d.pool.check()
+    assert torch.equal(*same)
