@@ -48,7 +48,8 @@ class Decoder:
         self.pool = KvPool.empty(s.n_layer, n_pages or n_rows * width, s.page_size, s.n_kv, s.head_dim, n_rows, width,
                                  s.cache, dev)
         self.caches = [self.pool.layer(i) for i in range(s.n_layer)]
-        self.cos_sin = rope_table(max_tokens, s.head_dim if s.rot_dim is None else s.rot_dim, s.rope_base,
+        # a row holds whole pages, and each of their tokens has its angles
+        self.cos_sin = rope_table(width * s.page_size, s.head_dim if s.rot_dim is None else s.rot_dim, s.rope_base,
                                   s.rope_scaling, dev)
         self.moe = [make_layer(s.moe, seed * 1009 + i, dev) for i in range(s.n_layer)]
         self.wqkv, self.wo = [], []

@@ -89,3 +89,15 @@ def test_refused_growth_touches_no_cache(make):
     same = [x.forward(hidden(3, 4), *x.extend([0, 1, 3], [1, 1, 1])) for x in (d, free)]
     d.pool.check()
     assert torch.equal(*same)
+
+
+def test_rows_reach_the_end_of_their_pages(make):
+    """max_tokens that is no multiple of the page: a row holds whole pages, and every token of them has its angles"""
+    from pulsar_b200 import kv_error
+    kv_error()
+    short, whole = make(max_tokens=20), make(max_tokens=24)
+    a, b = (x.forward(hidden(24, 5), *x.extend([2], [24])) for x in (short, whole))
+    assert kv_error() == 0
+    short.pool.check()
+    assert torch.equal(a, b)
+    assert torch.equal(short.pool.data[:, :, short.pool.table[2, :3].long()], whole.pool.data[:, :, whole.pool.table[2, :3].long()])
