@@ -115,7 +115,7 @@ def rope_table(n_pos: int, rot_dim: int, base: float = 10000.0, scaling: dict | 
             return half * math.log(trained / (2 * math.pi * turns)) / math.log(base)
 
         lo = max(math.floor(pair_of(scaling.get("fast", 32.0))), 0)
-        hi = min(math.ceil(pair_of(scaling.get("slow", 1.0))), half - 1)
+        hi = min(math.ceil(pair_of(scaling.get("slow", 1.0))), rot_dim - 1)  # behind the last pair, where none turns so slowly
         ramp = ((i - lo) / max(hi - lo, 1e-3)).clamp(0.0, 1.0)
         f = f * (1.0 - ramp) + f / s * ramp
         mul = float(scaling.get("mscale", 1.0 + 0.1 * math.log(s) if s > 1 else 1.0))
