@@ -81,9 +81,9 @@ __global__ void __launch_bounds__(256, V == 8 && !NEAR && HU > 1 ? 3 : 4) /* 64 
     const uint32_t step = gridDim.y * blockDim.y;
     uint32_t t = blockIdx.y * blockDim.y + threadIdx.y;
     int32_t pos = -1, seq = -1;
-    if (t < A.n_tok) {
-        pos = __ldg(A.pos + t);
-        seq = __ldg(A.seq + t);
+    if (t < A.n_tok) { /* plain loads: a kernel that this one overlapped may have written them (a pool's lengths) */
+        pos = A.pos[t];
+        seq = A.seq[t];
     }
     while (t < A.n_tok) {
         /* the values wait for nothing, angles and page for the position, which came a token ahead */
@@ -102,8 +102,8 @@ __global__ void __launch_bounds__(256, V == 8 && !NEAR && HU > 1 ? 3 : 4) /* 64 
         const bool more = A.n_tok - t > step;
         t = more ? t + step : A.n_tok;
         if (more) {
-            pos = __ldg(A.pos + t);
-            seq = __ldg(A.seq + t);
+            pos = A.pos[t];
+            seq = A.seq[t];
         }
         if (p >= 0 && A.rot_dim && (uint32_t)p >= A.n_pos) { /* no angles: nothing of the token is written */
             atomicOr(err, PULSAR_KV_ERR_SPAN);

@@ -144,3 +144,35 @@ def test_first_attend_on_another_stream(kv):
     a, b = pool.layer(0), pool.layer(1)
     assert a._ws.data_ptr() == b._ws.data_ptr()
     assert kv.kv_error() == 0
+
+
+def test_lengths_as_positions_of_an_overlapped_call(kv):
+    """the pool's lengths, which a growth just wrote, as the positions of the next append, nothing between them: every
+    token is where the same calls put it with the device waited for"""
+    rows, page, n_kv, D, steps = 48, 8, 2, 64, 30
+    gen = torch.Generator(device="cuda").manual_seed(71)
+    x = values((steps, rows, 2 * n_kv * D), BF16, gen)
+    cut = [[z.unflatten(1, (-1, D)) for z in x[t].split(n_kv * D, 1)] for t in range(steps)]
+    ids, one = i32(list(range(rows))), i32([1] * rows)
+    cs = kv.rope_table(steps + 2, D)
+
+    def run(wait):
+        pool = kv.KvPool.empty(1, rows * 4, page, n_kv, D, rows, 4)
+        pool.grow(i32([4 * page] * rows))
+        count = kv.KvPool.empty(0, rows * 4, page, n_kv, D, rows, 4)  # whose lengths are the positions
+        layer = pool.layer(0)
+        torch.cuda.synchronize()
+        for t in range(steps):
+            for f in (lambda: count.grow(one, ids), lambda: layer.append(None, *cut[t], ids, count.lens, cs, None)):
+                f()
+                if wait:
+                    torch.cuda.synchronize()
+        torch.cuda.synchronize()
+        assert count.lens.tolist() == [steps] * rows
+        return pool
+
+    a, b = run(True), run(False)
+    assert torch.equal(a.data, b.data) and kv.kv_error() == 0
+    # token t of the calls is at position t + 1
+    v = torch.stack([a.data[0, 1, a.table[:, (t + 1) // page].long(), :, (t + 1) % page] for t in range(steps)])
+    assert torch.equal(v, torch.stack([c[1] for c in cut]))
