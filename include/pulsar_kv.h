@@ -30,7 +30,7 @@ extern "C" {
 #define PULSAR_TYPE_E4M3 3u /* caches only */
 
 /* error word bits */
-#define PULSAR_KV_ERR_PAGE 1u /* a page id outside [0, n_pages) */
+#define PULSAR_KV_ERR_PAGE 1u /* a page id outside [0, n_pages); compact: a page that no count holds, behind the live ones */
 #define PULSAR_KV_ERR_SPAN 2u /* a length or position past the table's width or the position table's end */
 #define PULSAR_KV_ERR_ROW 4u  /* a table row outside [0, n_rows) */
 

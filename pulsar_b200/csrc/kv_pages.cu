@@ -452,6 +452,7 @@ __global__ void __launch_bounds__(PK_PLAN) pk_compact_plan_kernel(pulsar_kv_pool
     const uint32_t live = pk_choose(P.refs, 0, P.n_pages, true, scan, none, [](uint32_t, uint32_t) {});
     const uint32_t moves = pk_choose(P.refs, 0, live, false, scan, every,
                                      [&](uint32_t page, uint32_t rank) { to[rank] = (int32_t)page; });
+    for (uint32_t p = live + threadIdx.x; p < P.n_pages; p += PK_PLAN) map[p] = -1; /* but for the pages that move */
     __syncthreads();
     pk_choose(P.refs, live, P.n_pages, true, scan, every, [&](uint32_t page, uint32_t rank) {
         from[rank] = (int32_t)page;
@@ -491,10 +492,10 @@ __global__ void __launch_bounds__(256) pk_compact_apply_kernel(pulsar_kv_pool P,
         for (uint32_t c = lane; c < pk_ceil(len, P.page_size); c += 32) {
             const int32_t e = row[c];
             if ((uint32_t)e >= P.n_pages) atomicOr(err, PULSAR_KV_ERR_PAGE);
-            /* a page that no reference count holds is not in the map */
             else if ((uint32_t)e >= live) {
                 const int32_t m = map[e];
-                if ((uint32_t)m < live) row[c] = m;
+                if (m >= 0) row[c] = m;
+                else atomicOr(err, PULSAR_KV_ERR_PAGE); /* a page that no reference count holds */
             }
         }
     }

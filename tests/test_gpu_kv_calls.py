@@ -176,3 +176,21 @@ def test_lengths_as_positions_of_an_overlapped_call(kv):
     # token t of the calls is at position t + 1
     v = torch.stack([a.data[0, 1, a.table[:, (t + 1) // page].long(), :, (t + 1) % page] for t in range(steps)])
     assert torch.equal(v, torch.stack([c[1] for c in cut]))
+
+
+def test_compaction_leaves_pages_that_no_count_holds(kv):
+    """a table entry of a page with a zero count is not in the plan's map: it stays and is told, whatever the workspace
+    held before"""
+    for fill in (0, 1, -1, 7):
+        pool = kv.KvPool.empty(1, 16, 2, 1, 16, 3, 4, dtype=F16)
+        pool.grow(i32([4, 4, 4]))
+        pool.free(i32([0]))
+        assert pool.table[2, :2].tolist() == [4, 5]
+        pool.refs[5] = 0
+        pool._ws[:pool._ws.numel() // 4 * 4].view(torch.int32).fill_(fill)
+        pool.compact()
+        pool.check()
+        # pages 2, 3, 4 are live: 3 and 4 move to 0 and 1
+        assert pool.table[1, :2].tolist() == [2, 0] and pool.table[2, :2].tolist() == [1, 5]
+        assert pool.refs.tolist() == [1, 1, 1] + [0] * 13
+        assert kv.kv_error() == kv.ERR_PAGE and kv.kv_error() == 0
