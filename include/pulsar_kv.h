@@ -95,7 +95,8 @@ int pulsar_kv_append(const pulsar_kv_desc *d, const pulsar_kv_append_args *a, vo
  * token's span have no influence, whatever their bytes are; an infinite or
  * NaN score or value that is seen gives what the formula gives, or NaN.  (Where
  * a value that some of a sequence's n_q tokens see and others do not is
- * infinite or NaN, the outputs of those that see it are NaN throughout.)
+ * infinite or NaN, the outputs of those that see it are NaN throughout; lse,
+ * which no value enters, is what the formula gives.)
  * ws: pulsar_kv_attend_workspace bytes (with a NULL: enough for any
  * arguments over this cache), aligned to 16; its first PULSAR_KV_WS_ZEROED bytes
  * are zero before the first call and are zero again after every call.  One

@@ -1058,7 +1058,8 @@ __global__ void __launch_bounds__(PK_WARPS * 32, pk_shape<CT, DP, R, QP>::OCC) p
             if (J.A.n_q > 1) {
                 /* rows of several tokens: a value that is not a number, seen by some of them, would reach the
                  * others as 0 * NaN.  Where the tile's spans end in this chunk, such values are taken out and
-                 * the rows that see them become NaN. */
+                 * a weight of the rows that see them becomes NaN, and with it their outputs (not their sums of
+                 * weights, which make the lse). */
                 bool edge = false;
 #pragma unroll
                 for (int y = 0; y < R; y++)
@@ -1069,7 +1070,7 @@ __global__ void __launch_bounds__(PK_WARPS * 32, pk_shape<CT, DP, R, QP>::OCC) p
                     for (int y = 0; y < R; y++) {
                         const int32_t a = slo[y] - key0, z = shi[y] - key0;
                         const uint32_t from = a <= 0 ? ~0u : a >= 32 ? 0u : ~0u << a, to = z <= 0 ? 0u : z >= 32 ? ~0u : ~(~0u << z);
-                        if (odd & from & to) l[y] = __int_as_float(0x7fffffff);
+                        if (odd & from & to) pa[0][y] = 0x7fff7fffu; /* two NaN weights of row 8 y + g, in either type */
                     }
                 }
             }

@@ -1,11 +1,12 @@
 """Calls of the paged cache off the beaten track, against the model of the
 pages and the plain 64-bit forms."""
+import math
 import random
 
 import pytest
 
 import kv_ref
-from test_gpu_kv import BF16, F16, cache, held, i32, same, values
+from test_gpu_kv import BF16, E4M3, F16, cache, held, i32, same, values
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
@@ -194,3 +195,41 @@ def test_compaction_leaves_pages_that_no_count_holds(kv):
         assert pool.table[1, :2].tolist() == [2, 0] and pool.table[2, :2].tolist() == [1, 5]
         assert pool.refs.tolist() == [1, 1, 1] + [0] * 13
         assert kv.kv_error() == kv.ERR_PAGE and kv.kv_error() == 0
+
+
+@pytest.mark.parametrize("ct,H,n_kv,D,n_q,window", [(BF16, 4, 2, 128, 3, 0), (F16, 12, 1, 64, 4, 40), (E4M3, 8, 2, 80, 3, 0),
+                                                    (BF16, 3, 1, 256, 5, 33), (E4M3, 20, 2, 192, 2, 64), (F16, 2, 1, 192, 3, 0)])
+def test_lse_does_not_depend_on_the_values(kv, ct, H, n_kv, D, n_q, window):
+    """NaN and infinite values (not keys) that some drafts of a sequence see: the outputs of those are not numbers, the
+    others' and every lse are the formula's"""
+    gen = torch.Generator(device="cuda").manual_seed(61)
+    lens, page = [70, 2, 200, 3000], 8
+    k, v, table = cache(lens, n_kv, D, page, ct, gen)
+    q = values((len(lens), n_q, H, D), BF16, gen)
+    ks = torch.ones(n_kv, device="cuda") if ct == E4M3 else None
+    want = kv_ref.attend(q, k, v, table, lens, window=window, k_scale=ks, v_scale=ks)
+    raw = v.view(torch.uint8) if ct == E4M3 else v
+    bad = torch.tensor([math.nan if ct == E4M3 else math.inf, math.nan], device="cuda").to(ct)
+    sees = torch.ones((len(lens), n_q), dtype=torch.bool)
+    for b, m in enumerate(lens):
+        spots = [m - 1]                                   # the last new token's own key
+        if window and m > window + n_q:
+            spots.append(m - n_q - window + 1)            # the first token's window begins there, the others' later
+        for x, j in enumerate(spots):
+            raw[table[b, j // page].long(), :, j % page, 5 + x] = bad[x].view(torch.uint8) if ct == E4M3 else bad[x]
+        for i in range(n_q):
+            hi = m - (n_q - 1 - i)
+            lo = max(0, hi - window) if window else 0
+            sees[b, i] = any(lo <= j < hi for j in spots)
+    out, lse = torch.zeros_like(q), torch.zeros((len(lens), n_q, H), device="cuda")
+    kv.PagedKv(k, v, table, ks, ks).attend(q, i32(lens), out, window=window, lse=lse)
+    got, seen_lse = out.cpu(), lse.cpu()
+    for b in range(len(lens)):
+        for i in range(n_q):
+            w = tuple(z[b:b + 1, i:i + 1] for z in want)
+            if sees[b, i]:
+                assert torch.isnan(got[b, i].float()).any(-1).all()
+                held(w[0].to(BF16), seen_lse[b:b + 1, i:i + 1], w, BF16, ct, max(lens), D)
+            else:
+                held(got[b:b + 1, i:i + 1], seen_lse[b:b + 1, i:i + 1], w, BF16, ct, max(lens), D)
+    assert kv.kv_error() == 0
