@@ -242,7 +242,7 @@ class PagedKv:
         a.scale = D ** -0.5 if scale is None else scale
         a.n_rows, a.n_q, a.n_head, a.window, a.q_type = n, n_q, n_head, window, kind
         if ws is not None:
-            where = ws.data_ptr(), ws.numel()
+            where = self._bytes(ws)
         else:
             where = self._where
         if not self._c_attend(self._pdesc, self._pargs, *where, _stream(stream, self._index)):
@@ -255,10 +255,13 @@ class PagedKv:
         _need(n > 0, "PagedKv: shape refused")
         return torch.zeros(n, dtype=torch.uint8, device=self.device)
 
-    def _take(self, ws: torch.Tensor) -> None:
+    def _bytes(self, ws: torch.Tensor):
         _need(ws.dtype == torch.uint8 and ws.device == self.device and ws.is_contiguous(),
               "PagedKv: a workspace is contiguous bytes beside the cache")
-        self._ws, self._where = ws, (ws.data_ptr(), ws.numel())
+        return ws.data_ptr(), ws.numel()
+
+    def _take(self, ws: torch.Tensor) -> None:
+        self._ws, self._where = ws, self._bytes(ws)
 
 
 # ------------------------------------------------------------------ all layers

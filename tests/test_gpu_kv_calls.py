@@ -233,3 +233,25 @@ def test_lse_does_not_depend_on_the_values(kv, ct, H, n_kv, D, n_q, window):
             else:
                 held(got[b:b + 1, i:i + 1], seen_lse[b:b + 1, i:i + 1], w, BF16, ct, max(lens), D)
     assert kv.kv_error() == 0
+
+
+def test_workspaces_that_are_refused(kv):
+    """attend's ws, given with the call: bytes beside the cache, as the object's own"""
+    gen = torch.Generator(device="cuda").manual_seed(72)
+    k, v, table = cache([20, 9], 2, 64, 8, BF16, gen)
+    c, n, q = kv.PagedKv(k, v, table), i32([20, 9]), values((2, 4, 64), BF16, gen)
+    out, size = torch.zeros_like(q), kv.PagedKv(k, v, table).workspace().numel()
+    for ws in (torch.zeros(size, dtype=torch.uint8), torch.zeros(size, dtype=torch.uint8).pin_memory(),
+               torch.zeros(size, device="cuda"), torch.zeros(2 * size, dtype=torch.uint8, device="cuda")[::2]):
+        with pytest.raises(ValueError):
+            c.attend(q, n, out, ws=ws)
+        with pytest.raises(ValueError):
+            kv.PagedKv(k, v, table, ws=ws)
+    assert (out == 0).all()
+    want = torch.zeros_like(q)
+    c.attend(q, n, want)
+    c.attend(q, n, out, ws=c.workspace())
+    assert torch.equal(out, want)
+    # a zeroed one at an address that is no multiple of 16 is the library's to refuse
+    with pytest.raises(kv.KernelError):
+        c.attend(q, n, out, ws=torch.zeros(size + 8, dtype=torch.uint8, device="cuda")[8:])
