@@ -32,8 +32,9 @@ def kv_error() -> int:
     return int(lib().pulsar_kv_error())
 
 
-_device = torch._C._cuda_getDevice
-_raw_stream = torch._C._cuda_getCurrentRawStream  # current_stream() builds an object: 3 us a call
+# current_stream() builds an object: 3 us a call.  (A torch without CUDA has neither; nor can it make a cache.)
+_device = getattr(torch._C, "_cuda_getDevice", None)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 def _need(ok: bool, what: str) -> None:

@@ -1,9 +1,13 @@
-"""The paged cache's host side without a GPU: rotary tables."""
+"""The paged cache's host side without a GPU: rotary tables, the package's import."""
 import math
+import os
+import subprocess
+import sys
 
 import pytest
 
 torch = pytest.importorskip("torch")
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 
 @pytest.mark.parametrize("rot,base,trained,factor", [(64, 10000.0, 131072, 4.0), (64, 10000.0, 65536, 16.0),
@@ -26,3 +30,15 @@ def test_yarn_blends_as_published(rot, base, trained, factor):
         ramp = min(max((i - lo) / (hi - lo), 0.0), 1.0)
         want = f * (1 - ramp) + f / factor * ramp
         assert abs(float(got[i]) - want) <= 2.0 ** -22 * want, (i, float(got[i]), want)
+
+
+def test_package_imports_beside_a_torch_without_cuda():
+    """a torch built for the CPU has no CUDA bindings: the package, the layer builder's host side and the rotary tables
+    need none"""
+    code = ("import torch\n"
+            "for n in [n for n in dir(torch._C) if n.startswith('_cuda_')]: delattr(torch._C, n)\n"
+            "import pulsar_b200\n"
+            "assert pulsar_b200.row_bytes(pulsar_b200.QUANT_Q4_K, 256) == 144\n"
+            "assert pulsar_b200.rope_table(4, 8, device='cpu').shape == (4, 2, 4)\n")
+    r = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr[-2000:]
