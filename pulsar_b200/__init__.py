@@ -8,10 +8,11 @@ runs both (decoder.py).
 """
 from ._lib import (LIB_PATH, QUANT_IQ2_XXS, QUANT_MXFP4, QUANT_Q2_K, QUANT_Q4_K, QUANT_Q8_0, QUANTS, ExpertPtrs,
                    KernelError, LayerDesc, abi_error, build, lib, row_bytes)
+from .decoder import Decoder, DecoderSpec
+from .kv import KvPool, PagedKv, kv_error, rope_table
 from .layer import LayerSpec, MoeLayer, make_layer, seeded_hidden
 
 __all__ = ["LIB_PATH", "QUANT_IQ2_XXS", "QUANT_MXFP4", "QUANT_Q2_K", "QUANT_Q4_K", "QUANT_Q8_0", "QUANTS",
            "ExpertPtrs", "KernelError", "LayerDesc", "abi_error", "build", "lib", "row_bytes", "LayerSpec",
-           "MoeLayer", "make_layer", "seeded_hidden"]
-from .kv import KvPool, PagedKv, kv_error, rope_table
-from .decoder import Decoder, DecoderSpec
+           "MoeLayer", "make_layer", "seeded_hidden", "KvPool", "PagedKv", "kv_error", "rope_table", "Decoder",
+           "DecoderSpec"]

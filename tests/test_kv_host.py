@@ -42,3 +42,11 @@ def test_package_imports_beside_a_torch_without_cuda():
             "assert pulsar_b200.rope_table(4, 8, device='cpu').shape == (4, 2, 4)\n")
     r = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True)
     assert r.returncode == 0, r.stderr[-2000:]
+
+
+def test_star_import_has_the_cache():
+    import pulsar_b200
+    from pulsar_b200 import decoder, kv
+    for m in (kv, decoder):
+        for n in ("KvPool", "PagedKv", "kv_error", "rope_table") if m is kv else ("Decoder", "DecoderSpec"):
+            assert n in pulsar_b200.__all__ and getattr(pulsar_b200, n) is getattr(m, n)
