@@ -81,6 +81,11 @@ class Decoder:
         s, T, dev = self.spec, x.shape[0], x.device
         st = torch.cuda.current_stream()
         q, kv, h = s.n_head * s.head_dim, s.n_kv * s.head_dim, s.moe.n_embd
+        if x.shape != (T, h) or x.dtype != torch.float32 or dev != self.pool.device or not x.is_contiguous():
+            raise ValueError(f"Decoder: x is f32 [T][{h}], contiguous, beside the cache")
+        for t in (seq, pos):
+            if t.shape != (T,) or t.dtype != torch.int32 or t.device != dev or not t.is_contiguous():
+                raise ValueError("Decoder: seq and pos are int32 [T], contiguous, beside the cache")
         n, y = torch.empty_like(x), torch.empty_like(x)
         qkv = torch.empty((T, q + 2 * kv), dtype=torch.float32, device=dev)
         turned = torch.empty((T, s.n_head, s.head_dim), dtype=torch.float32, device=dev)

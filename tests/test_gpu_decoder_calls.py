@@ -101,3 +101,17 @@ def test_rows_reach_the_end_of_their_pages(make):
     short.pool.check()
     assert torch.equal(a, b)
     assert torch.equal(short.pool.data[:, :, short.pool.table[2, :3].long()], whole.pool.data[:, :, whole.pool.table[2, :3].long()])
+
+
+def test_refusals(make):
+    """rows and positions of another type, width or place: refused before any launch"""
+    d = make()
+    seq, pos = d.extend([1], [5])
+    x, was = hidden(5, 1), d.pool.data.clone()
+    for a in ((x.bfloat16(), seq, pos), (x.double(), seq, pos), (x[:, :128].contiguous(), seq, pos), (hidden(10, 1)[::2], seq, pos),
+              (x.T.contiguous().T, seq, pos), (x.cpu(), seq, pos), (x[0], seq, pos), (x, seq[:4], pos), (x, seq, pos[:4]),
+              (x, seq.long(), pos), (x, seq, pos.long()), (x, seq.cpu(), pos), (x, seq, torch.stack((pos, pos), 1)[:, 0])):
+        with pytest.raises(ValueError):
+            d.forward(*a)
+    assert torch.equal(d.pool.data, was)
+    assert torch.isfinite(d.forward(x, seq, pos)).all()
