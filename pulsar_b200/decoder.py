@@ -86,6 +86,8 @@ class Decoder:
         for t in (seq, pos):
             if t.shape != (T,) or t.dtype != torch.int32 or t.device != dev or not t.is_contiguous():
                 raise ValueError("Decoder: seq and pos are int32 [T], contiguous, beside the cache")
+        if T == 0:
+            return torch.empty_like(x)
         n, y = torch.empty_like(x), torch.empty_like(x)
         qkv = torch.empty((T, q + 2 * kv), dtype=torch.float32, device=dev)
         turned = torch.empty((T, s.n_head, s.head_dim), dtype=torch.float32, device=dev)

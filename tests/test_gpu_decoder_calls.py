@@ -115,3 +115,15 @@ def test_refusals(make):
             d.forward(*a)
     assert torch.equal(d.pool.data, was)
     assert torch.isfinite(d.forward(x, seq, pos)).all()
+
+
+def test_no_tokens(make):
+    """a step in which no sequence has a new token"""
+    d = make()
+    d.forward(hidden(5, 1), *d.extend([1], [5]))
+    was = d.pool.data.clone()
+    for rows, n_new in (([], []), ([1, 2], [0, 0])):
+        seq, pos = d.extend(rows, n_new)
+        assert d.forward(hidden(0, 1), seq, pos).shape == (0, 256)
+    d.pool.check()
+    assert d.pool.lens.tolist() == [0, 5, 0, 0, 0, 0] and torch.equal(d.pool.data, was)
