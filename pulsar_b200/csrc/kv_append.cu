@@ -15,7 +15,7 @@
  * and reads a token's angles once for its heads; where there are too few
  * tokens for that, HU = 1 spreads a token wider.  Measured: 8 x 2048 tokens of
  * 64 + 8 + 8 f16 heads of 128, interleaved: 122 to 127 us, 5.5 TB/s (with one 16-byte
- * run a thread 211 us: too few loads in flight); one token: 2.1 us. */
+ * run a thread 211 us: too few loads in flight); one token: 2.2 us. */
 #include "pk_common.h"
 
 struct pk_append_geo {

@@ -13,7 +13,7 @@
  * lengths, marks and counts one behind the other).  Measured on the device:
  * compaction of 128 sequences, 335 MB read and written, 66 us (53 of them the
  * copies, 6.2 TB/s); fork of 32 x 8 beams with 63 MB of copies, and growth,
- * 23 us; of 2 x 4 beams 12 us. */
+ * 22 us; of 2 x 4 beams 13 us. */
 #include "pk_common.h"
 
 __device__ uint32_t pk_err_word_dev;

@@ -37,9 +37,10 @@
  *   16 rows high anyway, so the second part costs nothing.
  *   R = 2: 16 query rows a tile, one product per part.
  * Two f16 parts hold 22 bits (q's rows and p are first scaled by a power of
- * two, so that nothing of weight falls among f16's subnormals), two bf16 parts
- * 16; QP = 3 adds a third where a bf16 cache meets wider q, so that f32
- * results are f32 results.  QP = 1: q has the cache's type or fewer bits. */
+ * two, so that nothing of weight falls among f16's subnormals: weights are lost
+ * below 2^-32 of the row's largest), two bf16 parts 16, which is more than
+ * their bf16 results have; QP = 3 adds a third where a bf16 cache meets wider q,
+ * so that f32 results are f32 results.  QP = 1: q has the cache's type or fewer bits. */
 #pragma once
 #include "pk_common.h"
 

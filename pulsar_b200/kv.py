@@ -2,12 +2,13 @@
 over the pages, and the pages' bookkeeping (include/pulsar_kv.h).
 
 PagedKv is one layer's cache (append, attend), KvPool a whole cache's pages
-shared by its layers (grow, fork, free, compact), RopeTable the angles.  All
-work on preallocated torch CUDA tensors as the caller's device buffers, on
-the current stream unless one is given; nothing allocates per call once a
-workspace has its size, and nothing synchronises except check().  A refused
-call raises KernelError.  What the device finds out of range (a page id, a
-length) it does not follow; kv_error() tells and clears.
+shared by its layers (grow, fork, free, compact), rope_table() the angles.
+All work on preallocated torch CUDA tensors as the caller's device buffers, on
+the current stream unless one is given; the objects make their buffers when
+they are made, no call allocates, and none synchronises but check() and
+kv_error().  Tensors of the wrong kind raise ValueError, what the library
+refuses KernelError.  What the device finds out of range (a page id, a length)
+it does not follow; kv_error() tells and clears.
 """
 from __future__ import annotations
 
