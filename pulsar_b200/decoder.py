@@ -84,7 +84,7 @@ class Decoder:
         if x.shape != (T, h) or x.dtype != torch.float32 or dev != self.pool.device or not x.is_contiguous():
             raise ValueError(f"Decoder: x is f32 [T][{h}], contiguous, beside the cache")
         for t in (seq, pos):
-            if t.shape != (T,) or t.dtype != torch.int32 or t.device != dev or not t.is_contiguous():
+            if t.numel() != T or t.dtype != torch.int32 or t.device != dev or not t.is_contiguous():
                 raise ValueError("Decoder: seq and pos are int32 [T], contiguous, beside the cache")
         if T == 0:
             return torch.empty_like(x)

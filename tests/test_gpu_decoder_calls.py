@@ -114,7 +114,8 @@ def test_refusals(make):
         with pytest.raises(ValueError):
             d.forward(*a)
     assert torch.equal(d.pool.data, was)
-    assert torch.isfinite(d.forward(x, seq, pos)).all()
+    a, b = d.forward(x, seq, pos), d.forward(x, seq.view(5, 1), pos.view(1, 5))
+    assert torch.isfinite(a).all() and torch.equal(a, b)
 
 
 def test_no_tokens(make):
